@@ -18,7 +18,7 @@ GAT_OK = 0
 GAT_EINVAL = -1
 GAT_EUNSUPPORTED = -2
 GAT_EWORKSPACE = -3
-GAT_ABI_VERSION = 12
+GAT_ABI_VERSION = 13
 GAT_HINT_LOCAL = 1 << 30  # OR'd into edges_per_row_hint (include/gat_amd.h)
 GAT_HINT_SHORT = 1 << 29  # every row < 1024 in-edges (include/gat_amd.h, ABI 11)
 GAT_SEG_LOAD = 1
@@ -29,6 +29,9 @@ GAT_ACT_LEAKY_RELU = 0
 GAT_ACT_LOG_SIGMOID = 1
 GAT_ACT_TANH = 2
 GAT_ACT_HEAD_SOFTMAX = 3
+GAT_F32 = 0
+GAT_BF16 = 1
+GAT_F16 = 2
 
 _c_int, _c_ll, _c_float, _c_vp = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
 _c_size_p = ctypes.POINTER(ctypes.c_size_t)
@@ -117,6 +120,17 @@ SIGNATURES = {
     "gat_src_backward": (_c_int, [_c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_vp, _c_vp,
                                   _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_int,
                                   _c_vp, _c_vp, _c_int, _c_vp]),
+    "gat_layer_norm": (_c_int, [_c_vp, _c_ll, _c_int, _c_int, _c_vp, _c_vp, _c_float, _c_vp,
+                                _c_ll, _c_vp, _c_int, _c_vp]),
+    "gat_layer_norm_backward_workspace_size": (_c_int, [_c_int, _c_int, _c_int, _c_size_p]),
+    "gat_layer_norm_backward": (_c_int, [_c_vp, _c_ll, _c_vp, _c_ll, _c_int, _c_int, _c_vp,
+                                         _c_vp, _c_vp, _c_ll, _c_vp, _c_vp, _c_vp,
+                                         ctypes.c_size_t, _c_int, _c_vp]),
+    "gat_embedding": (_c_int, [_c_vp, _c_int, _c_ll, _c_vp, _c_ll, _c_int, _c_int, _c_float,
+                               _c_vp, _c_ll, _c_int, _c_vp]),
+    "gat_embedding_grad_workspace_size": (_c_int, [_c_ll, _c_int, _c_int, _c_size_p]),
+    "gat_embedding_grad": (_c_int, [_c_vp, _c_int, _c_ll, _c_vp, _c_ll, _c_int, _c_int, _c_float,
+                                    _c_ll, _c_vp, _c_ll, _c_vp, ctypes.c_size_t, _c_int, _c_vp]),
 }
 
 _lock = threading.Lock()
@@ -228,3 +242,19 @@ def project_workspace_bytes(fin: int, heads: int, f: int) -> int:
     check(load().gat_project_workspace_size(fin, heads, f, ctypes.byref(n)),
           "gat_project_workspace_size")
     return int(n.value)
+
+
+@functools.lru_cache(maxsize=256)  # pure function of the shape
+def layer_norm_workspace_size(rows: int, cols: int, dtype: int) -> int:
+    out = ctypes.c_size_t()
+    check(load().gat_layer_norm_backward_workspace_size(rows, cols, dtype, ctypes.byref(out)),
+          "gat_layer_norm_backward_workspace_size")
+    return out.value
+
+
+@functools.lru_cache(maxsize=256)  # pure function of the shape
+def embedding_grad_workspace_size(tokens: int, vocab: int, cols: int) -> int:
+    out = ctypes.c_size_t()
+    check(load().gat_embedding_grad_workspace_size(tokens, vocab, cols, ctypes.byref(out)),
+          "gat_embedding_grad_workspace_size")
+    return out.value

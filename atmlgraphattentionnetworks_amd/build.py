@@ -1,11 +1,10 @@
 """In-tree build of libgat_amd.so for gfx950 (no JIT cache: the .so travels
 with the repo snapshot to the GPU box).
 
-The library is five HIP translation units (csrc/*.hip, sharing
-csrc/gat_common.h); each compiles to an object under build/obj in its own
-hipcc process, in parallel, and one link makes the shared library.  Objects
-are rebuilt when their source, the shared header or include/gat_amd.h is
-newer.
+The library is one HIP translation unit per csrc/*.hip (sharing csrc/*.h);
+each compiles to an object under build/obj in its own hipcc process, in
+parallel, and one link makes the shared library.  Objects are rebuilt when
+their source, a shared header or include/gat_amd.h is newer.
 
     python -m atmlgraphattentionnetworks_amd.build [--force]
 """
@@ -20,13 +19,16 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 SRCS = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
-COMMON = os.path.join(CSRC, "gat_common.h")
+HEADERS = sorted(glob.glob(os.path.join(CSRC, "*.h")))
 HDR = os.path.join(ROOT, "include", "gat_amd.h")
 OBJ = os.path.join(ROOT, "build", "obj")
 LIB = os.path.join(PKG, "libgat_amd.so")
 ARCH = os.environ.get("GAT_OFFLOAD_ARCH", "gfx950")
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
-         "-munsafe-fp-atomics"]
+         "-munsafe-fp-atomics",
+         # no packed float32 instructions: some of their forms have given wrong
+         # results on this hardware (the host pass warns about the unknown feature)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # GAT_AB_KERNELS=1: a tools-only build that also carries the measured-slower
 # kernels kept for A/B (the fp32-MFMA k_project_pipe2 behind GAT_PROJ_X3=0);
 # the product library never defines it.  Use --force when switching.
@@ -52,7 +54,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
     for src in SRCS:
         obj = os.path.join(OBJ, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
-        if force or _stale(obj, [src, COMMON, HDR]):
+        if force or _stale(obj, [src, *HEADERS, HDR]):
             cmd = [hipcc(), f"--offload-arch={ARCH}", *FLAGS, "-c", "-o", obj + ".tmp", src]
             if verbose:
                 print("[build]", " ".join(cmd), flush=True)

@@ -1,0 +1,494 @@
+// Embedding lookup with a scale, and the gradient of its table (gat_embedding,
+// gat_embedding_grad).
+//
+//   y[t] = scale * w[ids[t]]          dw[v] = scale * sum over t with ids[t] = v of g[t]
+//
+// Bound: memory.  The lookup reads a row and writes a row per token; the gradient has
+// to read g once and write the whole table once.
+//
+// Gradient: the tokens are sorted by id (stable, so each id's tokens stay in order) and
+// each table row is then one sum over its tokens' rows of g, written once, zeros
+// included: no atomics and no separate clearing pass, and the result does not depend on
+// timing.  An id with more than kPiece tokens would keep one row's lanes busy long after
+// the rest: the sorted order is cut into pieces of kPiece tokens, the pieces of such an
+// id are summed by workgroups of their own, and the partial sums are joined in order.
+// Sums are float32 and rounded once, after the scale.
+//
+// Sort: least significant digit first, 8 bits a pass, over (id, token) pairs; an id that
+// takes no gradient (out of range, or the padding id) sorts behind the table as id
+// `vocab`.  A pass is two launches: digit counts per workgroup, then every workgroup
+// adds up the counts before its own and writes its pairs in order.  The workgroups are
+// limited to 256 so that this sum stays short.
+
+#include "gat_seq.h"
+
+namespace {
+
+constexpr int kSortBlock = 256;  // one thread per digit in the sums
+constexpr int kSortMinItems = 1024;
+constexpr int kSortMaxBlocks = 256;
+constexpr int kPiece = 128;
+constexpr long long kMaxTokens = 1ll << 30;
+constexpr int kEmbedBlock = 256;
+
+struct Ids {
+    const void* ids;
+    int is64;
+    long long padding;  // an id without a gradient, or -1
+    int vocab;
+};
+
+__device__ __forceinline__ long long id_at(const Ids& s, long long t) {
+    return s.is64 ? static_cast<const long long*>(s.ids)[t]
+                  : (long long)static_cast<const int*>(s.ids)[t];
+}
+
+__device__ __forceinline__ unsigned key_at(const Ids& s, long long t) {
+    const long long id = id_at(s, t);
+    return id >= 0 && id < s.vocab && id != s.padding ? (unsigned)id : (unsigned)s.vocab;
+}
+
+// ---------------------------------------------------------------------------
+// Lookup: LPR lanes per token, 16 bytes a lane and step.
+// ---------------------------------------------------------------------------
+template <typename T, int LPR>
+__global__ __launch_bounds__(kEmbedBlock) void k_embed(Ids s, long long tokens, const T* w,
+                                                       long long ld_w, int cols, float scale,
+                                                       T* out, long long ld_out, int whole) {
+    constexpr int N = Vec16<T>::N;
+    constexpr int TPB = kEmbedBlock / LPR;
+    const int lane = threadIdx.x % LPR;
+    for (long long t = (long long)blockIdx.x * TPB + threadIdx.x / LPR; t < tokens;
+         t += (long long)gridDim.x * TPB) {
+        const long long id = id_at(s, t);
+        const bool in = id >= 0 && id < s.vocab;
+        const T* row = w + (in ? id : 0) * ld_w;
+        const float f = in ? scale : NAN;  // an id outside the table shows
+        T* to = out + t * ld_out;
+        for (int c = lane * N; c < cols; c += LPR * N) {
+            typename Vec16<T>::type v = load_vec<T>(row, c, in ? cols : 0, whole), y;
+#pragma unroll
+            for (int e = 0; e < N; ++e) y[e] = (T)((float)v[e] * f);
+            store_vec<T>(to, c, cols, whole, y);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Sort
+// ---------------------------------------------------------------------------
+template <bool FIRST>
+__global__ __launch_bounds__(kSortBlock) void k_sort_count(Ids s, const unsigned* keys, int n,
+                                                           int per, int shift, unsigned* counts) {
+    __shared__ unsigned h[256];
+    h[threadIdx.x] = 0;
+    __syncthreads();
+    const int a = blockIdx.x * per, e = a + per < n ? a + per : n;
+    for (int i = a + threadIdx.x; i < e; i += kSortBlock) {
+        const unsigned k = FIRST ? key_at(s, i) : keys[i];
+        atomicAdd(&h[(k >> shift) & 255], 1u);
+    }
+    __syncthreads();
+    counts[blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(kSortBlock) void k_sort_place(Ids s, const unsigned* keys,
+                                                           const unsigned* toks, int n, int per,
+                                                           int shift, const unsigned* counts,
+                                                           unsigned* keys_out, unsigned* toks_out) {
+    __shared__ unsigned base[256], wave_count[4][256], scan[256];
+    const int d = threadIdx.x, lane = d % kWave, wave = d / kWave;
+    unsigned before = 0, total = 0;  // of digit d: in the workgroups before, in all
+#pragma unroll 8
+    for (int b = 0; b < (int)gridDim.x; ++b) {
+        const unsigned c = counts[b * 256 + d];
+        before += b < (int)blockIdx.x ? c : 0;
+        total += c;
+    }
+    scan[d] = total;
+    __syncthreads();
+    for (int off = 1; off < 256; off <<= 1) {
+        const unsigned v = d >= off ? scan[d - off] : 0;
+        __syncthreads();
+        scan[d] += v;
+        __syncthreads();
+    }
+    base[d] = scan[d] - total + before;
+    const int a = blockIdx.x * per, e = a + per < n ? a + per : n;
+    for (int i0 = a; i0 < e; i0 += kSortBlock) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) wave_count[k][d] = 0;
+        __syncthreads();
+        const int i = i0 + d;
+        const bool in = i < e;
+        const unsigned key = in ? (FIRST ? key_at(s, i) : keys[i]) : 0;
+        const unsigned digit = (key >> shift) & 255;
+        // the lanes of this wave with the same digit
+        unsigned long long same = __ballot(in);
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            const unsigned long long m = __ballot((digit >> b) & 1);
+            same &= (digit >> b) & 1 ? m : ~m;
+        }
+        const unsigned rank = __popcll(same & ((1ull << lane) - 1));
+        if (in && rank == 0) wave_count[wave][digit] = __popcll(same);
+        __syncthreads();
+        if (in) {
+            unsigned at = base[digit] + rank;
+            for (int k = 0; k < wave; ++k) at += wave_count[k][digit];
+            keys_out[at] = key;
+            toks_out[at] = FIRST ? (unsigned)i : toks[i];
+        }
+        __syncthreads();
+        base[d] += wave_count[0][d] + wave_count[1][d] + wave_count[2][d] + wave_count[3][d];
+    }
+}
+
+// first[v] = position of the first sorted token with id >= v, for v in [0, vocab].
+// A lane writes the ids between its token's and the one before; a wide gap is shared
+// by the wave.
+__global__ __launch_bounds__(256) void k_sort_firsts(const unsigned* keys, int n, int vocab,
+                                                     int* first) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    const int lane = threadIdx.x % kWave;
+    int lo = 0, hi = -1;  // first[lo .. hi] = i
+    if (i <= n) {
+        lo = i > 0 ? (int)keys[i - 1] + 1 : 0;
+        hi = i < n ? (int)keys[i] : vocab;
+    }
+    const bool wide = hi - lo >= 16;
+    if (!wide)
+        for (int v = lo; v <= hi; ++v) first[v] = i;
+    for (unsigned long long m = __ballot(wide); m != 0; m &= m - 1) {
+        const int l = __ffsll((long long)m) - 1;
+        const int a = __shfl(lo, l), b = __shfl(hi, l), at = __shfl(i, l);
+        for (int v = a + lane; v <= b; v += kWave) first[v] = at;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Sums
+// ---------------------------------------------------------------------------
+
+// acc += the rows of g of sorted tokens [a, e), `step` apart, columns [c, c + N)
+template <typename T>
+__device__ __forceinline__ void add_rows(float (&acc)[Vec16<T>::N], const T* g, long long ld_g,
+                                         const unsigned* toks, int a, int e, int step, int c,
+                                         int cols, bool whole) {
+    constexpr int N = Vec16<T>::N, U = 4;
+    int i = a;
+    for (; i + (U - 1) * step < e; i += U * step) {
+        typename Vec16<T>::type v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            v[u] = load_vec<T>(g + (long long)toks[i + u * step] * ld_g, c, cols, whole);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k] += (float)v[u][k];
+    }
+    for (; i < e; i += step) {
+        const typename Vec16<T>::type v =
+            load_vec<T>(g + (long long)toks[i] * ld_g, c, cols, whole);
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += (float)v[k];
+    }
+}
+
+// acc of the workgroup's groups added up in order into group 0's
+template <int N, int LPR>
+__device__ __forceinline__ void join_groups(float (&acc)[N], float* lds) {
+    constexpr int G = kEmbedBlock / LPR;
+    const int lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+    if constexpr (G > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) lds[(grp * N + k) * LPR + lane] = acc[k];
+        __syncthreads();
+        if (grp == 0)
+            for (int j = 1; j < G; ++j)
+#pragma unroll
+                for (int k = 0; k < N; ++k) acc[k] += lds[(j * N + k) * LPR + lane];
+    }
+}
+
+// Piece j's partial sums, part[2 j + slot]: slot 0 the id that the piece begins with,
+// slot 1 the one that it ends with, where that id has more than kPiece tokens.
+template <typename T, int LPR>
+__global__ __launch_bounds__(kEmbedBlock) void k_embed_pieces(
+    const unsigned* keys, const unsigned* toks, const int* first, int n, int vocab, const T* g,
+    long long ld_g, int cols, int whole, float* part) {
+    constexpr int N = Vec16<T>::N;
+    __shared__ float lds[kEmbedBlock * N];
+    const int j = blockIdx.x >> 1, slot = blockIdx.x & 1;
+    const int a = j * kPiece, e = a + kPiece < n ? a + kPiece : n;
+    const unsigned head = keys[a], id = slot == 0 ? head : keys[e - 1];
+    if (id >= (unsigned)vocab || (slot == 1 && id == head)) return;
+    const int f = first[id], l = first[id + 1];
+    if (l - f <= kPiece) return;
+    const int from = f > a ? f : a, to = l < e ? l : e;
+    const int lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+    const int c = (blockIdx.y * LPR + lane) * N;
+    float acc[N] = {};
+    if (c < cols)
+        add_rows<T>(acc, g, ld_g, toks, from + grp, to, kEmbedBlock / LPR, c, cols, whole);
+    join_groups<N, LPR>(acc, lds);
+    if (grp == 0) {
+        float* p = part + (size_t)blockIdx.x * cols;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (c + k < cols) p[c + k] = acc[k];
+    }
+}
+
+// Table rows of ids with more than kPiece tokens: piece j's workgroup takes the one whose
+// tokens begin in it, if there is one.
+template <typename T, int LPR>
+__global__ __launch_bounds__(kEmbedBlock) void k_embed_join(const unsigned* keys, const int* first,
+                                                            int n, int vocab, int cols,
+                                                            const float* part, float scale, T* dw,
+                                                            long long ld_dw, int whole) {
+    constexpr int N = Vec16<T>::N;
+    __shared__ float lds[kEmbedBlock * N];
+    const int j = blockIdx.x;
+    const int a = j * kPiece, e = a + kPiece < n ? a + kPiece : n;
+    const unsigned id = keys[e - 1];
+    if (id >= (unsigned)vocab) return;
+    const int f = first[id], l = first[id + 1];
+    if (l - f <= kPiece || f < a) return;
+    const int lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+    const int c = (blockIdx.y * LPR + lane) * N;
+    const int last = (l - 1) / kPiece;
+    float acc[N] = {};
+    if (c < cols) {
+#pragma unroll 2
+        for (int p = j + grp; p <= last; p += kEmbedBlock / LPR) {
+            const float* row = part + (size_t)(2 * p + (p == j && f != a ? 1 : 0)) * cols;
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k] += c + k < cols ? row[c + k] : 0.f;
+        }
+    }
+    join_groups<N, LPR>(acc, lds);
+    if (grp == 0 && c < cols) {
+        typename Vec16<T>::type y;
+#pragma unroll
+        for (int k = 0; k < N; ++k) y[k] = (T)(acc[k] * scale);
+        store_vec<T>(dw + (long long)id * ld_dw, c, cols, whole, y);
+    }
+}
+
+// All other table rows, those of ids without a token too.
+template <typename T, int LPR>
+__global__ __launch_bounds__(kEmbedBlock) void k_embed_rows(const unsigned* toks, const int* first,
+                                                            int vocab, const T* g, long long ld_g,
+                                                            int whole_g, int cols, float scale,
+                                                            T* dw, long long ld_dw, int whole) {
+    constexpr int N = Vec16<T>::N;
+    const int lane = threadIdx.x % LPR;
+    const int v = blockIdx.x * (kEmbedBlock / LPR) + threadIdx.x / LPR;
+    if (v >= vocab) return;
+    const int a = first[v], e = first[v + 1];
+    if (e - a > kPiece) return;
+    for (int c = lane * N; c < cols; c += LPR * N) {
+        float acc[N] = {};
+        add_rows<T>(acc, g, ld_g, toks, a, e, 1, c, cols, whole_g);
+        typename Vec16<T>::type y;
+#pragma unroll
+        for (int k = 0; k < N; ++k) y[k] = (T)(acc[k] * scale);
+        store_vec<T>(dw + (long long)v * ld_dw, c, cols, whole, y);
+    }
+}
+
+// lanes per row: the power of two in [8, 64] that covers it, if one does
+inline int embed_lanes(int cols, int dtype) {
+    const int n = 16 / (int)dtype_size(dtype);
+    const int vecs = (cols + n - 1) / n;
+    return vecs <= 8 ? 8 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : 64;
+}
+
+inline bool rows_whole(const void* p, long long ld, int dtype) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((uintptr_t)ld * dtype_size(dtype) & 15) == 0;
+}
+
+struct SortPlan {
+    int per, blocks, passes;
+};
+inline SortPlan sort_plan(int n, int vocab) {
+    SortPlan s;
+    s.per = (n + kSortMaxBlocks - 1) / kSortMaxBlocks;
+    if (s.per < kSortMinItems) s.per = kSortMinItems;
+    s.blocks = (n + s.per - 1) / s.per;
+    int bits = 0;
+    while (bits < 32 && ((unsigned)vocab >> bits) != 0) ++bits;
+    s.passes = (bits + 7) / 8;
+    return s;
+}
+
+// Workspace: two sets of (key, token) arrays, the digit counts, first[], the pieces'
+// partial sums.
+struct GradLayout {
+    size_t keys[2], toks[2], counts, first, part, bytes;
+};
+inline GradLayout grad_layout(int n, int vocab, int cols) {
+    GradLayout l;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += align_up(bytes);
+        return here;
+    };
+    for (int k = 0; k < 2; ++k) {
+        l.keys[k] = take((size_t)n * 4);
+        l.toks[k] = take((size_t)n * 4);
+    }
+    l.counts = take((size_t)kSortMaxBlocks * 256 * 4);
+    l.first = take(((size_t)vocab + 1) * 4);
+    l.part = take(((size_t)n + kPiece - 1) / kPiece * 2 * cols * 4);
+    l.bytes = at;
+    return l;
+}
+
+template <typename T, int LPR>
+int embed_grad_sums(const unsigned* keys, const unsigned* toks, const int* first, int n, int vocab,
+                    const T* g, long long ld_g, int cols, float scale, float* part, T* dw,
+                    long long ld_dw, int dtype, hipStream_t s) {
+    constexpr int N = Vec16<T>::N;
+    const int whole_g = rows_whole(g, ld_g, dtype), whole = rows_whole(dw, ld_dw, dtype);
+    const int slabs = (cols + LPR * N - 1) / (LPR * N);
+    if (n > kPiece) {
+        const int pieces = (n + kPiece - 1) / kPiece;
+        k_embed_pieces<T, LPR><<<dim3(2 * pieces, slabs), kEmbedBlock, 0, s>>>(
+            keys, toks, first, n, vocab, g, ld_g, cols, whole_g, part);
+        k_embed_join<T, LPR><<<dim3(pieces, slabs), kEmbedBlock, 0, s>>>(
+            keys, first, n, vocab, cols, part, scale, dw, ld_dw, whole);
+    }
+    constexpr int RPB = kEmbedBlock / LPR;
+    k_embed_rows<T, LPR><<<(vocab + RPB - 1) / RPB, kEmbedBlock, 0, s>>>(
+        toks, first, vocab, g, ld_g, whole_g, cols, scale, dw, ld_dw, whole);
+    return status_of(hipGetLastError());
+}
+
+template <typename T>
+int embed_grad_by_lanes(int lanes, const unsigned* keys, const unsigned* toks, const int* first,
+                        int n, int vocab, const void* g, long long ld_g, int cols, float scale,
+                        float* part, void* dw, long long ld_dw, int dtype, hipStream_t s) {
+    const T* gt = static_cast<const T*>(g);
+    T* dt = static_cast<T*>(dw);
+    auto call = [&](auto l) {
+        return embed_grad_sums<T, decltype(l)::value>(keys, toks, first, n, vocab, gt, ld_g, cols,
+                                                      scale, part, dt, ld_dw, dtype, s);
+    };
+    if (lanes == 8) return call(std::integral_constant<int, 8>());
+    if (lanes == 16) return call(std::integral_constant<int, 16>());
+    if (lanes == 32) return call(std::integral_constant<int, 32>());
+    return call(std::integral_constant<int, 64>());
+}
+
+template <typename T>
+int embed_by_lanes(int lanes, const Ids& ids, long long tokens, const void* w, long long ld_w,
+                   int cols, float scale, void* out, long long ld_out, int dtype, hipStream_t s) {
+    const int whole = rows_whole(w, ld_w, dtype) && rows_whole(out, ld_out, dtype);
+    auto call = [&](auto l) {
+        constexpr int L = decltype(l)::value;
+        const int grid = grid_for(tokens, kEmbedBlock / L, 256 * 32);
+        k_embed<T, L><<<grid, kEmbedBlock, 0, s>>>(ids, tokens, static_cast<const T*>(w), ld_w,
+                                                   cols, scale, static_cast<T*>(out), ld_out, whole);
+        return status_of(hipGetLastError());
+    };
+    if (lanes == 8) return call(std::integral_constant<int, 8>());
+    if (lanes == 16) return call(std::integral_constant<int, 16>());
+    if (lanes == 32) return call(std::integral_constant<int, 32>());
+    return call(std::integral_constant<int, 64>());
+}
+
+inline bool ids_fit(const void* ids, int ids64, long long tokens) {
+    return tokens == 0 ||
+           (ids != nullptr && (reinterpret_cast<uintptr_t>(ids) & (ids64 ? 7 : 3)) == 0);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gat_embedding(const void* ids, int ids64, long long tokens, const void* w, long long ld_w,
+                  int vocab, int cols, float scale, void* out, long long ld_out, int dtype,
+                  void* stream) {
+    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || cols <= 0 || !known_dtype(dtype) ||
+        ld_w < cols || ld_out < cols || !ids_fit(ids, ids64, tokens))
+        return GAT_EINVAL;
+    if (tokens == 0) return GAT_OK;
+    if (w == nullptr || out == nullptr || !element_aligned(w, dtype) || !element_aligned(out, dtype))
+        return GAT_EINVAL;
+    const Ids s{ids, ids64, -1, vocab};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int lanes = embed_lanes(cols, dtype);
+    if (dtype == GAT_F32)
+        return embed_by_lanes<float>(lanes, s, tokens, w, ld_w, cols, scale, out, ld_out, dtype, st);
+    if (dtype == GAT_BF16)
+        return embed_by_lanes<bf16>(lanes, s, tokens, w, ld_w, cols, scale, out, ld_out, dtype, st);
+    return embed_by_lanes<f16>(lanes, s, tokens, w, ld_w, cols, scale, out, ld_out, dtype, st);
+}
+
+int gat_embedding_grad_workspace_size(long long tokens, int vocab, int cols, size_t* bytes) {
+    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || cols <= 0 || bytes == nullptr)
+        return GAT_EINVAL;
+    *bytes = grad_layout((int)tokens, vocab, cols).bytes;
+    return GAT_OK;
+}
+
+int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void* g, long long ld_g,
+                       int vocab, int cols, float scale, long long padding, void* dw,
+                       long long ld_dw, void* workspace, size_t workspace_bytes, int dtype,
+                       void* stream) {
+    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || cols <= 0 || !known_dtype(dtype) ||
+        ld_g < 0 || ld_dw < cols || dw == nullptr || !element_aligned(dw, dtype) ||
+        !ids_fit(ids, ids64, tokens) ||
+        (tokens > 0 && (g == nullptr || !element_aligned(g, dtype))))
+        return GAT_EINVAL;
+    const int n = (int)tokens;
+    const GradLayout l = grad_layout(n, vocab, cols);
+    if (workspace == nullptr || workspace_bytes < l.bytes) return GAT_EWORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return GAT_EINVAL;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    unsigned* keys[2] = {reinterpret_cast<unsigned*>(ws + l.keys[0]),
+                         reinterpret_cast<unsigned*>(ws + l.keys[1])};
+    unsigned* toks[2] = {reinterpret_cast<unsigned*>(ws + l.toks[0]),
+                         reinterpret_cast<unsigned*>(ws + l.toks[1])};
+    unsigned* counts = reinterpret_cast<unsigned*>(ws + l.counts);
+    int* first = reinterpret_cast<int*>(ws + l.first);
+    float* part = reinterpret_cast<float*>(ws + l.part);
+    const Ids s{ids, ids64, padding, vocab};
+    int cur = 0;
+    if (n > 0) {
+        const SortPlan p = sort_plan(n, vocab);
+        for (int k = 0; k < p.passes; ++k) {
+            const int shift = 8 * k;
+            if (k == 0) {
+                k_sort_count<true><<<p.blocks, kSortBlock, 0, st>>>(s, nullptr, n, p.per, shift, counts);
+                k_sort_place<true><<<p.blocks, kSortBlock, 0, st>>>(s, nullptr, nullptr, n, p.per, shift,
+                                                                    counts, keys[0], toks[0]);
+            } else {
+                k_sort_count<false><<<p.blocks, kSortBlock, 0, st>>>(s, keys[cur], n, p.per, shift,
+                                                                     counts);
+                k_sort_place<false><<<p.blocks, kSortBlock, 0, st>>>(s, keys[cur], toks[cur], n, p.per,
+                                                                     shift, counts, keys[cur ^ 1],
+                                                                     toks[cur ^ 1]);
+                cur ^= 1;
+            }
+        }
+    }
+    k_sort_firsts<<<n / 256 + 1, 256, 0, st>>>(keys[cur], n, vocab, first);
+    const int lanes = embed_lanes(cols, dtype);
+    if (dtype == GAT_F32)
+        return embed_grad_by_lanes<float>(lanes, keys[cur], toks[cur], first, n, vocab, g, ld_g, cols,
+                                          scale, part, dw, ld_dw, dtype, st);
+    if (dtype == GAT_BF16)
+        return embed_grad_by_lanes<bf16>(lanes, keys[cur], toks[cur], first, n, vocab, g, ld_g, cols,
+                                         scale, part, dw, ld_dw, dtype, st);
+    return embed_grad_by_lanes<f16>(lanes, keys[cur], toks[cur], first, n, vocab, g, ld_g, cols, scale,
+                                    part, dw, ld_dw, dtype, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,440 @@
+// Layer norm over the last dimension, forward and backward (gat_layer_norm,
+// gat_layer_norm_backward).
+//
+//   m = mean(x)   v = mean((x - m)^2)   r = 1 / sqrt(v + eps)   z = (x - m) r
+//   y = z w + b
+//   h = g w       dx = r (h - mean(h) - z mean(h z))
+//   dw = sum over rows of g z            db = sum over rows of g
+//
+// Bound: memory.  The forward has to read x and write y, the backward to read x
+// and g and write dx, so each is one pass: a row is held in registers (as it is
+// stored, 16 bytes a vector) between the sums and the output, and the variance is
+// the mean of the squared deviations, not a difference of two large sums.
+//
+// A row belongs to LPR lanes (8 to 64 lanes of a wave, or a whole workgroup of 256
+// for rows over 64 * 4 vectors) with NV vectors each; the groups walk the rows with
+// a stride that is a multiple of 8 rows, so a group's rows all start at the same
+// offset from a 16-byte boundary and a lane keeps the same columns: w, b and the
+// sums of dw and db stay in registers over the group's rows, also where the row
+// length is odd.
+//
+// dw and db: per-lane float32 sums over the group's rows, added up over the
+// workgroup's groups in LDS, one partial row per workgroup; k_norm_columns adds
+// those up in a fixed order.  No atomics: the result depends on the shape alone.
+
+#include "gat_seq.h"
+
+namespace {
+
+constexpr int kNormBlock = 256;
+
+struct NormArgs {
+    const void* x;
+    const void* g;  // backward: the incoming gradient
+    void* out;      // forward: y, backward: dx
+    const void* w;  // may be null (1)
+    const void* b;  // may be null (0)
+    float* stats;   // [rows, 2] mean, r; forward: may be null
+    float* part;    // backward: [workgroups, 2, cols], may be null
+    long long ld_x, ld_g, ld_out;
+    int rows, cols;
+    float eps;
+    int whole_g, whole_out;  // the tensor's rows have x's offset from a 16-byte boundary
+};
+
+// Sums of two values over the LPR lanes that share a row, given to all of them.
+// `red`: LDS for LPR = 256, a slot of its own per call of the row loop's parity.
+template <int LPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2]) {
+    constexpr int W = LPR < kWave ? LPR : kWave;
+#pragma unroll
+    for (int off = 1; off < W; off <<= 1) {
+        a += __shfl_xor(a, off);
+        b += __shfl_xor(b, off);
+    }
+    if constexpr (LPR > kWave) {
+        const int wave = threadIdx.x / kWave;
+        if (threadIdx.x % kWave == 0) {
+            red[wave][0] = a;
+            red[wave][1] = b;
+        }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int k = 0; k < LPR / kWave; ++k) {
+            a += red[k][0];
+            b += red[k][1];
+        }
+    }
+}
+
+template <typename T, int LPR, int NV>
+__global__ __launch_bounds__(kNormBlock) void k_norm_fwd(NormArgs p) {
+    constexpr int N = Vec16<T>::N;
+    constexpr int RPB = kNormBlock / LPR;
+    typedef typename Vec16<T>::type V;
+    __shared__ float red[4][4][2];
+    const int lane = threadIdx.x % LPR;
+    const int group = blockIdx.x * RPB + threadIdx.x / LPR;
+    const int groups = gridDim.x * RPB;
+    const T* x = static_cast<const T*>(p.x);
+    const int phase = phase_of(x + (long long)group * p.ld_x);
+    float w[NV][N], b[NV][N];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int c = (i * LPR + lane) * N - phase + e;
+            const bool in = c >= 0 && c < p.cols;
+            w[i][e] = in ? (p.w != nullptr ? (float)static_cast<const T*>(p.w)[c] : 1.f) : 0.f;
+            b[i][e] = in && p.b != nullptr ? (float)static_cast<const T*>(p.b)[c] : 0.f;
+        }
+    const float inv = 1.f / (float)p.cols;
+    int turn = 0;
+    // groups of one workgroup leave together where they meet at barriers (LPR = 256)
+    for (long long row = group; row < p.rows; row += groups, turn ^= 2) {
+        const T* xr = x + row * p.ld_x;
+        V v[NV];
+        float s = 0.f, unused = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            v[i] = load_vec<T>(xr, (i * LPR + lane) * N - phase, p.cols, true);
+#pragma unroll
+            for (int e = 0; e < N; ++e) s += (float)v[i][e];
+        }
+        row_sum2<LPR>(s, unused, red[turn]);
+        const float mean = s * inv;
+        float q = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int c = (i * LPR + lane) * N - phase + e;
+                const float d = (float)v[i][e] - mean;
+                q += c >= 0 && c < p.cols ? d * d : 0.f;
+            }
+        row_sum2<LPR>(q, unused, red[turn + 1]);
+        const float r = 1.f / sqrtf(q * inv + p.eps);
+        if (p.stats != nullptr && lane == 0) {
+            p.stats[2 * row] = mean;
+            p.stats[2 * row + 1] = r;
+        }
+        T* yr = static_cast<T*>(p.out) + row * p.ld_out;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            V y;
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                y[e] = (T)(((float)v[i][e] - mean) * r * w[i][e] + b[i][e]);
+            store_vec<T>(yr, (i * LPR + lane) * N - phase, p.cols, p.whole_out, y);
+        }
+    }
+}
+
+template <typename T, int LPR, int NV>
+__global__ __launch_bounds__(kNormBlock) void k_norm_bwd(NormArgs p) {
+    constexpr int N = Vec16<T>::N;
+    constexpr int RPB = kNormBlock / LPR;
+    typedef typename Vec16<T>::type V;
+    __shared__ float red[4][4][2];
+    constexpr int COLS = LPR * NV * N;
+    __shared__ float cs[RPB > 1 ? 2 * COLS : 1];
+    const int lane = threadIdx.x % LPR;
+    const int group = blockIdx.x * RPB + threadIdx.x / LPR;
+    const int groups = gridDim.x * RPB;
+    const T* x = static_cast<const T*>(p.x);
+    const int phase = phase_of(x + (long long)group * p.ld_x);
+    V w[NV];
+    float dw[NV][N], db[NV][N];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int c = (i * LPR + lane) * N - phase + e;
+            const bool in = c >= 0 && c < p.cols;
+            w[i][e] = in ? (p.w != nullptr ? static_cast<const T*>(p.w)[c] : (T)1.f) : (T)0.f;
+            dw[i][e] = db[i][e] = 0.f;
+        }
+    const float inv = 1.f / (float)p.cols;
+    int turn = 0;
+    for (long long row = group; row < p.rows; row += groups, turn ^= 1) {
+        const T* xr = x + row * p.ld_x;
+        const T* gr = static_cast<const T*>(p.g) + row * p.ld_g;
+        V v[NV], g[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c0 = (i * LPR + lane) * N - phase;
+            v[i] = load_vec<T>(xr, c0, p.cols, true);
+            g[i] = load_vec<T>(gr, c0, p.cols, p.whole_g);
+        }
+        const float mean = p.stats[2 * row], r = p.stats[2 * row + 1];
+        float sh = 0.f, shz = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                // outside the row g and w are 0, so nothing is added there
+                const float z = ((float)v[i][e] - mean) * r;
+                const float h = (float)g[i][e] * (float)w[i][e];
+                sh += h;
+                shz += h * z;
+                dw[i][e] += (float)g[i][e] * z;
+                db[i][e] += (float)g[i][e];
+            }
+        row_sum2<LPR>(sh, shz, red[turn]);
+        sh *= inv;
+        shz *= inv;
+        if (p.out != nullptr) {
+            T* dr = static_cast<T*>(p.out) + row * p.ld_out;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                V d;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float z = ((float)v[i][e] - mean) * r;
+                    d[e] = (T)(r * ((float)g[i][e] * (float)w[i][e] - sh - z * shz));
+                }
+                store_vec<T>(dr, (i * LPR + lane) * N - phase, p.cols, p.whole_out, d);
+            }
+        }
+    }
+    if (p.part == nullptr) return;
+    float* part = p.part + (size_t)blockIdx.x * 2 * p.cols;
+    if constexpr (RPB == 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int c = (i * LPR + lane) * N - phase + e;
+                if (c < 0 || c >= p.cols) continue;
+                part[c] = dw[i][e];
+                part[p.cols + c] = db[i][e];
+            }
+    } else {
+        // The groups' columns may be shifted against each other (odd row lengths), so
+        // they take turns: group j adds its sums to those of the groups before it.
+        for (int j = 0; j < RPB; ++j) {
+            if (threadIdx.x / LPR == j) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const int c = (i * LPR + lane) * N - phase + e;
+                        if (c < 0 || c >= p.cols) continue;
+                        cs[c] = (j == 0 ? 0.f : cs[c]) + dw[i][e];
+                        cs[COLS + c] = (j == 0 ? 0.f : cs[COLS + c]) + db[i][e];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < p.cols; c += kNormBlock) {
+            part[c] = cs[c];
+            part[p.cols + c] = cs[COLS + c];
+        }
+    }
+}
+
+// out[c] = sum over the partial rows, for the 2 * cols sums (dw, then db); 32 columns
+// by 32 strided partial chains a workgroup, joined in LDS in a fixed order.
+constexpr int kColsTile = 32;
+
+template <typename T>
+__global__ __launch_bounds__(1024) void k_norm_columns(const float* part, int parts, int cols,
+                                                       T* dw, T* db) {
+    __shared__ float s[32][kColsTile + 1];
+    const int c = blockIdx.x * kColsTile + threadIdx.x % kColsTile;
+    const int k = threadIdx.x / kColsTile;
+    float a = 0.f;
+    if (c < 2 * cols) {
+#pragma unroll 8
+        for (int j = k; j < parts; j += 32) a += part[(size_t)j * 2 * cols + c];
+    }
+    s[k][threadIdx.x % kColsTile] = a;
+    __syncthreads();
+    if (k != 0 || c >= 2 * cols) return;
+    a = 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) a += s[j][threadIdx.x];
+    if (c < cols) {
+        if (dw != nullptr) dw[c] = (T)a;
+    } else if (db != nullptr) {
+        db[c - cols] = (T)a;
+    }
+}
+
+// The lanes and vectors of a row: the fewest lanes that hold it with one vector each,
+// then more vectors, then a whole workgroup.  `vecs`: 16-byte vectors that a row of
+// any phase may span.
+struct NormShape {
+    int lpr, nv;
+};
+
+inline NormShape norm_shape(int cols, int dtype, bool aligned) {
+    const int n = 16 / (int)dtype_size(dtype);
+    const int vecs = (cols + (aligned ? 0 : n - 1) + n - 1) / n;
+    if (vecs <= 8) return {8, 1};
+    if (vecs <= 16) return {16, 1};
+    if (vecs <= 32) return {32, 1};
+    if (vecs <= 64) return {64, 1};
+    if (vecs <= 128) return {64, 2};
+    if (vecs <= 256) return {64, 4};
+    if (vecs <= 512) return {256, 2};
+    if (vecs <= 1024) return {256, 4};
+    if (vecs <= 2048) return {256, 8};
+    if (vecs <= 4096 && n == 4) return {256, 16};  // registers as for 8 vectors of 8
+    return {0, 0};
+}
+
+// Workgroups of a launch over `rows` rows: a multiple of 8 row groups in all.
+inline int norm_grid(int rows, int lpr, int most) {
+    const int rpb = kNormBlock / lpr;
+    const int step = rpb >= 8 ? 1 : 8 / rpb;
+    long long g = ((long long)rows + rpb - 1) / rpb;
+    if (g > most) g = most;
+    return (int)((g + step - 1) / step * step);
+}
+
+// Most workgroups of the two directions; the backward's each leave a partial row of
+// 2 * cols sums.
+constexpr int kNormFwdGrid = 2048;
+constexpr int kNormBwdGrid = 512;
+
+template <typename T, bool BWD>
+hipError_t norm_launch(const NormShape& sh, const NormArgs& a, hipStream_t s) {
+    const int grid = norm_grid(a.rows, sh.lpr, BWD ? kNormBwdGrid : kNormFwdGrid);
+#define GAT_NORM_CASE(L, V)                                                     \
+    if (sh.lpr == L && sh.nv == V) {                                            \
+        if constexpr (BWD)                                                      \
+            k_norm_bwd<T, L, V><<<grid, kNormBlock, 0, s>>>(a);                 \
+        else                                                                    \
+            k_norm_fwd<T, L, V><<<grid, kNormBlock, 0, s>>>(a);                 \
+        return hipGetLastError();                                               \
+    }
+    GAT_NORM_CASE(8, 1)
+    GAT_NORM_CASE(16, 1)
+    GAT_NORM_CASE(32, 1)
+    GAT_NORM_CASE(64, 1)
+    GAT_NORM_CASE(64, 2)
+    GAT_NORM_CASE(64, 4)
+    GAT_NORM_CASE(256, 2)
+    GAT_NORM_CASE(256, 4)
+    GAT_NORM_CASE(256, 8)
+    if constexpr (sizeof(T) == 4) {
+        GAT_NORM_CASE(256, 16)
+    }
+#undef GAT_NORM_CASE
+    return hipErrorInvalidValue;
+}
+
+template <bool BWD>
+hipError_t norm_by_type(const NormShape& sh, const NormArgs& a, int dtype, hipStream_t s) {
+    if (dtype == GAT_F32) return norm_launch<float, BWD>(sh, a, s);
+    if (dtype == GAT_BF16) return norm_launch<bf16, BWD>(sh, a, s);
+    return norm_launch<f16, BWD>(sh, a, s);
+}
+
+// The tensor's rows lie as x's against the 16-byte boundaries.
+inline int lies_as(const void* x, long long ld_x, const void* t, long long ld, int dtype) {
+    const uintptr_t z = dtype_size(dtype);
+    return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(t)) & 15) == 0 &&
+           ((uintptr_t)(ld_x - ld) * z & 15) == 0;
+}
+
+inline bool norm_aligned(const void* x, long long ld, int dtype) {
+    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ((uintptr_t)ld * dtype_size(dtype) & 15) == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gat_layer_norm(const void* x, long long ld_x, int rows, int cols, const void* w,
+                   const void* b, float eps, void* y, long long ld_y, float* stats, int dtype,
+                   void* stream) {
+    if (rows < 0 || cols <= 0 || !known_dtype(dtype) || !(eps >= 0.f)) return GAT_EINVAL;
+    const NormShape sh = norm_shape(cols, dtype, norm_aligned(x, ld_x, dtype));
+    if (sh.lpr == 0) return GAT_EUNSUPPORTED;
+    if (rows == 0) return GAT_OK;
+    if (x == nullptr || y == nullptr || ld_x < 0 || ld_y < cols || !element_aligned(x, dtype) ||
+        !element_aligned(y, dtype))
+        return GAT_EINVAL;
+    NormArgs a{};
+    a.x = x;
+    a.out = y;
+    a.w = w;
+    a.b = b;
+    a.stats = stats;
+    a.ld_x = ld_x;
+    a.ld_out = ld_y;
+    a.rows = rows;
+    a.cols = cols;
+    a.eps = eps;
+    a.whole_out = lies_as(x, ld_x, y, ld_y, dtype);
+    return status_of(norm_by_type<false>(sh, a, dtype, static_cast<hipStream_t>(stream)));
+}
+
+int gat_layer_norm_backward_workspace_size(int rows, int cols, int dtype, size_t* bytes) {
+    if (rows < 0 || cols <= 0 || !known_dtype(dtype) || bytes == nullptr) return GAT_EINVAL;
+    size_t most = 0;  // x's alignment is not known here: the larger of the two
+    for (int aligned = 0; aligned < 2; ++aligned) {
+        const NormShape sh = norm_shape(cols, dtype, aligned != 0);
+        if (sh.lpr == 0) {
+            if (aligned) return GAT_EUNSUPPORTED;
+            continue;
+        }
+        most = std::max(most, (size_t)norm_grid(rows, sh.lpr, kNormBwdGrid));
+    }
+    *bytes = most * 2 * (size_t)cols * sizeof(float);
+    return GAT_OK;
+}
+
+int gat_layer_norm_backward(const void* g, long long ld_g, const void* x, long long ld_x, int rows,
+                            int cols, const void* w, const float* stats, void* dx,
+                            long long ld_dx, void* dw, void* db, void* workspace,
+                            size_t workspace_bytes, int dtype, void* stream) {
+    if (rows < 0 || cols <= 0 || !known_dtype(dtype)) return GAT_EINVAL;
+    const NormShape sh = norm_shape(cols, dtype, norm_aligned(x, ld_x, dtype));
+    if (sh.lpr == 0) return GAT_EUNSUPPORTED;
+    const bool sums = dw != nullptr || db != nullptr;
+    const int parts = rows > 0 ? norm_grid(rows, sh.lpr, kNormBwdGrid) : 0;
+    if (sums && workspace_bytes < (size_t)parts * 2 * cols * sizeof(float)) return GAT_EWORKSPACE;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (rows > 0) {
+        if (g == nullptr || x == nullptr || stats == nullptr || ld_x < 0 || ld_g < 0 ||
+            (dx != nullptr && (ld_dx < cols || !element_aligned(dx, dtype))) ||
+            (sums && workspace == nullptr) || !element_aligned(x, dtype) ||
+            !element_aligned(g, dtype))
+            return GAT_EINVAL;
+        NormArgs a{};
+        a.x = x;
+        a.g = g;
+        a.out = dx;
+        a.w = w;
+        a.stats = const_cast<float*>(stats);
+        a.part = sums ? static_cast<float*>(workspace) : nullptr;
+        a.ld_x = ld_x;
+        a.ld_g = ld_g;
+        a.ld_out = ld_dx;
+        a.rows = rows;
+        a.cols = cols;
+        a.whole_g = lies_as(x, ld_x, g, ld_g, dtype);
+        a.whole_out = dx != nullptr && lies_as(x, ld_x, dx, ld_dx, dtype);
+        const hipError_t e = norm_by_type<true>(sh, a, dtype, s);
+        if (e != hipSuccess) return status_of(e);
+    }
+    if (!sums) return GAT_OK;
+    const int grid = (2 * cols + kColsTile - 1) / kColsTile;
+    const float* part = static_cast<const float*>(workspace);
+    if (dtype == GAT_F32)
+        k_norm_columns<float><<<grid, 1024, 0, s>>>(part, parts, cols, static_cast<float*>(dw),
+                                                    static_cast<float*>(db));
+    else if (dtype == GAT_BF16)
+        k_norm_columns<bf16><<<grid, 1024, 0, s>>>(part, parts, cols, static_cast<bf16*>(dw),
+                                                   static_cast<bf16*>(db));
+    else
+        k_norm_columns<f16><<<grid, 1024, 0, s>>>(part, parts, cols, static_cast<f16*>(dw),
+                                                  static_cast<f16*>(db));
+    return status_of(hipGetLastError());
+}
+
+}  // extern "C"

@@ -1,0 +1,262 @@
+"""Operators over rows that are packed along one dimension, as a batch of graphs packs
+its nodes: layer norm, embedding and (``packed_attention``) attention within each
+sequence.  Each is a hand-written HIP kernel behind ``libgat_amd.so`` with a HIP
+backward, next to :class:`GraphAttentionLayer`.
+
+Common to all: tensors on one ROCm device (a CPU tensor raises ``RuntimeError``; there
+is no CPU path), float32, bfloat16 or float16 where an operator does not say otherwise,
+float32 sums and statistics, one rounding at the end.  Work is enqueued on torch's
+current stream of the tensors' device, nothing synchronises the host, and every
+workspace comes from torch's allocator within the call, so calls can be captured in HIP
+graphs.  Results do not depend on timing: no kernel adds with atomics.
+
+When a step is captured in a graph, keep no autograd graph of an eager step on the same
+leaves alive (detach what is kept of the warm-up steps): its gradient accumulators
+belong to another stream.
+"""
+from __future__ import annotations
+
+import contextlib
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+__all__ = ["layer_norm", "embedding", "LayerNorm", "Embedding"]
+
+_DTYPES = {torch.float32: _lib.GAT_F32, torch.bfloat16: _lib.GAT_BF16,
+           torch.float16: _lib.GAT_F16}
+_NULL = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Launches go to the device the tensors are on, whichever is current."""
+    return _NULL if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _need_tensor(what: str, name: str, t, dtypes=_DTYPES) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: {name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{what} needs ROCm device tensors ({name} is on {t.device}); "
+                           "there is no CPU path")
+    if t.dtype not in dtypes:
+        names = ", ".join(str(d).replace("torch.", "") for d in dtypes)
+        raise ValueError(f"{what}: {name} must be one of {names}, got {t.dtype}")
+    return t
+
+
+def _need_like(what: str, name: str, t, like: torch.Tensor, dtype=True) -> None:
+    if t.device != like.device:
+        raise ValueError(f"{what}: {name} is on {t.device}, the input on {like.device}")
+    if dtype and t.dtype != like.dtype:
+        raise ValueError(f"{what}: {name} is {t.dtype}, the input {like.dtype}")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., C] as [rows, C] with adjacent columns; a copy only where no view does it."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+# ---------------------------------------------------------------------------
+# Layer norm
+# ---------------------------------------------------------------------------
+def _norm_forward(x2, w, b, eps, stats):
+    lib = _lib.load()
+    y = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device)
+    with _on(x2.device):
+        rc = lib.gat_layer_norm(x2.data_ptr(), x2.stride(0), x2.shape[0], x2.shape[1], _ptr(w),
+                                _ptr(b), eps, y.data_ptr(), y.stride(0), _ptr(stats),
+                                _DTYPES[x2.dtype], _stream(x2.device))
+    if rc == _lib.GAT_EUNSUPPORTED:
+        raise ValueError(f"layer_norm: {x2.shape[1]} columns are more than a row may have "
+                         "(16384, or 16377 / float32 16381 where rows are not 16-byte aligned)")
+    if rc:
+        _lib.check(rc, "gat_layer_norm")
+    return y
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, eps):
+        x2 = _rows(x)
+        stats = torch.empty(x2.shape[0], 2, dtype=torch.float32, device=x.device)
+        y = _norm_forward(x2, w, b, eps, stats)
+        ctx.save_for_backward(x2, w, stats)
+        return y.view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x2, w, stats = ctx.saved_tensors
+        n, c = x2.shape
+        shape, g = g.shape, _rows(g)
+        need = ctx.needs_input_grad
+        dt = _DTYPES[x2.dtype]
+        dx = torch.empty(n, c, dtype=x2.dtype, device=x2.device) if need[0] else None
+        dw, db = (torch.empty(c, dtype=x2.dtype, device=x2.device) if k else None
+                  for k in need[1:3])
+        size = _lib.layer_norm_workspace_size(n, c, dt) if need[1] or need[2] else 0
+        ws = torch.empty(size, dtype=torch.uint8, device=x2.device)
+        with _on(x2.device):
+            rc = _lib.load().gat_layer_norm_backward(
+                g.data_ptr(), g.stride(0), x2.data_ptr(), x2.stride(0), n, c, _ptr(w),
+                stats.data_ptr(), _ptr(dx), c, _ptr(dw), _ptr(db), ws.data_ptr(), size, dt,
+                _stream(x2.device))
+        if rc:
+            _lib.check(rc, "gat_layer_norm_backward")
+        return None if dx is None else dx.view(shape), dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of ``x``
+    (any leading shape and strides), as ``torch.nn.functional.layer_norm`` over one
+    dimension.  ``weight`` and ``bias`` are ``[C]`` of ``x``'s type or None.
+    Differentiable in all three; the gradients of ``weight`` and ``bias`` are summed
+    over the rows in float32 in a fixed order.  Up to 16,384 columns (16,377 where the
+    rows do not all start on 16-byte boundaries; float32: 16,381)."""
+    _need_tensor("layer_norm", "x", x)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"layer_norm: x needs a last dimension of at least 1, got {tuple(x.shape)}")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None:
+            _need_like("layer_norm", name, _need_tensor("layer_norm", name, p), x)
+            if p.shape != x.shape[-1:]:
+                raise ValueError(f"layer_norm: {name} must have shape [{x.shape[-1]}], "
+                                 f"got {tuple(p.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"layer_norm: eps must be at least 0, got {eps}")
+    if x.numel() // x.shape[-1] > 0x7FFFFFFF:
+        raise ValueError("layer_norm: at most 2^31 - 1 rows")
+    w, b = (None if p is None else p.contiguous() for p in (weight, bias))
+    if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)
+                                    or (b is not None and b.requires_grad)):
+        return _LayerNorm.apply(x, w, b, float(eps))
+    return _norm_forward(_rows(x), w, b, float(eps), None).view(x.shape)
+
+
+class LayerNorm(torch.nn.Module):
+    """:func:`layer_norm` with ``torch.nn.LayerNorm``'s parameters and state_dict keys,
+    over one trailing dimension."""
+
+    def __init__(self, normalized_shape: int, eps: float = 1e-5, elementwise_affine: bool = True,
+                 bias: bool = True):
+        super().__init__()
+        self.normalized_shape, self.eps = int(normalized_shape), float(eps)
+        self.weight = torch.nn.Parameter(torch.ones(self.normalized_shape)) \
+            if elementwise_affine else None
+        self.bias = torch.nn.Parameter(torch.zeros(self.normalized_shape)) \
+            if elementwise_affine and bias else None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1] != self.normalized_shape:
+            raise ValueError(f"LayerNorm({self.normalized_shape}) got {tuple(x.shape)}")
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self) -> str:
+        return f"{self.normalized_shape}, eps={self.eps}"
+
+
+# ---------------------------------------------------------------------------
+# Embedding
+# ---------------------------------------------------------------------------
+def _embed_forward(ids, w, scale):
+    out = torch.empty(ids.numel(), w.shape[1], dtype=w.dtype, device=w.device)
+    with _on(w.device):
+        rc = _lib.load().gat_embedding(ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(),
+                                       w.data_ptr(), w.stride(0), w.shape[0], w.shape[1], scale,
+                                       out.data_ptr(), out.stride(0), _DTYPES[w.dtype],
+                                       _stream(w.device))
+    if rc:
+        _lib.check(rc, "gat_embedding")
+    return out.view(*ids.shape, w.shape[1])
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, w, scale, padding):
+        ctx.save_for_backward(ids)
+        ctx.table, ctx.scale, ctx.padding = tuple(w.shape), scale, padding
+        return _embed_forward(ids, _rows(w), scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        ids, = ctx.saved_tensors
+        v, c = ctx.table
+        g = _rows(g)
+        dw = torch.empty(v, c, dtype=g.dtype, device=g.device)
+        size = _lib.embedding_grad_workspace_size(ids.numel(), v, c)
+        ws = torch.empty(size, dtype=torch.uint8, device=g.device)
+        with _on(g.device):
+            rc = _lib.load().gat_embedding_grad(
+                ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(), g.data_ptr(),
+                g.stride(0), v, c, ctx.scale, ctx.padding, dw.data_ptr(), c, ws.data_ptr(), size,
+                _DTYPES[g.dtype], _stream(g.device))
+        if rc:
+            _lib.check(rc, "gat_embedding_grad")
+        return None, dw, None, None
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
+              padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``scale * weight[ids]``: ``ids`` int32 or int64 of any shape, ``weight``
+    ``[vocab, C]``.  Differentiable in ``weight`` (a dense gradient, float32 sums over
+    each id's tokens in their order); tokens with ``padding_idx`` take no gradient, their
+    rows are read like any other.
+
+    An id outside ``[0, vocab)`` gives a row of NaN and takes no gradient: checking on the
+    host would cost a synchronisation per call.  At most 2^30 ids."""
+    _need_tensor("embedding", "weight", weight)
+    _need_tensor("embedding", "ids", ids, (torch.int64, torch.int32))
+    _need_like("embedding", "ids", ids, weight, dtype=False)
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"embedding: weight must be [vocab, C] with both at least 1, "
+                         f"got {tuple(weight.shape)}")
+    v = weight.shape[0]
+    if v > 0x7FFFFFFE or ids.numel() > 1 << 30:
+        raise ValueError("embedding: at most 2^31 - 2 table rows and 2^30 ids")
+    pad = -1
+    if padding_idx is not None:
+        if not -v <= padding_idx < v:
+            raise ValueError(f"embedding: padding_idx {padding_idx} is outside a table of {v}")
+        pad = int(padding_idx) % v
+    ids = ids.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _Embedding.apply(ids, weight, float(scale), pad)
+    return _embed_forward(ids, _rows(weight), float(scale))
+
+
+class Embedding(torch.nn.Module):
+    """:func:`embedding` with ``torch.nn.Embedding``'s parameter, initialisation and
+    state_dict key, and a ``scale`` on what it looks up."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, padding_idx: Optional[int] = None,
+                 scale: float = 1.0):
+        super().__init__()
+        if padding_idx is not None and not -num_embeddings <= padding_idx < num_embeddings:
+            raise ValueError(f"padding_idx {padding_idx} is outside a table of {num_embeddings}")
+        self.num_embeddings, self.embedding_dim = int(num_embeddings), int(embedding_dim)
+        self.padding_idx, self.scale = padding_idx, float(scale)
+        self.weight = torch.nn.Parameter(torch.empty(num_embeddings, embedding_dim))
+        torch.nn.init.normal_(self.weight)
+        if padding_idx is not None:
+            with torch.no_grad():
+                self.weight[padding_idx].zero_()
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        return embedding(ids, self.weight, self.scale, self.padding_idx)
+
+    def extra_repr(self) -> str:
+        return f"{self.num_embeddings}, {self.embedding_dim}, scale={self.scale}"

@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define GAT_ABI_VERSION 12
+#define GAT_ABI_VERSION 13
 
 #define GAT_OK 0
 #define GAT_EINVAL (-1)       /* malformed arguments (negative sizes, bad layout) */
@@ -577,6 +577,67 @@ int gat_sum_partials_workspace_size(int num_parts, long long width, size_t* byte
  */
 int gat_sum_partials(const float* partials, int num_parts, long long width, float* out,
                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Packed-sequence operators (ABI 13): layer norm, embedding.
+ * Tensors hold float32, bfloat16 or float16 (GAT_F32 / GAT_BF16 / GAT_F16); sums and
+ * statistics are float32, results are rounded once.
+ * ------------------------------------------------------------------------- */
+#define GAT_F32 0
+#define GAT_BF16 1
+#define GAT_F16 2
+
+/*
+ * y = (x - mean) / sqrt(var + eps) * w + b over the rows of x.
+ *   x      [rows, cols], row stride ld_x elements
+ *   w, b   [cols] of the same type; NULL: 1 / 0
+ *   y      [rows, cols], row stride ld_y >= cols; may be x itself
+ *   stats  [rows, 2] float32 (mean, 1 / sqrt(var + eps)) for the backward; may be NULL
+ * GAT_EUNSUPPORTED beyond 16384 columns (16377 or, in float32, 16381 where the rows do
+ * not all start on 16-byte boundaries).
+ */
+int gat_layer_norm(const void* x, long long ld_x, int rows, int cols, const void* w,
+                   const void* b, float eps, void* y, long long ld_y, float* stats, int dtype,
+                   void* stream);
+
+/* Workspace bytes of gat_layer_norm_backward (0 where it forms no dw and no db). */
+int gat_layer_norm_backward_workspace_size(int rows, int cols, int dtype, size_t* bytes);
+
+/*
+ * Gradients of gat_layer_norm for the incoming gradient g [rows, cols].
+ *   stats       as the forward stored them
+ *   dx          [rows, cols]; may be NULL
+ *   dw, db      [cols], summed over the rows in a fixed order; each may be NULL
+ */
+int gat_layer_norm_backward(const void* g, long long ld_g, const void* x, long long ld_x, int rows,
+                            int cols, const void* w, const float* stats, void* dx,
+                            long long ld_dx, void* dw, void* db, void* workspace,
+                            size_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * out[t] = scale * w[ids[t]] for tokens (at most 2^30) rows.
+ *   ids    int64 if ids64, else int32.  A row whose id is outside [0, vocab) is filled
+ *          with NaN: nothing outside the table is read, and the error shows.
+ *   w      [vocab, cols], row stride ld_w >= cols;  out [tokens, cols]
+ */
+int gat_embedding(const void* ids, int ids64, long long tokens, const void* w, long long ld_w,
+                  int vocab, int cols, float scale, void* out, long long ld_out, int dtype,
+                  void* stream);
+
+/* Workspace bytes of gat_embedding_grad. */
+int gat_embedding_grad_workspace_size(long long tokens, int vocab, int cols, size_t* bytes);
+
+/*
+ * dw[v] = scale * sum of g[t] over the tokens t with ids[t] = v, for every v in
+ * [0, vocab); rows without a token are zeros.  Deterministic.
+ *   padding  an id whose tokens take no gradient, or -1.  Ids outside [0, vocab) take
+ *            none either.
+ *   workspace  16-byte aligned
+ */
+int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void* g, long long ld_g,
+                       int vocab, int cols, float scale, long long padding, void* dw,
+                       long long ld_dw, void* workspace, size_t workspace_bytes, int dtype,
+                       void* stream);
 
 #ifdef __cplusplus
 }
