@@ -9,8 +9,9 @@ PyTorch-ROCm host code over the C-ABI HIP library ``libgat_amd.so``
 from .layer import (GraphAttentionLayer, GraphAttentionLayerActivationTest,  # noqa: F401
                     gat_forward, pack_params)
 from .graph import CSRGraph, build_csr, get_csr  # noqa: F401
-from .sequence import Embedding, LayerNorm, embedding, layer_norm  # noqa: F401
+from .sequence import (Embedding, LayerNorm, embedding, layer_norm,  # noqa: F401
+                       packed_attention)
 
 __all__ = ["GraphAttentionLayer", "GraphAttentionLayerActivationTest", "gat_forward",
            "pack_params", "CSRGraph", "build_csr", "get_csr", "layer_norm", "LayerNorm", "embedding",
-           "Embedding"]
+           "Embedding", "packed_attention"]

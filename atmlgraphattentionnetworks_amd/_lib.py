@@ -131,6 +131,14 @@ SIGNATURES = {
     "gat_embedding_grad_workspace_size": (_c_int, [_c_ll, _c_int, _c_int, _c_size_p]),
     "gat_embedding_grad": (_c_int, [_c_vp, _c_int, _c_ll, _c_vp, _c_ll, _c_int, _c_int, _c_float,
                                     _c_ll, _c_vp, _c_ll, _c_vp, ctypes.c_size_t, _c_int, _c_vp]),
+    "gat_packed_attention_workspace_size": (_c_int, [_c_int] * 7 + [_c_size_p]),
+    "gat_packed_attention": (_c_int, [_c_vp, _c_ll, _c_ll] * 3 + [_c_vp, _c_vp] + [_c_int] * 7 +
+                             [_c_float, _c_int, _c_vp, _c_vp, _c_vp, ctypes.c_size_t, _c_int,
+                              _c_vp]),
+    "gat_packed_attention_backward_workspace_size": (_c_int, [_c_int] * 7 + [_c_size_p]),
+    "gat_packed_attention_backward": (_c_int, [_c_vp, _c_ll, _c_ll] * 4 + [_c_vp] * 4 +
+                                      [_c_int] * 7 + [_c_float, _c_int] + [_c_vp] * 4 +
+                                      [ctypes.c_size_t, _c_int, _c_vp]),
 }
 
 _lock = threading.Lock()
@@ -257,4 +265,13 @@ def embedding_grad_workspace_size(tokens: int, vocab: int, cols: int) -> int:
     out = ctypes.c_size_t()
     check(load().gat_embedding_grad_workspace_size(tokens, vocab, cols, ctypes.byref(out)),
           "gat_embedding_grad_workspace_size")
+    return out.value
+
+
+@functools.lru_cache(maxsize=256)  # pure functions of the shape
+def packed_attention_workspace_size(backward: bool, *shape: int) -> int:
+    out = ctypes.c_size_t()
+    name = "gat_packed_attention_backward_workspace_size" if backward else \
+        "gat_packed_attention_workspace_size"
+    check(getattr(load(), name)(*shape, ctypes.byref(out)), name)
     return out.value

@@ -1,0 +1,1053 @@
+// Attention over packed sequences, forward and backward (gat_packed_attention,
+// gat_packed_attention_backward).
+//
+// Sequence b has the queries ptr[b] .. ptr[b+1] of q and the keys kv_ptr[b] ..
+// kv_ptr[b+1] of k and v.  Per query head h, with key head h / G (G query heads share
+// a key head):
+//   P = softmax(scale q k^T over the visible keys)        y = P v
+//   dP = g v^T     dS = P (dP - sum_d g y)
+//   dq = scale dS k    dk = scale sum_heads dS^T q    dv = sum_heads P^T g
+// Causal: key j is visible to query i iff j <= i + (keys - queries).  A query that
+// sees no key gives y = 0, lse = -inf and no gradient.
+//
+// One tile shape carries all three kernels.  A wave owns 32 COLUMNS (queries in the
+// forward and the dq kernel, keys in the dk/dv kernel), one per lane and half wave,
+// and streams ROWS of the other side through LDS, 32 at a time:
+//   scores[row][col]  = rows . columns        A: rows from LDS, B: columns in registers
+//   acc[d][col]      += X^T[d][row] W[row][col]     W: the scores after the softmax
+// A 32x32 matrix product leaves lane (col, half) with rows 8 i + 4 half + 0..3, and that
+// is the order in which it takes W back as its B operand: the scores never leave the
+// registers, and the softmax sums of a column are one lane's own plus one exchange
+// between the halves.  X^T comes out of LDS by the transposing 64-bit read.
+//
+// The query heads that share a key head are rows of one packed axis (row = query * G +
+// head in group): a tile holds whole groups, keys are read once for the group, and dk
+// and dv sum over the heads inside the kernel.
+//
+// Tiles are found without a launch that counts them: the sequence boundaries bnd are
+// monotone, so slot(s) = bnd[s] / tile + s leaves every sequence at least the slots it
+// needs.  The rows before the first and behind the last sequence form sequences without
+// keys, so their outputs and gradients are zeros.
+
+#include <climits>
+
+#include "gat_seq.h"
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+struct Rows {  // a [tokens, heads, dim] tensor; strides in elements
+    const void* p;
+    long long row, head;
+};
+
+struct AttnArgs {
+    Rows q, k, v, g, o;  // o: the forward's output
+    Rows dq, dk, dv;
+    float* lse;    // [queries, heads]
+    float* delta;  // [queries, heads] sum_d g y
+    const void *ptr, *kv_ptr;
+    float* part;  // partial results of a split axis
+    int ptr64, count;
+    int nq, nk;  // rows of q and of k
+    int kv_heads, group, dim;
+    unsigned div_mul, div_shift;  // row / group
+    float scale;
+    int causal, splits;
+};
+
+// The scores are formed as |scale| (+-columns) . rows, so that their maximum is that of the
+// products; a scale of 0 as 1 times zero columns (0 times a hidden row's -inf is no score).
+__device__ __forceinline__ float score_scale(float scale) { return scale == 0.f ? 1.f : fabsf(scale); }
+
+__device__ __forceinline__ int div_group(const AttnArgs& a, int r) {
+    return a.group == 1 ? r : (int)(__umulhi((unsigned)r, a.div_mul) >> a.div_shift);
+}
+
+// bnd[0] = 0, bnd[1 .. count + 1] = ptr, bnd[count + 2] = n: sequences 1 .. count are
+// the caller's, 0 and count + 1 the rows outside them.  Values are held to [0, n].
+__device__ __forceinline__ int bound_at(const void* ptr, int ptr64, int count, int n, int s) {
+    if (s <= 0) return 0;
+    if (s >= count + 2) return n;
+    const long long v = ptr64 ? static_cast<const long long*>(ptr)[s - 1]
+                              : (long long)static_cast<const int*>(ptr)[s - 1];
+    return (int)(v < 0 ? 0 : v > n ? n : v);
+}
+
+struct Tile {
+    int seq;    // as the caller counts, or -1 outside the sequences
+    int first;  // the sequence's first row, and its rows
+    int len;
+    int index;  // tile within the sequence
+};
+
+// The sequence and the tile of a slot; 64 boundaries a step.
+__device__ __forceinline__ Tile tile_of(const void* ptr, int ptr64, int count, int n, int group,
+                                        int size, int slot) {
+    const int lane = threadIdx.x % kWave;
+    int lo = 0, hi = count + 2;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + kWave - 1) / kWave;
+        const int at = lo + lane * step;
+        bool ok = false;
+        if (at < hi)
+            ok = (long long)bound_at(ptr, ptr64, count, n, at) * group / size + at <= slot;
+        const int got = __popcll(__ballot(ok));
+        lo += (got > 0 ? got - 1 : 0) * step;
+        if (lo + step < hi) hi = lo + step;
+    }
+    Tile t;
+    t.first = bound_at(ptr, ptr64, count, n, lo);
+    t.len = bound_at(ptr, ptr64, count, n, lo + 1) - t.first;
+    if (t.len < 0) t.len = 0;
+    t.index = slot - (int)((long long)t.first * group / size + lo);
+    t.seq = lo >= 1 && lo <= count ? lo - 1 : -1;
+    return t;
+}
+
+inline long long slots_of(long long n, int group, int size, int count) {
+    return n * group / size + count + 2;
+}
+
+// ---------------------------------------------------------------------------
+// Matrix products.  K of a step: two 16-byte vectors, one per half wave.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+
+template <typename T, int DP>
+struct Shape {
+    static constexpr int N = Vec16<T>::N;
+    static constexpr int STEPS = DP / (2 * N);       // products of a 32x32 score tile
+    static constexpr int DT = (DP + 31) / 32;        // 32-wide tiles of the head dimension
+    static constexpr int LD = DP + N;                // LDS row: a vector of padding spreads the banks
+    static constexpr int CPR = DP / N;               // vectors of a row
+    static constexpr int slab(int rows) { return rows * LD + 32; }  // the last tile may read past DP
+};
+
+// scores[row][col] of 32 rows in LDS against the wave's columns
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 scores(const T* rows, const typename Vec16<T>::type* cols) {
+    typedef Shape<T, DP> S;
+    const int lane = threadIdx.x % kWave;
+    const T* at = rows + (lane % 32) * S::LD + (lane / 32) * S::N;
+    f32x16 c = {};
+#pragma unroll
+    for (int s = 0; s < S::STEPS; ++s)
+        c = mma(*reinterpret_cast<const typename Vec16<T>::type*>(at + s * 2 * S::N), cols[s], c);
+    return c;
+}
+
+// four rows of one column of a row-major tile in LDS
+__device__ __forceinline__ bf16x4 read_transposed(const bf16* p) {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                          (lds_s16x4*)(__attribute__((address_space(3))) void*)p));
+}
+
+// acc[d][col] += sum over 32 rows of X[row][d] w[row][col]
+template <int DP>
+__device__ __forceinline__ void add_products(f32x16* acc, const bf16* rows, const f32x16& w) {
+    typedef Shape<bf16, DP> S;
+    const int lane = threadIdx.x % kWave;
+    const bf16* at = rows + (4 * (lane / 32) + lane % 16 / 4) * S::LD + lane % 32 / 16 * 16 +
+                     lane % 4 * 4;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        bf16x8 b;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = (bf16)w[8 * s + e];
+#pragma unroll
+        for (int t = 0; t < S::DT; ++t) {
+            const bf16x4 lo = read_transposed(at + 16 * s * S::LD + 32 * t);
+            const bf16x4 hi = read_transposed(at + (16 * s + 8) * S::LD + 32 * t);
+            acc[t] = mma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b, acc[t]);
+        }
+    }
+}
+template <int DP>
+__device__ __forceinline__ void add_products(f32x16* acc, const float* rows, const f32x16& w) {
+    typedef Shape<float, DP> S;
+    const int lane = threadIdx.x % kWave;
+    const float* at = rows + 4 * (lane / 32) * S::LD + lane % 32;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int t = 0; t < S::DT; ++t)
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[(8 * (i / 4) + i % 4) * S::LD + 32 * t],
+                                                          w[i], acc[t], 0, 0, 0);
+}
+
+// row within the 32 of register i of a product
+__device__ __forceinline__ int row_of(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
+
+// A column's vectors out of memory: vector s of lane (col, half) holds dimensions
+// (2 s + half) N ...; zeros where `in` is false and beyond `dim`.
+template <typename T, int DP>
+__device__ __forceinline__ void load_columns(typename Vec16<T>::type* cols, const T* row, int dim,
+                                             bool in, bool negate) {
+    typedef Shape<T, DP> S;
+    const int half = threadIdx.x % kWave / 32;
+#pragma unroll
+    for (int s = 0; s < S::STEPS; ++s) {
+        typename Vec16<T>::type v = {};
+        const int d = (2 * s + half) * S::N;
+        if (in && d < dim) v = *reinterpret_cast<const typename Vec16<T>::type*>(row + d);
+        cols[s] = negate ? -v : v;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Causal tiles that some column of the workgroup does not see in whole: a hidden row has
+// W = 0, but 0 times an infinity or NaN in its X would still reach the column.  Such a
+// tile is looked over as it is stored (`bad` takes its number); when it holds one, its
+// non-finite values are cleared in LDS once the scores are formed, and after the matrix
+// product their share is added for the rows that are seen.  All other rows get the same
+// bits as from a finite tile.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ bool non_finite(float v) {
+    return (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u;
+}
+
+template <typename T, int DP, int NW, int BN>
+__device__ __forceinline__ void clear_non_finite(T* lds) {
+    typedef Shape<T, DP> S;
+    typedef typename Vec16<T>::type V;
+#pragma unroll 1
+    for (int at = threadIdx.x; at < BN * S::CPR; at += NW * kWave) {
+        V* p = reinterpret_cast<V*>(lds + at / S::CPR * S::LD + at % S::CPR * S::N);
+        V x = *p;
+#pragma unroll
+        for (int e = 0; e < S::N; ++e)
+            if (non_finite((float)x[e])) x[e] = (T)0.f;
+        *p = x;
+    }
+}
+
+// bit i of `seen`: the column sees row r0 + row_of(i, half)
+template <typename T, int DP, typename F>
+__device__ __forceinline__ void add_non_finite(f32x16* acc, f32x16 w, unsigned seen, int r0, int end,
+                                               int dim, F addr) {
+    const int half = threadIdx.x % kWave / 32;
+    const unsigned seen_there = __shfl_xor(seen, 32);
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+        const float here = w[0], there = __shfl_xor(here, 32);
+        w = __builtin_shufflevector(w, w, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 0);
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+            const int row = r0 + row_of(i, k);
+            const unsigned s = k == half ? seen : seen_there;
+            if (row >= end || !((s >> i) & 1)) continue;
+            const float f = k == half ? here : there;
+            const T* x = addr(row);
+#pragma unroll
+            for (int t = 0; t < (DP + 31) / 32; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int d = 32 * t + row_of(e, half);
+                    const float v = d < dim ? (float)x[d] : 0.f;
+                    if (non_finite(v)) acc[t][e] += f * v;
+                }
+        }
+    }
+}
+
+// Row tiles: memory -> registers -> LDS, so that the next tile's loads are in flight
+// while the present one is worked on.
+template <typename T, int DP, int NW, int BN>
+struct Stage {
+    typedef Shape<T, DP> S;
+    typedef typename Vec16<T>::type V;
+    static constexpr int NT = NW * kWave;
+    static constexpr int CNT = (BN * S::CPR + NT - 1) / NT;
+    V v[CNT];
+
+    // rows [r0, end) of the sequence; `addr(row)` gives a row's address
+    template <typename F>
+    __device__ __forceinline__ void load(int r0, int end, int dim, F addr) {
+#pragma unroll
+        for (int j = 0; j < CNT; ++j) {
+            const int at = j * NT + threadIdx.x;
+            const int r = at / S::CPR, d = at % S::CPR * S::N;
+            V x = {};
+            if (at < BN * S::CPR && r0 + r < end && d < dim)
+                x = *reinterpret_cast<const V*>(addr(r0 + r) + d);
+            v[j] = x;
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int j = 0; j < CNT; ++j) {
+            const int at = j * NT + threadIdx.x;
+            const int r = at / S::CPR, d = at % S::CPR * S::N;
+            if (at < BN * S::CPR) *reinterpret_cast<V*>(lds + r * S::LD + d) = v[j];
+        }
+    }
+    // *bad = tag if a value is infinite or NaN
+    __device__ __forceinline__ void look_over(int* bad, int tag) const {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < CNT; ++j)
+#pragma unroll
+            for (int e = 0; e < S::N; ++e) any = any || non_finite((float)v[j][e]);
+        if (any) *bad = tag;
+    }
+};
+
+// acc[d][col] of one column as a row of T, or as float32 partial sums
+template <typename T, int DP>
+__device__ __forceinline__ void store_column(T* row, const f32x16* acc, float f, int dim) {
+    const int half = threadIdx.x % kWave / 32;
+    typedef T V4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int t = 0; t < (DP + 31) / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 32 * t + 8 * i + 4 * half;
+            if (d >= dim) continue;
+            V4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = (T)(acc[t][4 * i + e] * f);
+            *reinterpret_cast<V4*>(row + d) = y;
+        }
+}
+
+constexpr float kRescale = 8.f;  // log2 of how far p may pass 1 before the sums are rescaled
+
+// ---------------------------------------------------------------------------
+// Forward: columns = queries, rows = keys.  One pass with a running reference m: p =
+// exp(s - m), sums of p and p v; m follows the maximum only when that has grown by over
+// 2^8, so most tiles skip the rescaling of the accumulators (p stays far inside float32
+// and keeps its relative precision in bf16).  p is rounded to v's type for the second
+// product, the sum l uses the unrounded p.
+// ---------------------------------------------------------------------------
+template <typename T, int DP, int NW, int R>
+__global__ __launch_bounds__(NW * kWave) void k_attn_fwd(AttnArgs a) {
+    typedef Shape<T, DP> S;
+    typedef typename Vec16<T>::type V;
+    constexpr int BM = 32 * NW, BN = 32 * R;
+    __shared__ __align__(16) T lk[S::slab(BN)], lv[S::slab(BN)];
+    __shared__ int bad;
+    if (threadIdx.x == 0) bad = 0;
+    const Tile t = tile_of(a.ptr, a.ptr64, a.count, a.nq, a.group, BM, blockIdx.x);
+    const int rows = t.len * a.group;
+    if (t.index < 0 || (long long)t.index * BM >= rows) return;
+    const int kh = blockIdx.y;
+    const int k0 = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 1);
+    int nk = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 2) - k0;
+    if (nk < 0) nk = 0;
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    const int r0 = t.index * BM + threadIdx.x / kWave * 32;
+    const int r = r0 + lane % 32;
+    // the keys that a row sees: [0, limit)
+    auto limit = [&](int row) {
+        if (!a.causal) return nk;
+        const int l = div_group(a, row) + nk - t.len + 1;
+        return l < 0 ? 0 : l > nk ? nk : l;
+    };
+    const bool mine = r < rows;
+    const int rc = mine ? r : rows - 1;
+    const int qi = div_group(a, rc), gi = rc - qi * a.group;
+    const int head = kh * a.group + gi;
+    const int lim = limit(rc);
+    const int lim_first = limit(r0 < rows ? r0 : rows - 1);  // the wave's smallest
+    const int lim_last = r0 < rows ? limit(r0 + 31 < rows ? r0 + 31 : rows - 1) : 0;
+    const int last = t.index * BM + BM - 1;
+    const int lim_block = limit(last < rows ? last : rows - 1);
+    const int lim_whole = a.causal ? limit(t.index * BM) : INT_MAX;  // keys that all rows see
+    int from = 0, to = lim_block;
+    if (a.splits > 1) {
+        const int per = ((nk + a.splits - 1) / a.splits + BN - 1) / BN * BN;
+        from = blockIdx.z * per;
+        to = from + per < lim_block ? from + per : lim_block;
+    }
+
+    V qc[S::STEPS];
+    load_columns<T, DP>(qc,
+                        static_cast<const T*>(a.q.p) + (long long)(t.first + qi) * a.q.row +
+                            (long long)head * a.q.head,
+                        a.dim, mine && a.scale != 0.f, a.scale < 0.f);
+    const T* kb = static_cast<const T*>(a.k.p) + (long long)k0 * a.k.row + (long long)kh * a.k.head;
+    const T* vb = static_cast<const T*>(a.v.p) + (long long)k0 * a.v.row + (long long)kh * a.v.head;
+    auto k_at = [&](int row) { return kb + (long long)row * a.k.row; };
+    auto v_at = [&](int row) { return vb + (long long)row * a.v.row; };
+    const float c = score_scale(a.scale) * kLog2e;
+
+    f32x16 acc[S::DT] = {};
+    float m = -INFINITY, l = 0.f;
+    Stage<T, DP, NW, BN> sk, sv;
+    if (from < to) {
+        sk.load(from, nk, a.dim, k_at);
+        sv.load(from, nk, a.dim, v_at);
+    }
+    for (int n0 = from; n0 < to; n0 += BN) {
+        __syncthreads();
+        sk.store(lk);
+        sv.store(lv);
+        const bool edge = n0 + BN > lim_whole;
+        if (edge) sv.look_over(&bad, n0 + 1);
+        __syncthreads();
+        if (n0 + BN < to) {
+            sk.load(n0 + BN, nk, a.dim, k_at);
+            sv.load(n0 + BN, nk, a.dim, v_at);
+        }
+        const bool mend = edge && bad == n0 + 1;
+        if (n0 >= lim_last && !mend) continue;
+        f32x16 s[R];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            s[j] = scores<T, DP>(lk + 32 * j * S::LD, qc);
+            if (n0 + 32 * j + 32 > lim_first) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[j][i]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        if (__any((mx - m) * c > kRescale)) {  // -inf - -inf: false
+            const float to_m = fmaxf(m, mx);
+            const float f = m == -INFINITY ? 0.f : exp2f((m - to_m) * c);
+            m = to_m;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < S::DT; ++d) acc[d] *= f;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        if (mend) {
+            clear_non_finite<T, DP, NW, BN>(lv);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -mc));
+                l += s[j][i];
+            }
+            add_products<DP>(acc, lv + 32 * j * S::LD, s[j]);
+            if (mend) {
+                unsigned seen = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
+                add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, v_at);
+            }
+        }
+    }
+    l += __shfl_xor(l, 32);
+    if (!mine) return;
+    const long long qh = (long long)(t.first + qi) * a.kv_heads * a.group + head;
+    if (a.splits > 1) {
+        const long long at = (long long)blockIdx.z * a.nq * a.kv_heads * a.group + qh;
+        store_column<float, DP>(a.part + at * a.dim, acc, 1.f, a.dim);
+        float* ml = a.part + (long long)a.splits * a.nq * a.kv_heads * a.group * a.dim;
+        if (half == 0) {
+            ml[2 * at] = m;
+            ml[2 * at + 1] = lim == 0 && blockIdx.z == 0 ? 1.f : l;  // no key: 0 / 1, not 0 / 0
+        }
+        return;
+    }
+    T* out = static_cast<T*>(const_cast<void*>(a.o.p)) + (long long)(t.first + qi) * a.o.row +
+             (long long)head * a.o.head;
+    if (lim == 0) {  // sees no key
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) acc[d] = f32x16{};
+        l = 1.f;
+    }
+    store_column<T, DP>(out, acc, 1.f / l, a.dim);
+    if (a.lse != nullptr && half == 0)
+        a.lse[qh] = lim == 0 ? -INFINITY : m * score_scale(a.scale) + logf(l);
+}
+
+// Joins the forward's splits: y = sum_s f_s acc_s / sum_s f_s l_s, f_s = exp(m_s - max m).
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+    const int quads = a.dim / 4;
+    const long long n = (long long)a.nq * a.kv_heads * a.group;
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= n * quads) return;
+    const long long qh = at / quads;
+    const int d = (int)(at % quads) * 4;
+    const float* ml = a.part + a.splits * n * a.dim;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[2 * (s * n + qh)]);
+    const float c = score_scale(a.scale) * kLog2e;
+    float l = 0.f;
+    f32x4 acc = {};
+    for (int s = 0; s < a.splits; ++s) {
+        const long long i = s * n + qh;
+        const float f = m == -INFINITY ? 1.f : exp2f((ml[2 * i] - m) * c);
+        l += f * ml[2 * i + 1];
+        acc = fma4(f, *reinterpret_cast<const f32x4*>(a.part + i * a.dim + d), acc);
+    }
+    const long long tok = qh / (a.kv_heads * a.group), head = qh % (a.kv_heads * a.group);
+    T* out = static_cast<T*>(const_cast<void*>(a.o.p)) + tok * a.o.row + head * a.o.head + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = (T)(acc[e] / l);
+    if (a.lse != nullptr && d == 0)
+        a.lse[qh] = m == -INFINITY ? -INFINITY : m * score_scale(a.scale) + logf(l);
+}
+
+// out[i] = scale * sum over the splits, of one tensor's partial sums
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_sum(const float* part, int splits, long long step,
+                                                  long long n, float scale, T* out) {
+    const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= n) return;
+    f32x4 s = {};
+    for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + k * step + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[at + e] = (T)(s[e] * scale);
+}
+
+// ---------------------------------------------------------------------------
+// dq: columns = queries, rows = keys.  P comes back from the scores and lse; dS is
+// rounded to k's type for the product with k.  sum_d g y is formed here, in float32 from
+// the stored y, and left for the dk/dv kernel.
+// ---------------------------------------------------------------------------
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * kWave) void k_attn_dq(AttnArgs a) {
+    typedef Shape<T, DP> S;
+    typedef typename Vec16<T>::type V;
+    constexpr int BM = 32 * NW, BN = 32;
+    __shared__ __align__(16) T lk[S::slab(BN)], lv[S::slab(BN)];
+    __shared__ int bad;
+    if (threadIdx.x == 0) bad = 0;
+    const Tile t = tile_of(a.ptr, a.ptr64, a.count, a.nq, a.group, BM, blockIdx.x);
+    const int rows = t.len * a.group;
+    if (t.index < 0 || (long long)t.index * BM >= rows) return;
+    const int kh = blockIdx.y;
+    const int k0 = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 1);
+    int nk = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 2) - k0;
+    if (nk < 0) nk = 0;
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    const int r0 = t.index * BM + threadIdx.x / kWave * 32;
+    const int r = r0 + lane % 32;
+    auto limit = [&](int row) {
+        if (!a.causal) return nk;
+        const int l = div_group(a, row) + nk - t.len + 1;
+        return l < 0 ? 0 : l > nk ? nk : l;
+    };
+    const bool mine = r < rows;
+    const int rc = mine ? r : rows - 1;
+    const int qi = div_group(a, rc), gi = rc - qi * a.group;
+    const int head = kh * a.group + gi;
+    const int lim = limit(rc);
+    const int lim_first = limit(r0 < rows ? r0 : rows - 1);
+    const int lim_last = r0 < rows ? limit(r0 + 31 < rows ? r0 + 31 : rows - 1) : 0;
+    const int last = t.index * BM + BM - 1;
+    const int lim_block = limit(last < rows ? last : rows - 1);
+    const int lim_whole = a.causal ? limit(t.index * BM) : INT_MAX;  // keys that all rows see
+    int from = 0, to = lim_block;
+    if (a.splits > 1) {
+        const int per = ((nk + a.splits - 1) / a.splits + BN - 1) / BN * BN;
+        from = blockIdx.z * per;
+        to = from + per < lim_block ? from + per : lim_block;
+    }
+
+    V qc[S::STEPS], gc[S::STEPS];
+    const long long tok = t.first + qi;
+    const long long qh = tok * a.kv_heads * a.group + head;
+    load_columns<T, DP>(qc, static_cast<const T*>(a.q.p) + tok * a.q.row + (long long)head * a.q.head,
+                        a.dim, mine && a.scale != 0.f, a.scale < 0.f);
+    load_columns<T, DP>(gc, static_cast<const T*>(a.g.p) + tok * a.g.row + (long long)head * a.g.head,
+                        a.dim, mine, false);
+    float delta = 0.f;
+    {
+        V oc[S::STEPS];
+        load_columns<T, DP>(oc, static_cast<const T*>(a.o.p) + tok * a.o.row +
+                                    (long long)head * a.o.head, a.dim, mine, false);
+#pragma unroll
+        for (int s = 0; s < S::STEPS; ++s)
+#pragma unroll
+            for (int e = 0; e < S::N; ++e) delta = fmaf((float)gc[s][e], (float)oc[s][e], delta);
+        delta += __shfl_xor(delta, 32);
+    }
+    if (mine && half == 0 && blockIdx.z == 0) a.delta[qh] = delta;
+    const float lse2 = mine ? a.lse[qh] * kLog2e : 0.f;
+    const T* kb = static_cast<const T*>(a.k.p) + (long long)k0 * a.k.row + (long long)kh * a.k.head;
+    const T* vb = static_cast<const T*>(a.v.p) + (long long)k0 * a.v.row + (long long)kh * a.v.head;
+    auto k_at = [&](int row) { return kb + (long long)row * a.k.row; };
+    auto v_at = [&](int row) { return vb + (long long)row * a.v.row; };
+    const float c = score_scale(a.scale) * kLog2e;
+
+    f32x16 acc[S::DT] = {};
+    Stage<T, DP, NW, BN> sk, sv;
+    if (from < to) {
+        sk.load(from, nk, a.dim, k_at);
+        sv.load(from, nk, a.dim, v_at);
+    }
+    for (int n0 = from; n0 < to; n0 += BN) {
+        __syncthreads();
+        sk.store(lk);
+        sv.store(lv);
+        const bool edge = n0 + BN > lim_whole;
+        if (edge) sk.look_over(&bad, n0 + 1);
+        __syncthreads();
+        if (n0 + BN < to) {
+            sk.load(n0 + BN, nk, a.dim, k_at);
+            sv.load(n0 + BN, nk, a.dim, v_at);
+        }
+        const bool mend = edge && bad == n0 + 1;
+        if (n0 >= lim_last && !mend) continue;
+        f32x16 s = scores<T, DP>(lk, qc);
+        const f32x16 dp = scores<T, DP>(lv, gc);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2));
+            s[i] = p * (dp[i] - delta);
+        }
+        if (n0 + BN > lim_first) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (n0 + row_of(i, half) >= lim) s[i] = 0.f;
+        }
+        if (mend) {
+            __syncthreads();
+            clear_non_finite<T, DP, NW, BN>(lk);
+            __syncthreads();
+        }
+        add_products<DP>(acc, lk, s);
+        if (mend) {
+            unsigned seen = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) seen |= (n0 + row_of(i, half) < lim ? 1u : 0u) << i;
+            add_non_finite<T, DP>(acc, s, seen, n0, nk, a.dim, k_at);
+        }
+    }
+    if (!mine) return;
+    if (a.splits > 1) {
+        const long long at = (long long)blockIdx.z * a.nq * a.kv_heads * a.group + qh;
+        store_column<float, DP>(a.part + at * a.dim, acc, 1.f, a.dim);
+        return;
+    }
+    store_column<T, DP>(static_cast<T*>(const_cast<void*>(a.dq.p)) + tok * a.dq.row +
+                            (long long)head * a.dq.head,
+                        acc, a.scale, a.dim);
+}
+
+// ---------------------------------------------------------------------------
+// dk, dv: columns = keys, rows = (query, head of the group).
+// ---------------------------------------------------------------------------
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
+    typedef Shape<T, DP> S;
+    typedef typename Vec16<T>::type V;
+    constexpr int BM = 32 * NW, BN = 32, NT = NW * kWave;
+    __shared__ __align__(16) T lq[S::slab(BN)], lg[S::slab(BN)];
+    __shared__ __align__(16) float ll[BN], ld[BN];
+    __shared__ int bad;
+    if (threadIdx.x == 0) bad = 0;
+    const Tile t = tile_of(a.kv_ptr, a.ptr64, a.count, a.nk, 1, BM, blockIdx.x);
+    if (t.index < 0 || (long long)t.index * BM >= t.len) return;
+    const int kh = blockIdx.y;
+    const int q0 = t.seq < 0 ? 0 : bound_at(a.ptr, a.ptr64, a.count, a.nq, t.seq + 1);
+    int nq = t.seq < 0 ? 0 : bound_at(a.ptr, a.ptr64, a.count, a.nq, t.seq + 2) - q0;
+    if (nq < 0) nq = 0;
+    const int rows = nq * a.group;
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    const int c0 = t.index * BM + threadIdx.x / kWave * 32;
+    const int key = c0 + lane % 32;
+    const bool mine = key < t.len;
+    const int kc = mine ? key : t.len - 1;
+    // the rows that see a key: [start, rows)
+    auto start = [&](int k) {
+        if (!a.causal) return 0;
+        const int i = k - (t.len - nq);
+        return i < 0 ? 0 : i >= nq ? rows : i * a.group;
+    };
+    const int beg = start(kc);
+    const int beg_first = c0 < t.len ? start(c0) : rows;  // the wave's smallest
+    const int beg_last = start(c0 + 31 < t.len ? c0 + 31 : t.len - 1);
+    // the first row from which on all of the workgroup's keys are seen
+    const int beg_whole = start(t.index * BM + BM - 1 < t.len ? t.index * BM + BM - 1 : t.len - 1);
+    int from = start(t.index * BM) / BN * BN, to = rows;
+    if (a.splits > 1) {
+        const int per = ((rows + a.splits - 1) / a.splits + BN - 1) / BN * BN;
+        const int z = blockIdx.z * per;
+        if (from < z) from = z;
+        if (to > z + per) to = z + per;
+    }
+
+    V kcol[S::STEPS], vcol[S::STEPS];
+    const long long tok = t.first + kc;
+    load_columns<T, DP>(kcol, static_cast<const T*>(a.k.p) + tok * a.k.row + (long long)kh * a.k.head,
+                        a.dim, mine && a.scale != 0.f, a.scale < 0.f);
+    load_columns<T, DP>(vcol, static_cast<const T*>(a.v.p) + tok * a.v.row + (long long)kh * a.v.head,
+                        a.dim, mine, false);
+    const T* qb = static_cast<const T*>(a.q.p) + (long long)q0 * a.q.row +
+                  (long long)kh * a.group * a.q.head;
+    const T* gb = static_cast<const T*>(a.g.p) + (long long)q0 * a.g.row +
+                  (long long)kh * a.group * a.g.head;
+    auto q_at = [&](int row) {
+        const int i = div_group(a, row);
+        return qb + (long long)i * a.q.row + (long long)(row - i * a.group) * a.q.head;
+    };
+    auto g_at = [&](int row) {
+        const int i = div_group(a, row);
+        return gb + (long long)i * a.g.row + (long long)(row - i * a.group) * a.g.head;
+    };
+    // lse (in log2) and delta of a row tile: one row a thread, two where a wave is alone
+    constexpr int PER = BN > NT ? BN / NT : 1;
+    float rl[PER], rd[PER];
+    auto load_sums = [&](int n0) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int at = j * NT + threadIdx.x, row = n0 + at;
+            const bool in = at < BN && row < rows;
+            const int i = in ? div_group(a, row) : 0;
+            const long long qh = ((long long)(q0 + i) * a.kv_heads + kh) * a.group + (row - i * a.group);
+            rl[j] = in ? a.lse[qh] * kLog2e : INFINITY;  // exp(s - inf) = 0 behind the last row
+            rd[j] = in ? a.delta[qh] : 0.f;
+        }
+    };
+    const float c = score_scale(a.scale) * kLog2e;
+
+    f32x16 dk[S::DT] = {}, dv[S::DT] = {};
+    Stage<T, DP, NW, BN> sq, sg;
+    if (from < to) {
+        sq.load(from, rows, a.dim, q_at);
+        sg.load(from, rows, a.dim, g_at);
+        load_sums(from);
+    }
+    for (int n0 = from; n0 < to; n0 += BN) {
+        __syncthreads();
+        sq.store(lq);
+        sg.store(lg);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int at = j * NT + threadIdx.x;
+            if (at < BN) {
+                ll[at] = rl[j];
+                ld[at] = rd[j];
+            }
+        }
+        const bool edge = n0 < beg_whole;
+        if (edge) {
+            sq.look_over(&bad, n0 + 1);
+            sg.look_over(&bad, n0 + 1);
+        }
+        __syncthreads();
+        if (n0 + BN < to) {
+            sq.load(n0 + BN, rows, a.dim, q_at);
+            sg.load(n0 + BN, rows, a.dim, g_at);
+            load_sums(n0 + BN);
+        }
+        const bool mend = edge && bad == n0 + 1;
+        if (n0 + BN <= beg_first && !mend) continue;
+        f32x16 p = scores<T, DP>(lq, kcol);
+        f32x16 ds = scores<T, DP>(lg, vcol);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(ll + 8 * b + 4 * half);
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(ld + 8 * b + 4 * half);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * b + e;
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], c, -l4[e]));
+                ds[i] = p[i] * (ds[i] - d4[e]);
+            }
+        }
+        if (n0 < beg_last) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (n0 + row_of(i, half) < beg) p[i] = ds[i] = 0.f;
+        }
+        if (mend) {
+            __syncthreads();
+            clear_non_finite<T, DP, NW, BN>(lq);
+            clear_non_finite<T, DP, NW, BN>(lg);
+            __syncthreads();
+        }
+        add_products<DP>(dv, lg, p);
+        add_products<DP>(dk, lq, ds);
+        if (mend) {
+            unsigned seen = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) seen |= (n0 + row_of(i, half) >= beg ? 1u : 0u) << i;
+            add_non_finite<T, DP>(dv, p, seen, n0, rows, a.dim, g_at);
+            add_non_finite<T, DP>(dk, ds, seen, n0, rows, a.dim, q_at);
+        }
+    }
+    if (!mine) return;
+    if (a.splits > 1) {
+        const long long n = (long long)a.nk * a.kv_heads;
+        const long long at = (long long)blockIdx.z * n + tok * a.kv_heads + kh;
+        store_column<float, DP>(a.part + at * a.dim, dk, 1.f, a.dim);
+        store_column<float, DP>(a.part + (a.splits * n + at) * a.dim, dv, 1.f, a.dim);
+        return;
+    }
+    store_column<T, DP>(static_cast<T*>(const_cast<void*>(a.dk.p)) + tok * a.dk.row +
+                            (long long)kh * a.dk.head, dk, a.scale, a.dim);
+    store_column<T, DP>(static_cast<T*>(const_cast<void*>(a.dv.p)) + tok * a.dv.row +
+                            (long long)kh * a.dv.head, dv, 1.f, a.dim);
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+// A launch's waves per workgroup and its splits of the streamed axis, from the average
+// lengths (the lengths themselves are on the device).
+struct Plan {
+    int waves, splits;
+};
+
+// cols: rows of the axis whose tiles the grid walks; streamed: the other's.
+inline Plan plan_of(long long cols, long long streamed, int count, int kv_heads) {
+    const int n = count > 0 ? count : 1;
+    Plan p;
+    p.waves = cols <= 32ll * n ? 1 : 4;
+    const long long bm = 32 * p.waves;
+    const long long tiles = std::max<long long>(n, (cols + bm - 1) / bm) * kv_heads;
+    // Below about 8 waves a CU the axis is split, into parts of at least 128 rows
+    const long long want = (256ll * 8 / p.waves + tiles - 1) / tiles;
+    const long long most = streamed / n / 128;
+    p.splits = (int)std::max<long long>(1, std::min<long long>({want, most, 128}));
+    return p;
+}
+
+struct AttnSizes {
+    Plan fwd, dq, dkv;
+    size_t fwd_bytes, delta_bytes, dq_bytes, dkv_bytes;
+};
+
+inline AttnSizes attn_sizes(long long nq, long long nk, int count, int heads, int kv_heads, int dim) {
+    AttnSizes s;
+    const int group = heads / kv_heads;
+    s.fwd = plan_of(nq * group, nk, count, kv_heads);
+    s.dq = s.fwd;
+    s.dkv = plan_of(nk, nq * group, count, kv_heads);
+    const size_t q = (size_t)nq * heads, k = (size_t)nk * kv_heads;
+    s.fwd_bytes = s.fwd.splits > 1 ? s.fwd.splits * q * (dim + 2) * sizeof(float) : 0;
+    s.delta_bytes = align_up(q * sizeof(float));
+    s.dq_bytes = s.dq.splits > 1 ? s.dq.splits * q * dim * sizeof(float) : 0;
+    s.dkv_bytes = s.dkv.splits > 1 ? 2 * s.dkv.splits * k * dim * sizeof(float) : 0;
+    return s;
+}
+
+// What the kernels need of a call's sizes and layouts.
+inline int attn_check(int nq, int nk, int count, int heads, int kv_heads, int dim, int dtype) {
+    if (nq < 0 || nk < 0 || count < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
+        dim <= 0 || (dtype != GAT_F32 && dtype != GAT_BF16))
+        return GAT_EINVAL;
+    if (dim > GAT_PACKED_MAX_DIM || dim % (16 / (int)dtype_size(dtype)) != 0 ||
+        (long long)nq * (heads / kv_heads) > 0x3FFFFFFF || nk > 0x3FFFFFFF || count > 0x3FFFFFFF ||
+        kv_heads > 65535)
+        return GAT_EUNSUPPORTED;
+    return GAT_OK;
+}
+
+inline bool vec_rows(const Rows& r, int dtype) {
+    const int n = 16 / (int)dtype_size(dtype);
+    return (reinterpret_cast<uintptr_t>(r.p) & 15) == 0 && r.row % n == 0 && r.head % n == 0 &&
+           r.row >= 0 && r.head >= 0;
+}
+
+inline void set_group(AttnArgs& a, int group) {
+    a.group = group;
+    int s = 0;  // row / group = umulhi(row, mul) >> shift for rows below 2^31
+    while ((1 << (s + 1)) < group) ++s;
+    a.div_shift = s;
+    a.div_mul = group == 1 ? 0 : (unsigned)(((1ull << (32 + s)) + group - 1) / group);
+}
+
+enum AttnPass { kFwd, kDq, kDkv };
+
+template <typename T, int DP, AttnPass PASS>
+int attn_launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
+    const bool keys = PASS == kDkv;
+    const long long slots = slots_of(keys ? a.nk : a.nq, keys ? 1 : a.group, 32 * p.waves, a.count);
+    const dim3 grid((unsigned)slots, a.kv_heads, p.splits);
+    [[maybe_unused]] constexpr int R = sizeof(T) == 2 ? 2 : 1;  // 32-row tiles a step of the forward
+    if (p.waves == 1) {
+        if constexpr (PASS == kFwd) k_attn_fwd<T, DP, 1, R><<<grid, 64, 0, s>>>(a);
+        if constexpr (PASS == kDq) k_attn_dq<T, DP, 1><<<grid, 64, 0, s>>>(a);
+        if constexpr (PASS == kDkv) k_attn_dkv<T, DP, 1><<<grid, 64, 0, s>>>(a);
+    } else {
+        if constexpr (PASS == kFwd) k_attn_fwd<T, DP, 4, R><<<grid, 256, 0, s>>>(a);
+        if constexpr (PASS == kDq) k_attn_dq<T, DP, 4><<<grid, 256, 0, s>>>(a);
+        if constexpr (PASS == kDkv) k_attn_dkv<T, DP, 4><<<grid, 256, 0, s>>>(a);
+    }
+    return status_of(hipGetLastError());
+}
+
+template <typename T, AttnPass PASS>
+int attn_by_dim(const AttnArgs& a, const Plan& p, hipStream_t s) {
+    if constexpr (sizeof(T) == 4) {
+        if (a.dim <= 8) return attn_launch<T, 8, PASS>(a, p, s);
+    }
+    if (a.dim <= 16) return attn_launch<T, 16, PASS>(a, p, s);
+    if (a.dim <= 32) return attn_launch<T, 32, PASS>(a, p, s);
+    if (a.dim <= 64) return attn_launch<T, 64, PASS>(a, p, s);
+    if (a.dim <= 96) return attn_launch<T, 96, PASS>(a, p, s);
+    return attn_launch<T, 128, PASS>(a, p, s);
+}
+
+template <AttnPass PASS>
+int attn_pass(AttnArgs& a, const Plan& p, int dtype, hipStream_t s) {
+    a.splits = p.splits;
+    return dtype == GAT_F32 ? attn_by_dim<float, PASS>(a, p, s) : attn_by_dim<bf16, PASS>(a, p, s);
+}
+
+template <typename T>
+int attn_sum(const float* part, int splits, long long n, float scale, const Rows& out,
+             hipStream_t s) {
+    if (n == 0) return GAT_OK;
+    k_attn_sum<T><<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(
+        part, splits, n, n, scale, static_cast<T*>(const_cast<void*>(out.p)));
+    return status_of(hipGetLastError());
+}
+
+}  // namespace
+
+extern "C" {
+
+int gat_packed_attention_workspace_size(int nq, int nk, int count, int heads, int kv_heads, int dim,
+                                        int dtype, size_t* bytes) {
+    const int rc = attn_check(nq, nk, count, heads, kv_heads, dim, dtype);
+    if (rc != GAT_OK) return rc;
+    if (bytes == nullptr) return GAT_EINVAL;
+    *bytes = attn_sizes(nq, nk, count, heads, kv_heads, dim).fwd_bytes;
+    return GAT_OK;
+}
+
+int gat_packed_attention(const void* q, long long q_row, long long q_head, const void* k,
+                         long long k_row, long long k_head, const void* v, long long v_row,
+                         long long v_head, const void* ptr, const void* kv_ptr, int ptr64, int count,
+                         int nq, int nk, int heads, int kv_heads, int dim, float scale, int causal,
+                         void* out, float* lse, void* workspace, size_t workspace_bytes, int dtype,
+                         void* stream) {
+    const int rc = attn_check(nq, nk, count, heads, kv_heads, dim, dtype);
+    if (rc != GAT_OK) return rc;
+    if (nq == 0) return GAT_OK;
+    AttnArgs a{};
+    a.q = {q, q_row, q_head};
+    a.k = {k, k_row, k_head};
+    a.v = {v, v_row, v_head};
+    a.o = {out, (long long)heads * dim, dim};
+    if (q == nullptr || out == nullptr || ptr == nullptr || kv_ptr == nullptr ||
+        (nk > 0 && (k == nullptr || v == nullptr)))
+        return GAT_EINVAL;
+    if (!vec_rows(a.q, dtype) || !vec_rows(a.o, dtype) || !vec_rows(a.k, dtype) || !vec_rows(a.v, dtype))
+        return GAT_EUNSUPPORTED;
+    const AttnSizes sz = attn_sizes(nq, nk, count, heads, kv_heads, dim);
+    if (sz.fwd_bytes > 0 && (workspace == nullptr || workspace_bytes < sz.fwd_bytes))
+        return GAT_EWORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return GAT_EINVAL;
+    a.ptr = ptr;
+    a.kv_ptr = kv_ptr;
+    a.ptr64 = ptr64;
+    a.count = count;
+    a.nq = nq;
+    a.nk = nk;
+    a.kv_heads = kv_heads;
+    set_group(a, heads / kv_heads);
+    a.dim = dim;
+    a.scale = scale;
+    a.causal = causal;
+    a.lse = lse;
+    a.part = static_cast<float*>(workspace);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int st = attn_pass<kFwd>(a, sz.fwd, dtype, s);
+    if (st != GAT_OK || sz.fwd.splits == 1) return st;
+    const long long work = (long long)nq * heads * (dim / 4);
+    const unsigned grid = (unsigned)((work + 255) / 256);
+    if (dtype == GAT_F32)
+        k_attn_join<float><<<grid, 256, 0, s>>>(a);
+    else
+        k_attn_join<bf16><<<grid, 256, 0, s>>>(a);
+    return status_of(hipGetLastError());
+}
+
+int gat_packed_attention_backward_workspace_size(int nq, int nk, int count, int heads, int kv_heads,
+                                                 int dim, int dtype, size_t* bytes) {
+    const int rc = attn_check(nq, nk, count, heads, kv_heads, dim, dtype);
+    if (rc != GAT_OK) return rc;
+    if (bytes == nullptr) return GAT_EINVAL;
+    const AttnSizes s = attn_sizes(nq, nk, count, heads, kv_heads, dim);
+    *bytes = s.delta_bytes + std::max(s.dq_bytes, s.dkv_bytes);  // dq is done before dk and dv begin
+    return GAT_OK;
+}
+
+int gat_packed_attention_backward(const void* g, long long g_row, long long g_head, const void* q,
+                                  long long q_row, long long q_head, const void* k, long long k_row,
+                                  long long k_head, const void* v, long long v_row, long long v_head,
+                                  const void* out, const float* lse, const void* ptr,
+                                  const void* kv_ptr, int ptr64, int count, int nq, int nk, int heads,
+                                  int kv_heads, int dim, float scale, int causal, void* dq, void* dk,
+                                  void* dv, void* workspace, size_t workspace_bytes, int dtype,
+                                  void* stream) {
+    const int rc = attn_check(nq, nk, count, heads, kv_heads, dim, dtype);
+    if (rc != GAT_OK) return rc;
+    AttnArgs a{};
+    a.g = {g, g_row, g_head};
+    a.q = {q, q_row, q_head};
+    a.k = {k, k_row, k_head};
+    a.v = {v, v_row, v_head};
+    a.o = {out, (long long)heads * dim, dim};
+    a.dq = {dq, (long long)heads * dim, dim};
+    a.dk = {dk, (long long)kv_heads * dim, dim};
+    a.dv = {dv, (long long)kv_heads * dim, dim};
+    if (ptr == nullptr || kv_ptr == nullptr ||
+        (nq > 0 && (q == nullptr || g == nullptr || out == nullptr || lse == nullptr || dq == nullptr)) ||
+        (nk > 0 && (k == nullptr || v == nullptr || dk == nullptr || dv == nullptr)))
+        return GAT_EINVAL;
+    for (const Rows* r : {&a.g, &a.q, &a.k, &a.v, &a.o, &a.dq, &a.dk, &a.dv})
+        if (!vec_rows(*r, dtype)) return GAT_EUNSUPPORTED;
+    const AttnSizes sz = attn_sizes(nq, nk, count, heads, kv_heads, dim);
+    if (workspace_bytes < sz.delta_bytes + std::max(sz.dq_bytes, sz.dkv_bytes) ||
+        (workspace == nullptr && workspace_bytes > 0))
+        return GAT_EWORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return GAT_EINVAL;
+    a.ptr = ptr;
+    a.kv_ptr = kv_ptr;
+    a.ptr64 = ptr64;
+    a.count = count;
+    a.nq = nq;
+    a.nk = nk;
+    a.kv_heads = kv_heads;
+    set_group(a, heads / kv_heads);
+    a.dim = dim;
+    a.scale = scale;
+    a.causal = causal;
+    a.lse = const_cast<float*>(lse);
+    a.delta = static_cast<float*>(workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sz.delta_bytes);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    int st = GAT_OK;
+    if (nq > 0) {
+        st = attn_pass<kDq>(a, sz.dq, dtype, s);
+        if (st == GAT_OK && sz.dq.splits > 1) {
+            const long long n = (long long)nq * heads * dim;
+            st = dtype == GAT_F32 ? attn_sum<float>(a.part, sz.dq.splits, n, scale, a.dq, s)
+                                  : attn_sum<bf16>(a.part, sz.dq.splits, n, scale, a.dq, s);
+        }
+    }
+    if (st != GAT_OK || nk == 0) return st;
+    st = attn_pass<kDkv>(a, sz.dkv, dtype, s);
+    if (st != GAT_OK || sz.dkv.splits == 1) return st;
+    const long long n = (long long)nk * kv_heads * dim;
+    const float* pv = a.part + sz.dkv.splits * n;
+    st = dtype == GAT_F32 ? attn_sum<float>(a.part, sz.dkv.splits, n, scale, a.dk, s)
+                          : attn_sum<bf16>(a.part, sz.dkv.splits, n, scale, a.dk, s);
+    if (st != GAT_OK) return st;
+    return dtype == GAT_F32 ? attn_sum<float>(pv, sz.dkv.splits, n, 1.f, a.dv, s)
+                            : attn_sum<bf16>(pv, sz.dkv.splits, n, 1.f, a.dv, s);
+}
+
+}  // extern "C"

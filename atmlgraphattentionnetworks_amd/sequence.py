@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["layer_norm", "embedding", "LayerNorm", "Embedding"]
+__all__ = ["layer_norm", "embedding", "packed_attention", "LayerNorm", "Embedding"]
 
 _DTYPES = {torch.float32: _lib.GAT_F32, torch.bfloat16: _lib.GAT_BF16,
            torch.float16: _lib.GAT_F16}
@@ -260,3 +260,147 @@ class Embedding(torch.nn.Module):
 
     def extra_repr(self) -> str:
         return f"{self.num_embeddings}, {self.embedding_dim}, scale={self.scale}"
+
+
+# ---------------------------------------------------------------------------
+# Attention over packed sequences
+# ---------------------------------------------------------------------------
+def _vectors(t: torch.Tensor) -> torch.Tensor:
+    """[tokens, heads, dim] as the kernels read it: adjacent dimensions, rows of whole
+    16-byte vectors on 16-byte boundaries.  ``t`` itself where it is that already (a view
+    of a fused projection's output, say), else a copy padded with zeros."""
+    n = 16 // t.element_size()
+    d = t.shape[2]
+    if d % n == 0 and t.stride(2) == 1 and t.stride(0) % n == 0 and t.stride(1) % n == 0 \
+            and t.data_ptr() % 16 == 0:
+        return t
+    if d % n == 0:
+        return t.clone(memory_format=torch.contiguous_format)
+    return torch.nn.functional.pad(t, (0, -d % n))
+
+
+def _attn_forward(q, k, v, ptr, kv_ptr, causal, scale, want_lse):
+    """``q``, ``k``, ``v`` as :func:`_vectors` gives them."""
+    nq, h, d = q.shape
+    nk, hk = k.shape[:2]
+    dev, dt, count = q.device, _DTYPES[q.dtype], ptr.numel() - 1
+    out = torch.empty(nq, h, d, dtype=q.dtype, device=dev)
+    lse = torch.empty(nq, h, dtype=torch.float32, device=dev) if want_lse else None
+    size = _lib.packed_attention_workspace_size(False, nq, nk, count, h, hk, d, dt)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    with _on(dev):
+        rc = _lib.load().gat_packed_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+            v.data_ptr(), v.stride(0), v.stride(1), ptr.data_ptr(), kv_ptr.data_ptr(),
+            int(ptr.dtype == torch.int64), count, nq, nk, h, hk, d, scale, int(causal),
+            out.data_ptr(), _ptr(lse), _ptr(ws), size, dt, _stream(dev))
+    if rc:
+        _lib.check(rc, "gat_packed_attention")
+    return out, lse
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, ptr, kv_ptr, causal, scale):
+        d = q.shape[2]
+        q, k, v = _vectors(q), _vectors(k), _vectors(v)
+        out, lse = _attn_forward(q, k, v, ptr, kv_ptr, causal, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, ptr, kv_ptr)
+        ctx.causal, ctx.scale, ctx.dim = causal, scale, d
+        ctx.mark_non_differentiable(lse)
+        return (out if out.shape[2] == d else out[..., :d].contiguous()), lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _):
+        q, k, v, out, lse, ptr, kv_ptr = ctx.saved_tensors
+        g = _vectors(g)
+        nq, h, d = q.shape
+        nk, hk = k.shape[:2]
+        dev, dt, count = q.device, _DTYPES[q.dtype], ptr.numel() - 1
+        dq = torch.empty(nq, h, d, dtype=q.dtype, device=dev)
+        dk, dv = (torch.empty(nk, hk, d, dtype=q.dtype, device=dev) for _ in range(2))
+        size = _lib.packed_attention_workspace_size(True, nq, nk, count, h, hk, d, dt)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        with _on(dev):
+            rc = _lib.load().gat_packed_attention_backward(
+                g.data_ptr(), g.stride(0), g.stride(1), q.data_ptr(), q.stride(0), q.stride(1),
+                k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                out.data_ptr(), lse.data_ptr(), ptr.data_ptr(), kv_ptr.data_ptr(),
+                int(ptr.dtype == torch.int64), count, nq, nk, h, hk, d, ctx.scale,
+                int(ctx.causal), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), size,
+                dt, _stream(dev))
+        if rc:
+            _lib.check(rc, "gat_packed_attention_backward")
+        if ctx.dim != d:
+            dq, dk, dv = (t[..., :ctx.dim] for t in (dq, dk, dv))
+        return dq, dk, dv, None, None, None, None
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: torch.Tensor,
+                     kv_ptr: Optional[torch.Tensor] = None, causal: bool = False,
+                     scale: Optional[float] = None, return_lse: bool = False):
+    """Softmax attention of every query over the keys of its own sequence.
+
+    ``q`` is ``[queries, heads, dim]``, ``k`` and ``v`` ``[keys, kv_heads, dim]`` (float32 or
+    bfloat16; ``heads`` a multiple of ``kv_heads``, query head ``h`` reads key head
+    ``h // (heads // kv_heads)``; ``dim`` up to 128).  Sequence ``b`` has the queries
+    ``ptr[b]:ptr[b + 1]`` and the keys ``kv_ptr[b]:kv_ptr[b + 1]``; ``ptr`` is an ascending
+    int32 or int64 device tensor of ``count + 1`` offsets (a batch of graphs:
+    ``GraphData.ptr()``), ``kv_ptr`` defaults to it.  One query per sequence (a readout
+    over a graph's nodes, the next token of a text) is the same call with
+    ``ptr = arange(count + 1)``; a few queries over many keys are split over the keys.
+
+    ``causal``: the last query sees all keys of its sequence, each earlier one a key less
+    (key ``j`` is visible to query ``i`` iff ``j <= i + keys - queries``).  ``scale``
+    defaults to ``dim ** -0.5``.  Queries that see no key, and rows outside all sequences,
+    give zeros.  Offsets are not checked on the host: values outside the tensors are held
+    to them, descending ones give undefined results (but touch nothing outside).
+
+    Returns the output ``[queries, heads, dim]``, with ``return_lse`` also the float32
+    ``[queries, heads]`` logarithm of each softmax sum (-inf where no key is seen; not
+    differentiable).  Differentiable in ``q``, ``k`` and ``v``.  Scores, softmax sums and
+    accumulators are float32; in bfloat16 the probabilities and the scores' gradients are
+    rounded to bfloat16 for the second matrix product.  Inputs may be strided views
+    (16-byte aligned rows are read in place, others are copied)."""
+    kinds = (torch.float32, torch.bfloat16)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _need_tensor("packed_attention", name, t, kinds)
+        if t.dim() != 3:
+            raise ValueError(f"packed_attention: {name} must be [tokens, heads, dim], "
+                             f"got {tuple(t.shape)}")
+        if t is not q:
+            _need_like("packed_attention", name, t, q)
+    kv_ptr = ptr if kv_ptr is None else kv_ptr
+    for name, t in (("ptr", ptr), ("kv_ptr", kv_ptr)):
+        _need_tensor("packed_attention", name, t, (torch.int32, torch.int64))
+        _need_like("packed_attention", name, t, q, dtype=False)
+        if t.dim() != 1 or t.numel() < 1:
+            raise ValueError(f"packed_attention: {name} must hold count + 1 offsets, "
+                             f"got {tuple(t.shape)}")
+    if ptr.numel() != kv_ptr.numel():
+        raise ValueError(f"packed_attention: ptr has {ptr.numel()} offsets, kv_ptr {kv_ptr.numel()}")
+    nq, h, d = q.shape
+    nk, hk = k.shape[:2]
+    if v.shape != k.shape or k.shape[2] != d:
+        raise ValueError(f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and "
+                         f"v {tuple(v.shape)} do not fit: k and v alike, dim as q's")
+    if hk == 0 or h == 0 or h % hk:
+        raise ValueError(f"packed_attention: {h} query heads over {hk} key heads")
+    if not 1 <= d <= 128 or hk > 65535:
+        raise ValueError(f"packed_attention: dim must be 1 to 128 and kv_heads at most 65535, "
+                         f"got {d} and {hk}")
+    if max(nq * (h // hk), nk) >= 1 << 30:
+        raise ValueError("packed_attention: queries * heads / kv_heads and keys must be "
+                         "below 2^30")
+    if ptr.dtype != kv_ptr.dtype:
+        ptr, kv_ptr = ptr.long(), kv_ptr.long()
+    ptr, kv_ptr = ptr.contiguous(), kv_ptr.contiguous()
+    scale = float(d) ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _PackedAttention.apply(q, k, v, ptr, kv_ptr, bool(causal), scale)
+        return (out, lse) if return_lse else out
+    out, lse = _attn_forward(_vectors(q), _vectors(k), _vectors(v), ptr, kv_ptr, bool(causal),
+                             scale, return_lse)
+    out = out if out.shape[2] == d else out[..., :d].contiguous()
+    return (out, lse) if return_lse else out

@@ -579,7 +579,7 @@ int gat_sum_partials(const float* partials, int num_parts, long long width, floa
                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
- * Packed-sequence operators (ABI 13): layer norm, embedding.
+ * Packed-sequence operators (ABI 13): layer norm, embedding, attention.
  * Tensors hold float32, bfloat16 or float16 (GAT_F32 / GAT_BF16 / GAT_F16); sums and
  * statistics are float32, results are rounded once.
  * ------------------------------------------------------------------------- */
@@ -638,6 +638,51 @@ int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void*
                        int vocab, int cols, float scale, long long padding, void* dw,
                        long long ld_dw, void* workspace, size_t workspace_bytes, int dtype,
                        void* stream);
+
+/*
+ * Attention over packed sequences.  Sequence b (of `count`) has the queries
+ * ptr[b] .. ptr[b + 1] and the keys kv_ptr[b] .. kv_ptr[b + 1]; query head h reads key
+ * head h / (heads / kv_heads):
+ *   out = softmax(scale q k^T) v over the sequence's visible keys
+ * causal: key j of a sequence is visible to its query i iff j <= i + (keys - queries).
+ *   q        [nq, heads, dim], k, v [nk, kv_heads, dim]: GAT_F32 or GAT_BF16, token and head
+ *            strides in elements; addresses and strides multiples of 16 bytes, dim a
+ *            multiple of 16 bytes of elements and <= GAT_PACKED_MAX_DIM (GAT_EUNSUPPORTED
+ *            otherwise); heads a multiple of kv_heads
+ *   ptr, kv_ptr  [count + 1] int64 if ptr64, else int32, ascending.  Boundaries outside
+ *            [0, nq] / [0, nk] are held to it: nothing outside the tensors is touched.
+ *   out      [nq, heads, dim] contiguous.  Queries that see no key (an empty sequence, causal
+ *            queries before the first key) and rows outside all sequences: zeros
+ *   lse      [nq, heads] float32 log of the softmax sum (-inf where no key is seen);
+ *            may be NULL
+ *   workspace  16-byte aligned, gat_packed_attention_workspace_size bytes
+ */
+#define GAT_PACKED_MAX_DIM 128
+int gat_packed_attention_workspace_size(int nq, int nk, int count, int heads, int kv_heads, int dim,
+                                        int dtype, size_t* bytes);
+int gat_packed_attention(const void* q, long long q_row, long long q_head, const void* k,
+                         long long k_row, long long k_head, const void* v, long long v_row,
+                         long long v_head, const void* ptr, const void* kv_ptr, int ptr64, int count,
+                         int nq, int nk, int heads, int kv_heads, int dim, float scale, int causal,
+                         void* out, float* lse, void* workspace, size_t workspace_bytes, int dtype,
+                         void* stream);
+
+/*
+ * Gradients of gat_packed_attention for the incoming gradient g [nq, heads, dim] (strides as
+ * q's); out and lse as the forward stored them.  dq [nq, heads, dim], dk, dv
+ * [nk, kv_heads, dim] contiguous; dk and dv are sums over the query heads of a key head.
+ * Rows outside all sequences get zeros.  Deterministic.
+ */
+int gat_packed_attention_backward_workspace_size(int nq, int nk, int count, int heads, int kv_heads,
+                                                 int dim, int dtype, size_t* bytes);
+int gat_packed_attention_backward(const void* g, long long g_row, long long g_head, const void* q,
+                                  long long q_row, long long q_head, const void* k, long long k_row,
+                                  long long k_head, const void* v, long long v_row, long long v_head,
+                                  const void* out, const float* lse, const void* ptr,
+                                  const void* kv_ptr, int ptr64, int count, int nq, int nk, int heads,
+                                  int kv_heads, int dim, float scale, int causal, void* dq, void* dk,
+                                  void* dv, void* workspace, size_t workspace_bytes, int dtype,
+                                  void* stream);
 
 #ifdef __cplusplus
 }
