@@ -24,10 +24,11 @@
 
 namespace {
 
-constexpr int kSortBlock = 256;  // one thread per digit in the sums
+constexpr int kSortBlock = 1024;
+constexpr int kSortWaves = kSortBlock / kWave;
 constexpr int kSortMinItems = 1024;
 constexpr int kSortMaxBlocks = 256;
-constexpr int kPiece = 128;
+constexpr int kPiece = 32;
 constexpr long long kMaxTokens = 1ll << 30;
 constexpr int kEmbedBlock = 256;
 
@@ -81,7 +82,7 @@ template <bool FIRST>
 __global__ __launch_bounds__(kSortBlock) void k_sort_count(Ids s, const unsigned* keys, int n,
                                                            int per, int shift, unsigned* counts) {
     __shared__ unsigned h[256];
-    h[threadIdx.x] = 0;
+    if (threadIdx.x < 256) h[threadIdx.x] = 0;
     __syncthreads();
     const int a = blockIdx.x * per, e = a + per < n ? a + per : n;
     for (int i = a + threadIdx.x; i < e; i += kSortBlock) {
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(kSortBlock) void k_sort_count(Ids s, const unsigned
         atomicAdd(&h[(k >> shift) & 255], 1u);
     }
     __syncthreads();
-    counts[blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
+    if (threadIdx.x < 256) counts[blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
 }
 
 template <bool FIRST>
@@ -97,30 +98,49 @@ __global__ __launch_bounds__(kSortBlock) void k_sort_place(Ids s, const unsigned
                                                            const unsigned* toks, int n, int per,
                                                            int shift, const unsigned* counts,
                                                            unsigned* keys_out, unsigned* toks_out) {
-    __shared__ unsigned base[256], wave_count[4][256], scan[256];
-    const int d = threadIdx.x, lane = d % kWave, wave = d / kWave;
-    unsigned before = 0, total = 0;  // of digit d: in the workgroups before, in all
+    __shared__ unsigned base[256], wave_count[kSortWaves][256], sums[2][4][256];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    {
+        // of digit d: its count in the workgroups before this one and in all, by four
+        // threads a digit
+        const int d = tid % 256, quarter = tid / 256;
+        unsigned before = 0, total = 0;
 #pragma unroll 8
-    for (int b = 0; b < (int)gridDim.x; ++b) {
-        const unsigned c = counts[b * 256 + d];
-        before += b < (int)blockIdx.x ? c : 0;
-        total += c;
+        for (int b = quarter; b < (int)gridDim.x; b += 4) {
+            const unsigned c = counts[b * 256 + d];
+            before += b < (int)blockIdx.x ? c : 0;
+            total += c;
+        }
+        sums[0][quarter][d] = before;
+        sums[1][quarter][d] = total;
     }
-    scan[d] = total;
     __syncthreads();
-    for (int off = 1; off < 256; off <<= 1) {
-        const unsigned v = d >= off ? scan[d - off] : 0;
-        __syncthreads();
-        scan[d] += v;
-        __syncthreads();
+    if (wave == 0) {  // where each digit begins: lane l adds up digits 4 l .. 4 l + 3
+        unsigned t[4], all = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int d = 4 * lane + k;
+            t[k] = all;
+            all += sums[1][0][d] + sums[1][1][d] + sums[1][2][d] + sums[1][3][d];
+        }
+        unsigned upto = all;
+#pragma unroll
+        for (int off = 1; off < kWave; off <<= 1) {
+            const unsigned v = __shfl_up(upto, off);
+            if (lane >= off) upto += v;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int d = 4 * lane + k;
+            base[d] = upto - all + t[k] + sums[0][0][d] + sums[0][1][d] + sums[0][2][d] + sums[0][3][d];
+        }
     }
-    base[d] = scan[d] - total + before;
     const int a = blockIdx.x * per, e = a + per < n ? a + per : n;
     for (int i0 = a; i0 < e; i0 += kSortBlock) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) wave_count[k][d] = 0;
+        for (int k = 0; k < 4; ++k) wave_count[wave][4 * lane + k] = 0;
         __syncthreads();
-        const int i = i0 + d;
+        const int i = i0 + tid;
         const bool in = i < e;
         const unsigned key = in ? (FIRST ? key_at(s, i) : keys[i]) : 0;
         const unsigned digit = (key >> shift) & 255;
@@ -141,7 +161,13 @@ __global__ __launch_bounds__(kSortBlock) void k_sort_place(Ids s, const unsigned
             toks_out[at] = FIRST ? (unsigned)i : toks[i];
         }
         __syncthreads();
-        base[d] += wave_count[0][d] + wave_count[1][d] + wave_count[2][d] + wave_count[3][d];
+        if (tid < 256) {
+            unsigned c = 0;
+#pragma unroll
+            for (int k = 0; k < kSortWaves; ++k) c += wave_count[k][tid];
+            base[tid] += c;
+        }
+        __syncthreads();
     }
 }
 
@@ -172,27 +198,23 @@ __global__ __launch_bounds__(256) void k_sort_firsts(const unsigned* keys, int n
 // ---------------------------------------------------------------------------
 
 // acc += the rows of g of sorted tokens [a, e), `step` apart, columns [c, c + N)
-template <typename T>
+template <typename T, int U = 8>
 __device__ __forceinline__ void add_rows(float (&acc)[Vec16<T>::N], const T* g, long long ld_g,
                                          const unsigned* toks, int a, int e, int step, int c,
                                          int cols, bool whole) {
-    constexpr int N = Vec16<T>::N, U = 4;
-    int i = a;
-    for (; i + (U - 1) * step < e; i += U * step) {
+    constexpr int N = Vec16<T>::N;
+    for (int i = a; i < e; i += U * step) {  // U rows in flight, also where fewer are left
         typename Vec16<T>::type v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            v[u] = load_vec<T>(g + (long long)toks[i + u * step] * ld_g, c, cols, whole);
+        for (int u = 0; u < U; ++u) {
+            v[u] = typename Vec16<T>::type{};
+            if (i + u * step < e)
+                v[u] = load_vec<T>(g + (long long)toks[i + u * step] * ld_g, c, cols, whole);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int k = 0; k < N; ++k) acc[k] += (float)v[u][k];
-    }
-    for (; i < e; i += step) {
-        const typename Vec16<T>::type v =
-            load_vec<T>(g + (long long)toks[i] * ld_g, c, cols, whole);
-#pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += (float)v[k];
     }
 }
 
@@ -262,7 +284,7 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_join(const unsigned* keys
     const int last = (l - 1) / kPiece;
     float acc[N] = {};
     if (c < cols) {
-#pragma unroll 2
+#pragma unroll 8
         for (int p = j + grp; p <= last; p += kEmbedBlock / LPR) {
             const float* row = part + (size_t)(2 * p + (p == j && f != a ? 1 : 0)) * cols;
 #pragma unroll
@@ -284,19 +306,39 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_rows(const unsigned* toks
                                                             int vocab, const T* g, long long ld_g,
                                                             int whole_g, int cols, float scale,
                                                             T* dw, long long ld_dw, int whole) {
-    constexpr int N = Vec16<T>::N;
+    // two table rows a group: the loads of both fly together (most have few tokens)
+    constexpr int N = Vec16<T>::N, U = 4;
+    typedef typename Vec16<T>::type V;
     const int lane = threadIdx.x % LPR;
-    const int v = blockIdx.x * (kEmbedBlock / LPR) + threadIdx.x / LPR;
-    if (v >= vocab) return;
-    const int a = first[v], e = first[v + 1];
-    if (e - a > kPiece) return;
-    for (int c = lane * N; c < cols; c += LPR * N) {
+    const int v = (blockIdx.x * (kEmbedBlock / LPR) + threadIdx.x / LPR) * 2;
+    const int c = (blockIdx.y * LPR + lane) * N;
+    if (v >= vocab || c >= cols) return;
+    int at[3];
+    at[0] = first[v];
+    at[1] = first[v + 1];
+    at[2] = v + 1 < vocab ? first[v + 2] : at[1];
+    V x[2][U];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            x[r][u] = V{};
+            if (at[r] + u < at[r + 1] && at[r + 1] - at[r] <= kPiece)
+                x[r][u] = load_vec<T>(g + (long long)toks[at[r] + u] * ld_g, c, cols, whole_g);
+        }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        if (v + r >= vocab || at[r + 1] - at[r] > kPiece) continue;
         float acc[N] = {};
-        add_rows<T>(acc, g, ld_g, toks, a, e, 1, c, cols, whole_g);
-        typename Vec16<T>::type y;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k] += (float)x[r][u][k];
+        add_rows<T>(acc, g, ld_g, toks, at[r] + U, at[r + 1], 1, c, cols, whole_g);
+        V y;
 #pragma unroll
         for (int k = 0; k < N; ++k) y[k] = (T)(acc[k] * scale);
-        store_vec<T>(dw + (long long)v * ld_dw, c, cols, whole, y);
+        store_vec<T>(dw + (long long)(v + r) * ld_dw, c, cols, whole, y);
     }
 }
 
@@ -364,7 +406,7 @@ int embed_grad_sums(const unsigned* keys, const unsigned* toks, const int* first
             keys, first, n, vocab, cols, part, scale, dw, ld_dw, whole);
     }
     constexpr int RPB = kEmbedBlock / LPR;
-    k_embed_rows<T, LPR><<<(vocab + RPB - 1) / RPB, kEmbedBlock, 0, s>>>(
+    k_embed_rows<T, LPR><<<dim3(((vocab + 1) / 2 + RPB - 1) / RPB, slabs), kEmbedBlock, 0, s>>>(
         toks, first, vocab, g, ld_g, whole_g, cols, scale, dw, ld_dw, whole);
     return status_of(hipGetLastError());
 }

@@ -12,7 +12,7 @@
 // the mean of the squared deviations, not a difference of two large sums.
 //
 // A row belongs to LPR lanes (8 to 64 lanes of a wave, or a whole workgroup of 256
-// for rows over 64 * 4 vectors) with NV vectors each; the groups walk the rows with
+// for rows over 128 vectors) with NV vectors each; the groups walk the rows with
 // a stride that is a multiple of 8 rows, so a group's rows all start at the same
 // offset from a 16-byte boundary and a lane keeps the same columns: w, b and the
 // sums of dw and db stay in registers over the group's rows, also where the row
@@ -47,11 +47,8 @@ struct NormArgs {
 template <int LPR>
 __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2]) {
     constexpr int W = LPR < kWave ? LPR : kWave;
-#pragma unroll
-    for (int off = 1; off < W; off <<= 1) {
-        a += __shfl_xor(a, off);
-        b += __shfl_xor(b, off);
-    }
+    a = lanes_sum<W>(a);
+    b = lanes_sum<W>(b);
     if constexpr (LPR > kWave) {
         const int wave = threadIdx.x / kWave;
         if (threadIdx.x % kWave == 0) {
@@ -68,40 +65,71 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[2]) {
     }
 }
 
+// A lane's columns of w or b.  Where the row does not start on a 16-byte boundary they lie
+// across the vectors of w: then the workgroup's copy in LDS (LPR <= 64) is read element by
+// element instead of memory.
+template <typename T, int LPR, int NV>
+__device__ __forceinline__ void load_params(typename Vec16<T>::type* out, const void* from, float none,
+                                            int phase, int cols, T* lds) {
+    constexpr int N = Vec16<T>::N;
+    const int lane = threadIdx.x % LPR;
+    const T* w = static_cast<const T*>(from);
+    if (w == nullptr) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int c = (i * LPR + lane) * N - phase + e;
+                out[i][e] = c >= 0 && c < cols ? (T)none : (T)0.f;
+            }
+        return;
+    }
+    if constexpr (LPR <= kWave) {
+        __syncthreads();
+        for (int c = threadIdx.x; c < cols; c += kNormBlock) lds[c] = w[c];
+        __syncthreads();
+        w = lds;
+    }
+    const bool whole = LPR > kWave && phase == 0 && phase_of(w) == 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) out[i] = load_vec<T>(w, (i * LPR + lane) * N - phase, cols, whole);
+}
+
 template <typename T, int LPR, int NV>
 __global__ __launch_bounds__(kNormBlock) void k_norm_fwd(NormArgs p) {
     constexpr int N = Vec16<T>::N;
     constexpr int RPB = kNormBlock / LPR;
     typedef typename Vec16<T>::type V;
     __shared__ float red[4][4][2];
+    __shared__ T wl[LPR <= kWave ? LPR * NV * N : 1];
     const int lane = threadIdx.x % LPR;
     const int group = blockIdx.x * RPB + threadIdx.x / LPR;
     const int groups = gridDim.x * RPB;
     const T* x = static_cast<const T*>(p.x);
     const int phase = phase_of(x + (long long)group * p.ld_x);
-    float w[NV][N], b[NV][N];
+    constexpr bool AHEAD = NV <= 4;  // the next row's loads fly meanwhile, registers permitting
+    V v[NV], next[NV], w[NV], b[NV];
+    auto load_row = [&](V* to, long long row) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const int c = (i * LPR + lane) * N - phase + e;
-            const bool in = c >= 0 && c < p.cols;
-            w[i][e] = in ? (p.w != nullptr ? (float)static_cast<const T*>(p.w)[c] : 1.f) : 0.f;
-            b[i][e] = in && p.b != nullptr ? (float)static_cast<const T*>(p.b)[c] : 0.f;
-        }
+        for (int i = 0; i < NV; ++i)
+            to[i] = load_vec<T>(x + row * p.ld_x, (i * LPR + lane) * N - phase, p.cols, true);
+    };
+    if (AHEAD && group < p.rows) load_row(next, group);
+    load_params<T, LPR, NV>(w, p.w, 1.f, phase, p.cols, wl);
+    load_params<T, LPR, NV>(b, p.b, 0.f, phase, p.cols, wl);
     const float inv = 1.f / (float)p.cols;
     int turn = 0;
     // groups of one workgroup leave together where they meet at barriers (LPR = 256)
     for (long long row = group; row < p.rows; row += groups, turn ^= 2) {
-        const T* xr = x + row * p.ld_x;
-        V v[NV];
         float s = 0.f, unused = 0.f;
+        if (!AHEAD) load_row(next, row);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            v[i] = load_vec<T>(xr, (i * LPR + lane) * N - phase, p.cols, true);
+            v[i] = next[i];
 #pragma unroll
             for (int e = 0; e < N; ++e) s += (float)v[i][e];
         }
+        if (AHEAD && row + groups < p.rows) load_row(next, row + groups);
         row_sum2<LPR>(s, unused, red[turn]);
         const float mean = s * inv;
         float q = 0.f;
@@ -125,7 +153,7 @@ __global__ __launch_bounds__(kNormBlock) void k_norm_fwd(NormArgs p) {
             V y;
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                y[e] = (T)(((float)v[i][e] - mean) * r * w[i][e] + b[i][e]);
+                y[e] = (T)(((float)v[i][e] - mean) * r * (float)w[i][e] + (float)b[i][e]);
             store_vec<T>(yr, (i * LPR + lane) * N - phase, p.cols, p.whole_out, y);
         }
     }
@@ -136,45 +164,49 @@ __global__ __launch_bounds__(kNormBlock) void k_norm_bwd(NormArgs p) {
     constexpr int N = Vec16<T>::N;
     constexpr int RPB = kNormBlock / LPR;
     typedef typename Vec16<T>::type V;
-    __shared__ float red[4][4][2];
     constexpr int COLS = LPR * NV * N;
-    __shared__ float cs[RPB > 1 ? 2 * COLS : 1];
+    __shared__ float red[4][4][2];
+    __shared__ __align__(16) float cs[RPB > 1 ? 2 * COLS : 1];
     const int lane = threadIdx.x % LPR;
     const int group = blockIdx.x * RPB + threadIdx.x / LPR;
     const int groups = gridDim.x * RPB;
     const T* x = static_cast<const T*>(p.x);
     const int phase = phase_of(x + (long long)group * p.ld_x);
-    V w[NV];
-    float dw[NV][N], db[NV][N];
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const int c = (i * LPR + lane) * N - phase + e;
-            const bool in = c >= 0 && c < p.cols;
-            w[i][e] = in ? (p.w != nullptr ? static_cast<const T*>(p.w)[c] : (T)1.f) : (T)0.f;
-            dw[i][e] = db[i][e] = 0.f;
-        }
-    const float inv = 1.f / (float)p.cols;
-    int turn = 0;
-    for (long long row = group; row < p.rows; row += groups, turn ^= 1) {
-        const T* xr = x + row * p.ld_x;
+    constexpr bool AHEAD = NV <= 2;
+    V v[NV], g[NV], vn[NV], gn[NV], w[NV];
+    float mean = 0.f, r = 0.f;
+    auto load_row = [&](long long row) {
         const T* gr = static_cast<const T*>(p.g) + row * p.ld_g;
-        V v[NV], g[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c0 = (i * LPR + lane) * N - phase;
-            v[i] = load_vec<T>(xr, c0, p.cols, true);
-            g[i] = load_vec<T>(gr, c0, p.cols, p.whole_g);
+            vn[i] = load_vec<T>(x + row * p.ld_x, c0, p.cols, true);
+            gn[i] = load_vec<T>(gr, c0, p.cols, p.whole_g);
         }
-        const float mean = p.stats[2 * row], r = p.stats[2 * row + 1];
+        mean = p.stats[2 * row];
+        r = p.stats[2 * row + 1];
+    };
+    if (AHEAD && group < p.rows) load_row(group);
+    load_params<T, LPR, NV>(w, p.w, 1.f, phase, p.cols, reinterpret_cast<T*>(cs));
+    float dw[NV][N] = {}, db[NV][N] = {};
+    const float inv = 1.f / (float)p.cols;
+    int turn = 0;
+    for (long long row = group; row < p.rows; row += groups, turn ^= 1) {
+        if (!AHEAD) load_row(row);
+        const float m = mean, rs = r;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            v[i] = vn[i];
+            g[i] = gn[i];
+        }
+        if (AHEAD && row + groups < p.rows) load_row(row + groups);
         float sh = 0.f, shz = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 // outside the row g and w are 0, so nothing is added there
-                const float z = ((float)v[i][e] - mean) * r;
+                const float z = ((float)v[i][e] - m) * rs;
                 const float h = (float)g[i][e] * (float)w[i][e];
                 sh += h;
                 shz += h * z;
@@ -191,8 +223,8 @@ __global__ __launch_bounds__(kNormBlock) void k_norm_bwd(NormArgs p) {
                 V d;
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const float z = ((float)v[i][e] - mean) * r;
-                    d[e] = (T)(r * ((float)g[i][e] * (float)w[i][e] - sh - z * shz));
+                    const float z = ((float)v[i][e] - m) * rs;
+                    d[e] = (T)(rs * ((float)g[i][e] * (float)w[i][e] - sh - z * shz));
                 }
                 store_vec<T>(dr, (i * LPR + lane) * N - phase, p.cols, p.whole_out, d);
             }
@@ -211,6 +243,7 @@ __global__ __launch_bounds__(kNormBlock) void k_norm_bwd(NormArgs p) {
                 part[p.cols + c] = db[i][e];
             }
     } else {
+        __syncthreads();  // cs held w
         // The groups' columns may be shifted against each other (odd row lengths), so
         // they take turns: group j adds its sums to those of the groups before it.
         for (int j = 0; j < RPB; ++j) {
@@ -277,7 +310,7 @@ inline NormShape norm_shape(int cols, int dtype, bool aligned) {
     if (vecs <= 32) return {32, 1};
     if (vecs <= 64) return {64, 1};
     if (vecs <= 128) return {64, 2};
-    if (vecs <= 256) return {64, 4};
+    if (vecs <= 256) return {256, 1};
     if (vecs <= 512) return {256, 2};
     if (vecs <= 1024) return {256, 4};
     if (vecs <= 2048) return {256, 8};
@@ -294,10 +327,10 @@ inline int norm_grid(int rows, int lpr, int most) {
     return (int)((g + step - 1) / step * step);
 }
 
-// Most workgroups of the two directions; the backward's each leave a partial row of
-// 2 * cols sums.
+// Most workgroups of the two directions (what is resident at once; the backward's each
+// leave a partial row of 2 * cols sums).
 constexpr int kNormFwdGrid = 2048;
-constexpr int kNormBwdGrid = 512;
+constexpr int kNormBwdGrid = 1024;
 
 template <typename T, bool BWD>
 hipError_t norm_launch(const NormShape& sh, const NormArgs& a, hipStream_t s) {
@@ -315,7 +348,7 @@ hipError_t norm_launch(const NormShape& sh, const NormArgs& a, hipStream_t s) {
     GAT_NORM_CASE(32, 1)
     GAT_NORM_CASE(64, 1)
     GAT_NORM_CASE(64, 2)
-    GAT_NORM_CASE(64, 4)
+    GAT_NORM_CASE(256, 1)
     GAT_NORM_CASE(256, 2)
     GAT_NORM_CASE(256, 4)
     GAT_NORM_CASE(256, 8)

@@ -128,11 +128,20 @@ __device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {
 template <typename T, int DP>
 struct Shape {
     static constexpr int N = Vec16<T>::N;
-    static constexpr int STEPS = DP / (2 * N);       // products of a 32x32 score tile
-    static constexpr int DT = (DP + 31) / 32;        // 32-wide tiles of the head dimension
-    static constexpr int LD = DP + N;                // LDS row: a vector of padding spreads the banks
-    static constexpr int CPR = DP / N;               // vectors of a row
-    static constexpr int slab(int rows) { return rows * LD + 32; }  // the last tile may read past DP
+    static constexpr int STEPS = DP / (2 * N);  // products of a 32x32 score tile
+    static constexpr int DT = (DP + 31) / 32;   // 32-wide tiles of the head dimension
+    static constexpr int CPR = DP / N;          // 16-byte vectors of a row
+    // A tile of `rows` in LDS, rows without gaps (as the loads to LDS write them).  Vector c
+    // of row r lies at place c ^ turn(r): reads of one vector of 8 rows, and transposing
+    // reads of 4 rows, then meet all banks.  The last tile of the head dimension may read
+    // past DP, into what follows.
+    static constexpr int slab(int rows) { return rows * DP; }
+    static constexpr int kSlack = 32;
+    static __device__ __forceinline__ int turn(int r) {
+        if constexpr (CPR % 8 == 0) return (r & 3) << 1 | (r >> 2 & 1);
+        if constexpr (CPR % 4 == 0) return r >> 1 & 3;
+        return r >> 2 & 1;
+    }
 };
 
 // scores[row][col] of 32 rows in LDS against the wave's columns
@@ -140,11 +149,12 @@ template <typename T, int DP>
 __device__ __forceinline__ f32x16 scores(const T* rows, const typename Vec16<T>::type* cols) {
     typedef Shape<T, DP> S;
     const int lane = threadIdx.x % kWave;
-    const T* at = rows + (lane % 32) * S::LD + (lane / 32) * S::N;
+    const T* at = rows + lane % 32 * DP;
+    const int place = (lane / 32) ^ S::turn(lane % 32);
     f32x16 c = {};
 #pragma unroll
     for (int s = 0; s < S::STEPS; ++s)
-        c = mma(*reinterpret_cast<const typename Vec16<T>::type*>(at + s * 2 * S::N), cols[s], c);
+        c = mma(*reinterpret_cast<const typename Vec16<T>::type*>(at + ((2 * s) ^ place) * S::N), cols[s], c);
     return c;
 }
 
@@ -160,8 +170,9 @@ template <int DP>
 __device__ __forceinline__ void add_products(f32x16* acc, const bf16* rows, const f32x16& w) {
     typedef Shape<bf16, DP> S;
     const int lane = threadIdx.x % kWave;
-    const bf16* at = rows + (4 * (lane / 32) + lane % 16 / 4) * S::LD + lane % 32 / 16 * 16 +
-                     lane % 4 * 4;
+    const int row = 4 * (lane / 32) + lane % 16 / 4;  // all rows read have row's low three bits
+    const bf16* at = rows + row * DP + lane % 2 * 4;
+    const int place = (lane % 32 / 16 * 2 + lane % 4 / 2) ^ S::turn(row);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         bf16x8 b;
@@ -169,8 +180,9 @@ __device__ __forceinline__ void add_products(f32x16* acc, const bf16* rows, cons
         for (int e = 0; e < 8; ++e) b[e] = (bf16)w[8 * s + e];
 #pragma unroll
         for (int t = 0; t < S::DT; ++t) {
-            const bf16x4 lo = read_transposed(at + 16 * s * S::LD + 32 * t);
-            const bf16x4 hi = read_transposed(at + (16 * s + 8) * S::LD + 32 * t);
+            const bf16* x = at + 16 * s * DP + ((4 * t) ^ place) * 8;
+            const bf16x4 lo = read_transposed(x);
+            const bf16x4 hi = read_transposed(x + 8 * DP);
             acc[t] = mma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b, acc[t]);
         }
     }
@@ -178,14 +190,15 @@ __device__ __forceinline__ void add_products(f32x16* acc, const bf16* rows, cons
 template <int DP>
 __device__ __forceinline__ void add_products(f32x16* acc, const float* rows, const f32x16& w) {
     typedef Shape<float, DP> S;
-    const int lane = threadIdx.x % kWave;
-    const float* at = rows + 4 * (lane / 32) * S::LD + lane % 32;
+    const int lane = threadIdx.x % kWave, half = lane / 32, d = lane % 32;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 16; ++i) {
+        const int row = 8 * (i / 4) + 4 * half + i % 4;
+        const float* x = rows + row * DP + (d / 4 ^ S::turn(row)) * 4 + d % 4;
 #pragma unroll
         for (int t = 0; t < S::DT; ++t)
-            acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[(8 * (i / 4) + i % 4) * S::LD + 32 * t],
-                                                          w[i], acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[32 * t], w[i], acc[t], 0, 0, 0);
+    }
 }
 
 // row within the 32 of register i of a product
@@ -210,7 +223,7 @@ __device__ __forceinline__ void load_columns(typename Vec16<T>::type* cols, cons
 // ---------------------------------------------------------------------------
 // Causal tiles that some column of the workgroup does not see in whole: a hidden row has
 // W = 0, but 0 times an infinity or NaN in its X would still reach the column.  Such a
-// tile is looked over as it is stored (`bad` takes its number); when it holds one, its
+// tile is looked over when it has arrived (`bad` takes its number); when it holds one, its
 // non-finite values are cleared in LDS once the scores are formed, and after the matrix
 // product their share is added for the rows that are seen.  All other rows get the same
 // bits as from a finite tile.
@@ -219,19 +232,24 @@ __device__ __forceinline__ bool non_finite(float v) {
     return (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u;
 }
 
-template <typename T, int DP, int NW, int BN>
-__device__ __forceinline__ void clear_non_finite(T* lds) {
+// Whether a tile holds an infinity or NaN: *bad = tag.  CLEAR: puts zeros in their place.
+template <typename T, int DP, int NW, int BN, bool CLEAR>
+__device__ __forceinline__ void look_over(T* lds, int* bad, int tag) {
     typedef Shape<T, DP> S;
     typedef typename Vec16<T>::type V;
+    bool any = false;
 #pragma unroll 1
     for (int at = threadIdx.x; at < BN * S::CPR; at += NW * kWave) {
-        V* p = reinterpret_cast<V*>(lds + at / S::CPR * S::LD + at % S::CPR * S::N);
-        V x = *p;
+        V x = reinterpret_cast<V*>(lds)[at];
 #pragma unroll
         for (int e = 0; e < S::N; ++e)
-            if (non_finite((float)x[e])) x[e] = (T)0.f;
-        *p = x;
+            if (non_finite((float)x[e])) {
+                any = true;
+                x[e] = (T)0.f;
+            }
+        if (CLEAR && any) reinterpret_cast<V*>(lds)[at] = x;
     }
+    if (!CLEAR && any) *bad = tag;
 }
 
 // bit i of `seen`: the column sees row r0 + row_of(i, half)
@@ -263,45 +281,84 @@ __device__ __forceinline__ void add_non_finite(f32x16* acc, f32x16 w, unsigned s
     }
 }
 
-// Row tiles: memory -> registers -> LDS, so that the next tile's loads are in flight
-// while the present one is worked on.
-template <typename T, int DP, int NW, int BN>
-struct Stage {
-    typedef Shape<T, DP> S;
-    typedef typename Vec16<T>::type V;
-    static constexpr int NT = NW * kWave;
-    static constexpr int CNT = (BN * S::CPR + NT - 1) / NT;
-    V v[CNT];
+// Row tiles go from memory straight into LDS (buffer loads with the lds bit: 64 lanes leave
+// 64 consecutive vectors), two tiles deep: a tile is loaded while the one before it is
+// worked on, without a register in between.  The buffer's size ends with the last row, so
+// rows behind it and dimensions behind `dim` arrive as zeros.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-    // rows [r0, end) of the sequence; `addr(row)` gives a row's address
-    template <typename F>
-    __device__ __forceinline__ void load(int r0, int end, int dim, F addr) {
+__device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned offset, unsigned lds) {
+    // m0 holds the LDS address; the nops cover scalar operands that a vector instruction wrote
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset),
+        "s"(buffer)
+        : "memory");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+__device__ __forceinline__ i32x4 make_buffer(const void* p, unsigned bytes) {
+    const unsigned long long a = reinterpret_cast<unsigned long long>(p);
+    i32x4 b;
+    b[0] = uniform((int)(unsigned)a);
+    b[1] = uniform((int)(unsigned)(a >> 32) & 0xFFFF);
+    b[2] = uniform((int)bytes);
+    b[3] = 0x00020000;
+    return b;
+}
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)(unsigned long long)(__attribute__((address_space(3))) const void*)p;
+}
+
+template <typename T, int DP, int NW, int BN>
+struct Loader {
+    typedef Shape<T, DP> S;
+    static constexpr int LOADS = (BN * S::CPR + kWave - 1) / kWave;  // of a wave each
+    static constexpr int CNT = (LOADS + NW - 1) / NW;
+    unsigned offset[CNT];  // of this lane's vectors within a tile
+
+    __device__ __forceinline__ void init(long long row_elements, int dim) {
 #pragma unroll
         for (int j = 0; j < CNT; ++j) {
-            const int at = j * NT + threadIdx.x;
-            const int r = at / S::CPR, d = at % S::CPR * S::N;
-            V x = {};
-            if (at < BN * S::CPR && r0 + r < end && d < dim)
-                x = *reinterpret_cast<const V*>(addr(r0 + r) + d);
-            v[j] = x;
+            const int at = (threadIdx.x / kWave + NW * j) * kWave + threadIdx.x % kWave;
+            const int r = at / S::CPR, c = at % S::CPR ^ S::turn(r);
+            offset[j] = c * S::N < dim ? (unsigned)(r * (int)row_elements + c * S::N) * (unsigned)sizeof(T)
+                                       : 0x80000000u;
         }
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    // rows [0, rows) from `base` on, into `lds`
+    __device__ __forceinline__ void load(const T* base, long long row_elements, int rows, int dim,
+                                         T* lds) const {
+        const int n = rows < BN ? rows : BN;
+        const i32x4 b =
+            make_buffer(base, (unsigned)((n - 1) * (int)row_elements + dim) * (unsigned)sizeof(T));
+        const unsigned to = lds_address(lds);
 #pragma unroll
         for (int j = 0; j < CNT; ++j) {
-            const int at = j * NT + threadIdx.x;
-            const int r = at / S::CPR, d = at % S::CPR * S::N;
-            if (at < BN * S::CPR) *reinterpret_cast<V*>(lds + r * S::LD + d) = v[j];
+            const int k = uniform(threadIdx.x / kWave) + NW * j;
+            if (LOADS % NW != 0 && k >= LOADS) break;
+            load_to_lds(b, offset[j], uniform((int)(to + k * kWave * 16)));
         }
     }
-    // *bad = tag if a value is infinite or NaN
-    __device__ __forceinline__ void look_over(int* bad, int tag) const {
-        bool any = false;
+    // The same for rows of the packed (query, head of the group) axis: rows [r0, end), row r
+    // being head r % group of query r / group.
+    __device__ __forceinline__ void load_packed(const AttnArgs& a, const T* base, const Rows& x, int r0,
+                                                int end, T* lds) const {
+        const int i0 = uniform(div_group(a, r0));
+        const i32x4 b = make_buffer(base + (long long)i0 * x.row, 0x7FFFFFFFu);
+        const unsigned to = lds_address(lds);
 #pragma unroll
-        for (int j = 0; j < CNT; ++j)
-#pragma unroll
-            for (int e = 0; e < S::N; ++e) any = any || non_finite((float)v[j][e]);
-        if (any) *bad = tag;
+        for (int j = 0; j < CNT; ++j) {
+            const int k = uniform(threadIdx.x / kWave) + NW * j;
+            if (LOADS % NW != 0 && k >= LOADS) break;
+            const int at = k * kWave + threadIdx.x % kWave;
+            const int r = r0 + at / S::CPR, i = div_group(a, r);
+            const unsigned o = (unsigned)((i - i0) * (int)x.row + (r - i * a.group) * (int)x.head) *
+                                   (unsigned)sizeof(T) + offset[j];
+            load_to_lds(b, r < end ? o : 0x80000000u, uniform((int)(to + k * kWave * 16)));
+        }
     }
 };
 
@@ -333,20 +390,21 @@ constexpr float kRescale = 8.f;  // log2 of how far p may pass 1 before the sums
 // product, the sum l uses the unrounded p.
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int NW, int R>
-__global__ __launch_bounds__(NW * kWave) void k_attn_fwd(AttnArgs a) {
+__global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
     typedef Shape<T, DP> S;
     typedef typename Vec16<T>::type V;
-    constexpr int BM = 32 * NW, BN = 32 * R;
-    __shared__ __align__(16) T lk[S::slab(BN)], lv[S::slab(BN)];
+    constexpr int BM = 32 * NW, BN = 32 * R, SLAB = S::slab(BN);
+    __shared__ __align__(16) T lds[4 * SLAB + S::kSlack];  // keys and values, two tiles of each
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
-    const Tile t = tile_of(a.ptr, a.ptr64, a.count, a.nq, a.group, BM, blockIdx.x);
+    // later tiles of a causal sequence take longer: they go first
+    const Tile t = tile_of(a.ptr, a.ptr64, a.count, a.nq, a.group, BM, gridDim.x - 1 - blockIdx.x);
     const int rows = t.len * a.group;
     if (t.index < 0 || (long long)t.index * BM >= rows) return;
     const int kh = blockIdx.y;
     const int k0 = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 1);
     int nk = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 2) - k0;
-    if (nk < 0) nk = 0;
+    nk = uniform(nk < 0 ? 0 : nk);
     const int lane = threadIdx.x % kWave, half = lane / 32;
     const int r0 = t.index * BM + threadIdx.x / kWave * 32;
     const int r = r0 + lane % 32;
@@ -361,11 +419,11 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_fwd(AttnArgs a) {
     const int qi = div_group(a, rc), gi = rc - qi * a.group;
     const int head = kh * a.group + gi;
     const int lim = limit(rc);
-    const int lim_first = limit(r0 < rows ? r0 : rows - 1);  // the wave's smallest
-    const int lim_last = r0 < rows ? limit(r0 + 31 < rows ? r0 + 31 : rows - 1) : 0;
+    const int lim_first = uniform(limit(r0 < rows ? r0 : rows - 1));  // the wave's smallest
+    const int lim_last = uniform(r0 < rows ? limit(r0 + 31 < rows ? r0 + 31 : rows - 1) : 0);
     const int last = t.index * BM + BM - 1;
-    const int lim_block = limit(last < rows ? last : rows - 1);
-    const int lim_whole = a.causal ? limit(t.index * BM) : INT_MAX;  // keys that all rows see
+    const int lim_block = uniform(limit(last < rows ? last : rows - 1));
+    const int lim_whole = uniform(a.causal ? limit(t.index * BM) : INT_MAX);  // keys that all rows see
     int from = 0, to = lim_block;
     if (a.splits > 1) {
         const int per = ((nk + a.splits - 1) / a.splits + BN - 1) / BN * BN;
@@ -380,35 +438,37 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_fwd(AttnArgs a) {
                         a.dim, mine && a.scale != 0.f, a.scale < 0.f);
     const T* kb = static_cast<const T*>(a.k.p) + (long long)k0 * a.k.row + (long long)kh * a.k.head;
     const T* vb = static_cast<const T*>(a.v.p) + (long long)k0 * a.v.row + (long long)kh * a.v.head;
-    auto k_at = [&](int row) { return kb + (long long)row * a.k.row; };
     auto v_at = [&](int row) { return vb + (long long)row * a.v.row; };
     const float c = score_scale(a.scale) * kLog2e;
 
     f32x16 acc[S::DT] = {};
     float m = -INFINITY, l = 0.f;
-    Stage<T, DP, NW, BN> sk, sv;
-    if (from < to) {
-        sk.load(from, nk, a.dim, k_at);
-        sv.load(from, nk, a.dim, v_at);
-    }
-    for (int n0 = from; n0 < to; n0 += BN) {
+    Loader<T, DP, NW, BN> kl, vl;
+    kl.init(a.k.row, a.dim);
+    vl.init(a.v.row, a.dim);
+    auto load_tile = [&](int n0, T* to_lds) {
+        kl.load(kb + (long long)n0 * a.k.row, a.k.row, nk - n0, a.dim, to_lds);
+        vl.load(vb + (long long)n0 * a.v.row, a.v.row, nk - n0, a.dim, to_lds + SLAB);
+    };
+    if (from < to) load_tile(from, lds);
+    for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
+        T* lk = lds + 2 * SLAB * turn;
+        T* lv = lk + SLAB;
+        wait_loads();
         __syncthreads();
-        sk.store(lk);
-        sv.store(lv);
-        const bool edge = n0 + BN > lim_whole;
-        if (edge) sv.look_over(&bad, n0 + 1);
-        __syncthreads();
-        if (n0 + BN < to) {
-            sk.load(n0 + BN, nk, a.dim, k_at);
-            sv.load(n0 + BN, nk, a.dim, v_at);
+        if (n0 + BN < to) load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
+        bool mend = false;
+        if (n0 + BN > lim_whole) {
+            look_over<T, DP, NW, BN, false>(lv, &bad, n0 + 1);
+            __syncthreads();
+            mend = bad == n0 + 1;
         }
-        const bool mend = edge && bad == n0 + 1;
         if (n0 >= lim_last && !mend) continue;
         f32x16 s[R];
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            s[j] = scores<T, DP>(lk + 32 * j * S::LD, qc);
+            s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
             if (n0 + 32 * j + 32 > lim_first) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -428,7 +488,7 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_fwd(AttnArgs a) {
         }
         const float mc = m == -INFINITY ? 0.f : m * c;
         if (mend) {
-            clear_non_finite<T, DP, NW, BN>(lv);
+            look_over<T, DP, NW, BN, true>(lv, nullptr, 0);
             __syncthreads();
         }
 #pragma unroll
@@ -438,7 +498,7 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_fwd(AttnArgs a) {
                 s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -mc));
                 l += s[j][i];
             }
-            add_products<DP>(acc, lv + 32 * j * S::LD, s[j]);
+            add_products<DP>(acc, lv + S::slab(32 * j), s[j]);
             if (mend) {
                 unsigned seen = 0;
 #pragma unroll
@@ -523,20 +583,22 @@ template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * kWave) void k_attn_dq(AttnArgs a) {
     typedef Shape<T, DP> S;
     typedef typename Vec16<T>::type V;
-    constexpr int BM = 32 * NW, BN = 32;
-    __shared__ __align__(16) T lk[S::slab(BN)], lv[S::slab(BN)];
+    constexpr int BM = 32 * NW, BN = 32, SLAB = S::slab(BN);
+    __shared__ __align__(16) T lds[4 * SLAB + S::kSlack];
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
-    const Tile t = tile_of(a.ptr, a.ptr64, a.count, a.nq, a.group, BM, blockIdx.x);
+    // later tiles of a causal sequence take longer: they go first
+    const Tile t = tile_of(a.ptr, a.ptr64, a.count, a.nq, a.group, BM, gridDim.x - 1 - blockIdx.x);
     const int rows = t.len * a.group;
     if (t.index < 0 || (long long)t.index * BM >= rows) return;
     const int kh = blockIdx.y;
     const int k0 = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 1);
     int nk = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 2) - k0;
-    if (nk < 0) nk = 0;
+    nk = uniform(nk < 0 ? 0 : nk);
     const int lane = threadIdx.x % kWave, half = lane / 32;
     const int r0 = t.index * BM + threadIdx.x / kWave * 32;
     const int r = r0 + lane % 32;
+    // the keys that a row sees: [0, limit)
     auto limit = [&](int row) {
         if (!a.causal) return nk;
         const int l = div_group(a, row) + nk - t.len + 1;
@@ -547,11 +609,11 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dq(AttnArgs a) {
     const int qi = div_group(a, rc), gi = rc - qi * a.group;
     const int head = kh * a.group + gi;
     const int lim = limit(rc);
-    const int lim_first = limit(r0 < rows ? r0 : rows - 1);
-    const int lim_last = r0 < rows ? limit(r0 + 31 < rows ? r0 + 31 : rows - 1) : 0;
+    const int lim_first = uniform(limit(r0 < rows ? r0 : rows - 1));  // the wave's smallest
+    const int lim_last = uniform(r0 < rows ? limit(r0 + 31 < rows ? r0 + 31 : rows - 1) : 0);
     const int last = t.index * BM + BM - 1;
-    const int lim_block = limit(last < rows ? last : rows - 1);
-    const int lim_whole = a.causal ? limit(t.index * BM) : INT_MAX;  // keys that all rows see
+    const int lim_block = uniform(limit(last < rows ? last : rows - 1));
+    const int lim_whole = uniform(a.causal ? limit(t.index * BM) : INT_MAX);  // keys that all rows see
     int from = 0, to = lim_block;
     if (a.splits > 1) {
         const int per = ((nk + a.splits - 1) / a.splits + BN - 1) / BN * BN;
@@ -582,27 +644,29 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dq(AttnArgs a) {
     const T* kb = static_cast<const T*>(a.k.p) + (long long)k0 * a.k.row + (long long)kh * a.k.head;
     const T* vb = static_cast<const T*>(a.v.p) + (long long)k0 * a.v.row + (long long)kh * a.v.head;
     auto k_at = [&](int row) { return kb + (long long)row * a.k.row; };
-    auto v_at = [&](int row) { return vb + (long long)row * a.v.row; };
     const float c = score_scale(a.scale) * kLog2e;
 
     f32x16 acc[S::DT] = {};
-    Stage<T, DP, NW, BN> sk, sv;
-    if (from < to) {
-        sk.load(from, nk, a.dim, k_at);
-        sv.load(from, nk, a.dim, v_at);
-    }
-    for (int n0 = from; n0 < to; n0 += BN) {
+    Loader<T, DP, NW, BN> kl, vl;
+    kl.init(a.k.row, a.dim);
+    vl.init(a.v.row, a.dim);
+    auto load_tile = [&](int n0, T* to_lds) {
+        kl.load(kb + (long long)n0 * a.k.row, a.k.row, nk - n0, a.dim, to_lds);
+        vl.load(vb + (long long)n0 * a.v.row, a.v.row, nk - n0, a.dim, to_lds + SLAB);
+    };
+    if (from < to) load_tile(from, lds);
+    for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
+        T* lk = lds + 2 * SLAB * turn;
+        T* lv = lk + SLAB;
+        wait_loads();
         __syncthreads();
-        sk.store(lk);
-        sv.store(lv);
-        const bool edge = n0 + BN > lim_whole;
-        if (edge) sk.look_over(&bad, n0 + 1);
-        __syncthreads();
-        if (n0 + BN < to) {
-            sk.load(n0 + BN, nk, a.dim, k_at);
-            sv.load(n0 + BN, nk, a.dim, v_at);
+        if (n0 + BN < to) load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
+        bool mend = false;
+        if (n0 + BN > lim_whole) {
+            look_over<T, DP, NW, BN, false>(lk, &bad, n0 + 1);
+            __syncthreads();
+            mend = bad == n0 + 1;
         }
-        const bool mend = edge && bad == n0 + 1;
         if (n0 >= lim_last && !mend) continue;
         f32x16 s = scores<T, DP>(lk, qc);
         const f32x16 dp = scores<T, DP>(lv, gc);
@@ -618,7 +682,7 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dq(AttnArgs a) {
         }
         if (mend) {
             __syncthreads();
-            clear_non_finite<T, DP, NW, BN>(lk);
+            look_over<T, DP, NW, BN, true>(lk, nullptr, 0);
             __syncthreads();
         }
         add_products<DP>(acc, lk, s);
@@ -647,9 +711,9 @@ template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
     typedef Shape<T, DP> S;
     typedef typename Vec16<T>::type V;
-    constexpr int BM = 32 * NW, BN = 32, NT = NW * kWave;
-    __shared__ __align__(16) T lq[S::slab(BN)], lg[S::slab(BN)];
-    __shared__ __align__(16) float ll[BN], ld[BN];
+    constexpr int BM = 32 * NW, BN = 32, SLAB = S::slab(BN);
+    __shared__ __align__(16) T lds[4 * SLAB + S::kSlack];  // q and g, two tiles of each
+    __shared__ __align__(16) float sums[2][2][BN];          // lse and delta of their rows
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
     const Tile t = tile_of(a.kv_ptr, a.ptr64, a.count, a.nk, 1, BM, blockIdx.x);
@@ -658,7 +722,7 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
     const int q0 = t.seq < 0 ? 0 : bound_at(a.ptr, a.ptr64, a.count, a.nq, t.seq + 1);
     int nq = t.seq < 0 ? 0 : bound_at(a.ptr, a.ptr64, a.count, a.nq, t.seq + 2) - q0;
     if (nq < 0) nq = 0;
-    const int rows = nq * a.group;
+    const int rows = uniform(nq * a.group);
     const int lane = threadIdx.x % kWave, half = lane / 32;
     const int c0 = t.index * BM + threadIdx.x / kWave * 32;
     const int key = c0 + lane % 32;
@@ -671,8 +735,8 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
         return i < 0 ? 0 : i >= nq ? rows : i * a.group;
     };
     const int beg = start(kc);
-    const int beg_first = c0 < t.len ? start(c0) : rows;  // the wave's smallest
-    const int beg_last = start(c0 + 31 < t.len ? c0 + 31 : t.len - 1);
+    const int beg_first = uniform(c0 < t.len ? start(c0) : rows);  // the wave's smallest
+    const int beg_last = uniform(start(c0 + 31 < t.len ? c0 + 31 : t.len - 1));
     // the first row from which on all of the workgroup's keys are seen
     const int beg_whole = start(t.index * BM + BM - 1 < t.len ? t.index * BM + BM - 1 : t.len - 1);
     int from = start(t.index * BM) / BN * BN, to = rows;
@@ -701,60 +765,60 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
         const int i = div_group(a, row);
         return gb + (long long)i * a.g.row + (long long)(row - i * a.group) * a.g.head;
     };
-    // lse (in log2) and delta of a row tile: one row a thread, two where a wave is alone
-    constexpr int PER = BN > NT ? BN / NT : 1;
-    float rl[PER], rd[PER];
+    // lse (in log2) and delta of a row tile, by the first wave's lower half
+    float rl = 0.f, rd = 0.f;
     auto load_sums = [&](int n0) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int at = j * NT + threadIdx.x, row = n0 + at;
-            const bool in = at < BN && row < rows;
+        const int row = n0 + threadIdx.x;
+        const bool in = threadIdx.x < BN && row < rows;
+        if (threadIdx.x < BN) {
             const int i = in ? div_group(a, row) : 0;
             const long long qh = ((long long)(q0 + i) * a.kv_heads + kh) * a.group + (row - i * a.group);
-            rl[j] = in ? a.lse[qh] * kLog2e : INFINITY;  // exp(s - inf) = 0 behind the last row
-            rd[j] = in ? a.delta[qh] : 0.f;
+            rl = in ? a.lse[qh] * kLog2e : INFINITY;  // exp(s - inf) = 0 behind the last row
+            rd = in ? a.delta[qh] : 0.f;
         }
     };
     const float c = score_scale(a.scale) * kLog2e;
 
     f32x16 dk[S::DT] = {}, dv[S::DT] = {};
-    Stage<T, DP, NW, BN> sq, sg;
+    Loader<T, DP, NW, BN> ld;
+    ld.init(0, a.dim);
+    auto load_tile = [&](int n0, T* to_lds) {
+        ld.load_packed(a, qb, a.q, n0, rows, to_lds);
+        ld.load_packed(a, gb, a.g, n0, rows, to_lds + SLAB);
+    };
     if (from < to) {
-        sq.load(from, rows, a.dim, q_at);
-        sg.load(from, rows, a.dim, g_at);
         load_sums(from);
+        load_tile(from, lds);
     }
-    for (int n0 = from; n0 < to; n0 += BN) {
-        __syncthreads();
-        sq.store(lq);
-        sg.store(lg);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int at = j * NT + threadIdx.x;
-            if (at < BN) {
-                ll[at] = rl[j];
-                ld[at] = rd[j];
-            }
+    for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
+        T* lq = lds + 2 * SLAB * turn;
+        T* lg = lq + SLAB;
+        const float* ll = sums[turn][0];
+        const float* ldl = sums[turn][1];
+        if (threadIdx.x < BN) {
+            sums[turn][0][threadIdx.x] = rl;
+            sums[turn][1][threadIdx.x] = rd;
         }
-        const bool edge = n0 < beg_whole;
-        if (edge) {
-            sq.look_over(&bad, n0 + 1);
-            sg.look_over(&bad, n0 + 1);
-        }
+        wait_loads();
         __syncthreads();
         if (n0 + BN < to) {
-            sq.load(n0 + BN, rows, a.dim, q_at);
-            sg.load(n0 + BN, rows, a.dim, g_at);
             load_sums(n0 + BN);
+            load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
         }
-        const bool mend = edge && bad == n0 + 1;
+        bool mend = false;
+        if (n0 < beg_whole) {
+            look_over<T, DP, NW, BN, false>(lq, &bad, n0 + 1);
+            look_over<T, DP, NW, BN, false>(lg, &bad, n0 + 1);
+            __syncthreads();
+            mend = bad == n0 + 1;
+        }
         if (n0 + BN <= beg_first && !mend) continue;
         f32x16 p = scores<T, DP>(lq, kcol);
         f32x16 ds = scores<T, DP>(lg, vcol);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const f32x4 l4 = *reinterpret_cast<const f32x4*>(ll + 8 * b + 4 * half);
-            const f32x4 d4 = *reinterpret_cast<const f32x4*>(ld + 8 * b + 4 * half);
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(ldl + 8 * b + 4 * half);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * b + e;
@@ -769,8 +833,8 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
         }
         if (mend) {
             __syncthreads();
-            clear_non_finite<T, DP, NW, BN>(lq);
-            clear_non_finite<T, DP, NW, BN>(lg);
+            look_over<T, DP, NW, BN, true>(lq, nullptr, 0);
+            look_over<T, DP, NW, BN, true>(lg, nullptr, 0);
             __syncthreads();
         }
         add_products<DP>(dv, lg, p);
@@ -852,10 +916,11 @@ inline int attn_check(int nq, int nk, int count, int heads, int kv_heads, int di
     return GAT_OK;
 }
 
-inline bool vec_rows(const Rows& r, int dtype) {
+inline bool vec_rows(const Rows& r, int dim, int group, int dtype) {
     const int n = 16 / (int)dtype_size(dtype);
     return (reinterpret_cast<uintptr_t>(r.p) & 15) == 0 && r.row % n == 0 && r.head % n == 0 &&
-           r.row >= 0 && r.head >= 0;
+           r.row >= dim && r.row <= (1 << 22) && r.head >= 0 &&
+           r.head * group <= (1 << 28);  // offsets within a tile fit 31 bits of bytes
 }
 
 inline void set_group(AttnArgs& a, int group) {
@@ -875,7 +940,7 @@ int attn_launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
     const dim3 grid((unsigned)slots, a.kv_heads, p.splits);
     [[maybe_unused]] constexpr int R = sizeof(T) == 2 ? 2 : 1;  // 32-row tiles a step of the forward
     if (p.waves == 1) {
-        if constexpr (PASS == kFwd) k_attn_fwd<T, DP, 1, R><<<grid, 64, 0, s>>>(a);
+        if constexpr (PASS == kFwd) k_attn_fwd<T, DP, 1, 1><<<grid, 64, 0, s>>>(a);
         if constexpr (PASS == kDq) k_attn_dq<T, DP, 1><<<grid, 64, 0, s>>>(a);
         if constexpr (PASS == kDkv) k_attn_dkv<T, DP, 1><<<grid, 64, 0, s>>>(a);
     } else {
@@ -943,8 +1008,8 @@ int gat_packed_attention(const void* q, long long q_row, long long q_head, const
     if (q == nullptr || out == nullptr || ptr == nullptr || kv_ptr == nullptr ||
         (nk > 0 && (k == nullptr || v == nullptr)))
         return GAT_EINVAL;
-    if (!vec_rows(a.q, dtype) || !vec_rows(a.o, dtype) || !vec_rows(a.k, dtype) || !vec_rows(a.v, dtype))
-        return GAT_EUNSUPPORTED;
+    for (const Rows* r : {&a.q, &a.k, &a.v, &a.o})
+        if (!vec_rows(*r, dim, heads / kv_heads, dtype)) return GAT_EUNSUPPORTED;
     const AttnSizes sz = attn_sizes(nq, nk, count, heads, kv_heads, dim);
     if (sz.fwd_bytes > 0 && (workspace == nullptr || workspace_bytes < sz.fwd_bytes))
         return GAT_EWORKSPACE;
@@ -1008,7 +1073,7 @@ int gat_packed_attention_backward(const void* g, long long g_row, long long g_he
         (nk > 0 && (k == nullptr || v == nullptr || dk == nullptr || dv == nullptr)))
         return GAT_EINVAL;
     for (const Rows* r : {&a.g, &a.q, &a.k, &a.v, &a.o, &a.dq, &a.dk, &a.dv})
-        if (!vec_rows(*r, dtype)) return GAT_EUNSUPPORTED;
+        if (!vec_rows(*r, dim, heads / kv_heads, dtype)) return GAT_EUNSUPPORTED;
     const AttnSizes sz = attn_sizes(nq, nk, count, heads, kv_heads, dim);
     if (workspace_bytes < sz.delta_bytes + std::max(sz.dq_bytes, sz.dkv_bytes) ||
         (workspace == nullptr && workspace_bytes > 0))

@@ -33,10 +33,13 @@ __device__ __forceinline__ typename Vec16<T>::type load_vec(const T* row, int co
     if (whole && col0 >= 0 && col0 + N <= cols) {
         v = *reinterpret_cast<const typename Vec16<T>::type*>(row + col0);
     } else {
+        v = typename Vec16<T>::type{};
+        if (col0 < cols && col0 + N > 0) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const int c = col0 + e;
-            v[e] = c >= 0 && c < cols ? row[c] : (T)0.f;
+            for (int e = 0; e < N; ++e) {
+                const int c = col0 + e;
+                if (c >= 0 && c < cols) v[e] = row[c];
+            }
         }
     }
     return v;
@@ -48,13 +51,29 @@ __device__ __forceinline__ void store_vec(T* row, int col0, int cols, bool whole
     constexpr int N = Vec16<T>::N;
     if (whole && col0 >= 0 && col0 + N <= cols) {
         *reinterpret_cast<typename Vec16<T>::type*>(row + col0) = v;
-    } else {
+    } else if (col0 < cols && col0 + N > 0) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             const int c = col0 + e;
             if (c >= 0 && c < cols) row[c] = v[e];
         }
     }
+}
+
+// Sum over the aligned group of W lanes that this one is in, given to all of them: no LDS
+// round trip (DPP within 16 lanes, then the lane-half swaps).
+template <int W>
+__device__ __forceinline__ float lanes_sum(float v) {
+    v = group_sum16(v, W);
+    if constexpr (W >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (W >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
 }
 
 // elements from the 16-byte boundary at or before p to p

@@ -32,7 +32,7 @@ _NULL = contextlib.nullcontext()
 
 def _on(device: torch.device):
     """Launches go to the device the tensors are on, whichever is current."""
-    return _NULL if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _NULL if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _stream(device: torch.device) -> int:
@@ -60,6 +60,8 @@ def _need_like(what: str, name: str, t, like: torch.Tensor, dtype=True) -> None:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., C] as [rows, C] with adjacent columns; a copy only where no view does it."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
@@ -93,7 +95,7 @@ class _LayerNorm(torch.autograd.Function):
         stats = torch.empty(x2.shape[0], 2, dtype=torch.float32, device=x.device)
         y = _norm_forward(x2, w, b, eps, stats)
         ctx.save_for_backward(x2, w, stats)
-        return y.view(x.shape)
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -103,9 +105,9 @@ class _LayerNorm(torch.autograd.Function):
         shape, g = g.shape, _rows(g)
         need = ctx.needs_input_grad
         dt = _DTYPES[x2.dtype]
-        dx = torch.empty(n, c, dtype=x2.dtype, device=x2.device) if need[0] else None
-        dw, db = (torch.empty(c, dtype=x2.dtype, device=x2.device) if k else None
-                  for k in need[1:3])
+        dx = x2.new_empty(n, c) if need[0] else None
+        dw = x2.new_empty(c) if need[1] else None
+        db = x2.new_empty(c) if need[2] else None
         size = _lib.layer_norm_workspace_size(n, c, dt) if need[1] or need[2] else 0
         ws = torch.empty(size, dtype=torch.uint8, device=x2.device)
         with _on(x2.device):
@@ -115,7 +117,7 @@ class _LayerNorm(torch.autograd.Function):
                 _stream(x2.device))
         if rc:
             _lib.check(rc, "gat_layer_norm_backward")
-        return None if dx is None else dx.view(shape), dw, db, None
+        return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, db, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -267,12 +269,14 @@ class Embedding(torch.nn.Module):
 # ---------------------------------------------------------------------------
 def _vectors(t: torch.Tensor) -> torch.Tensor:
     """[tokens, heads, dim] as the kernels read it: adjacent dimensions, rows of whole
-    16-byte vectors on 16-byte boundaries.  ``t`` itself where it is that already (a view
-    of a fused projection's output, say), else a copy padded with zeros."""
+    16-byte vectors on 16-byte boundaries, no two tokens in one place and strides that 31-bit offsets
+    reach.  ``t`` itself where it is that already (a view of a fused projection's output,
+    say), else a copy padded with zeros."""
     n = 16 // t.element_size()
     d = t.shape[2]
-    if d % n == 0 and t.stride(2) == 1 and t.stride(0) % n == 0 and t.stride(1) % n == 0 \
-            and t.data_ptr() % 16 == 0:
+    row, head, one = t.stride()
+    if d % n == 0 and one == 1 and row % n == 0 and head % n == 0 and t.data_ptr() % 16 == 0 \
+            and d <= row <= 1 << 22 and head * t.shape[1] <= 1 << 28:
         return t
     if d % n == 0:
         return t.clone(memory_format=torch.contiguous_format)
@@ -308,12 +312,15 @@ class _PackedAttention(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, out, lse, ptr, kv_ptr)
         ctx.causal, ctx.scale, ctx.dim = causal, scale, d
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)  # no zeros for lse
         return (out if out.shape[2] == d else out[..., :d].contiguous()), lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
         q, k, v, out, lse, ptr, kv_ptr = ctx.saved_tensors
+        if g is None:
+            return (None,) * 7
         g = _vectors(g)
         nq, h, d = q.shape
         nk, hk = k.shape[:2]
