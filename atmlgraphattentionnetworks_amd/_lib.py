@@ -133,10 +133,10 @@ SIGNATURES = {
                                     _c_ll, _c_vp, _c_ll, _c_vp, ctypes.c_size_t, _c_int, _c_vp]),
     "gat_packed_attention_workspace_size": (_c_int, [_c_int] * 7 + [_c_size_p]),
     "gat_packed_attention": (_c_int, [_c_vp, _c_ll, _c_ll] * 3 + [_c_vp, _c_vp] + [_c_int] * 7 +
-                             [_c_float, _c_int, _c_vp, _c_vp, _c_vp, ctypes.c_size_t, _c_int,
-                              _c_vp]),
+                             [_c_float, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, ctypes.c_size_t,
+                              _c_int, _c_vp]),
     "gat_packed_attention_backward_workspace_size": (_c_int, [_c_int] * 7 + [_c_size_p]),
-    "gat_packed_attention_backward": (_c_int, [_c_vp, _c_ll, _c_ll] * 4 + [_c_vp] * 4 +
+    "gat_packed_attention_backward": (_c_int, [_c_vp, _c_ll, _c_ll] * 4 + [_c_vp] * 5 +
                                       [_c_int] * 7 + [_c_float, _c_int] + [_c_vp] * 4 +
                                       [ctypes.c_size_t, _c_int, _c_vp]),
 }

@@ -9,9 +9,9 @@
 // Gradient: the tokens are sorted by id (stable, so each id's tokens stay in order) and
 // each table row is then one sum over its tokens' rows of g, written once, zeros
 // included: no atomics and no separate clearing pass, and the result does not depend on
-// timing.  An id with more than kPiece tokens would keep one row's lanes busy long after
-// the rest: the sorted order is cut into pieces of kPiece tokens, the pieces of such an
-// id are summed by workgroups of their own, and the partial sums are joined in order.
+// timing.  An id with many tokens would keep one row's lanes busy long after the rest: the
+// sorted order is cut into pieces, the pieces of an id with more tokens than a piece are
+// summed by workgroups of their own, and the partial sums are joined in order.
 // Sums are float32 and rounded once, after the scale.
 //
 // Sort: least significant digit first, 8 bits a pass, over (id, token) pairs; an id that
@@ -28,7 +28,7 @@ constexpr int kSortBlock = 1024;
 constexpr int kSortWaves = kSortBlock / kWave;
 constexpr int kSortMinItems = 1024;
 constexpr int kSortMaxBlocks = 256;
-constexpr int kPiece = 32;
+constexpr int kMinPiece = 16, kMaxPieces = 4096;
 constexpr long long kMaxTokens = 1ll << 30;
 constexpr int kEmbedBlock = 256;
 
@@ -236,19 +236,19 @@ __device__ __forceinline__ void join_groups(float (&acc)[N], float* lds) {
 }
 
 // Piece j's partial sums, part[2 j + slot]: slot 0 the id that the piece begins with,
-// slot 1 the one that it ends with, where that id has more than kPiece tokens.
+// slot 1 the one that it ends with, where that id has more tokens than a piece.
 template <typename T, int LPR>
 __global__ __launch_bounds__(kEmbedBlock) void k_embed_pieces(
-    const unsigned* keys, const unsigned* toks, const int* first, int n, int vocab, const T* g,
-    long long ld_g, int cols, int whole, float* part) {
+    const unsigned* keys, const unsigned* toks, const int* first, int n, int vocab, int piece,
+    const T* g, long long ld_g, int cols, int whole, float* part) {
     constexpr int N = Vec16<T>::N;
     __shared__ float lds[kEmbedBlock * N];
     const int j = blockIdx.x >> 1, slot = blockIdx.x & 1;
-    const int a = j * kPiece, e = a + kPiece < n ? a + kPiece : n;
+    const int a = j * piece, e = a + piece < n ? a + piece : n;
     const unsigned head = keys[a], id = slot == 0 ? head : keys[e - 1];
     if (id >= (unsigned)vocab || (slot == 1 && id == head)) return;
     const int f = first[id], l = first[id + 1];
-    if (l - f <= kPiece) return;
+    if (l - f <= piece) return;
     const int from = f > a ? f : a, to = l < e ? l : e;
     const int lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
     const int c = (blockIdx.y * LPR + lane) * N;
@@ -264,24 +264,24 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_pieces(
     }
 }
 
-// Table rows of ids with more than kPiece tokens: piece j's workgroup takes the one whose
+// Table rows of ids with more tokens than a piece: piece j's workgroup takes the one whose
 // tokens begin in it, if there is one.
 template <typename T, int LPR>
 __global__ __launch_bounds__(kEmbedBlock) void k_embed_join(const unsigned* keys, const int* first,
-                                                            int n, int vocab, int cols,
+                                                            int n, int vocab, int piece, int cols,
                                                             const float* part, float scale, T* dw,
                                                             long long ld_dw, int whole) {
     constexpr int N = Vec16<T>::N;
     __shared__ float lds[kEmbedBlock * N];
     const int j = blockIdx.x;
-    const int a = j * kPiece, e = a + kPiece < n ? a + kPiece : n;
+    const int a = j * piece, e = a + piece < n ? a + piece : n;
     const unsigned id = keys[e - 1];
     if (id >= (unsigned)vocab) return;
     const int f = first[id], l = first[id + 1];
-    if (l - f <= kPiece || f < a) return;
+    if (l - f <= piece || f < a) return;
     const int lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
     const int c = (blockIdx.y * LPR + lane) * N;
-    const int last = (l - 1) / kPiece;
+    const int last = (l - 1) / piece;
     float acc[N] = {};
     if (c < cols) {
 #pragma unroll 8
@@ -300,45 +300,70 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_join(const unsigned* keys
     }
 }
 
-// All other table rows, those of ids without a token too.
-template <typename T, int LPR>
+// All other table rows, those of ids without a token too: R rows a group, whose tokens lie
+// together in the sorted order, so that U rows of g are in flight across the table rows'
+// borders (most ids have few tokens).
+template <typename T, int LPR, int R>
 __global__ __launch_bounds__(kEmbedBlock) void k_embed_rows(const unsigned* toks, const int* first,
-                                                            int vocab, const T* g, long long ld_g,
-                                                            int whole_g, int cols, float scale,
-                                                            T* dw, long long ld_dw, int whole) {
-    // two table rows a group: the loads of both fly together (most have few tokens)
-    constexpr int N = Vec16<T>::N, U = 4;
+                                                            int vocab, int piece, const T* g,
+                                                            long long ld_g, int whole_g, int cols,
+                                                            float scale, T* dw, long long ld_dw,
+                                                            int whole) {
+    constexpr int N = Vec16<T>::N, U = 8;
     typedef typename Vec16<T>::type V;
     const int lane = threadIdx.x % LPR;
-    const int v = (blockIdx.x * (kEmbedBlock / LPR) + threadIdx.x / LPR) * 2;
+    const int v0 = (blockIdx.x * (kEmbedBlock / LPR) + threadIdx.x / LPR) * R;
     const int c = (blockIdx.y * LPR + lane) * N;
-    if (v >= vocab || c >= cols) return;
-    int at[3];
-    at[0] = first[v];
-    at[1] = first[v + 1];
-    at[2] = v + 1 < vocab ? first[v + 2] : at[1];
-    V x[2][U];
+    if (v0 >= vocab || c >= cols) return;
+    const int rows = vocab - v0 < R ? vocab - v0 : R;
+    int at[R + 1];
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int r = 0; r <= R; ++r) at[r] = first[v0 + (r < rows ? r : rows)];
+    for (int r = 0; r < rows;) {
+        // rows r .. e - 1 with at most a piece each; row e has more, or is not ours
+        int e = r, end = at[0], cur_end = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            x[r][u] = V{};
-            if (at[r] + u < at[r + 1] && at[r + 1] - at[r] <= kPiece)
-                x[r][u] = load_vec<T>(g + (long long)toks[at[r] + u] * ld_g, c, cols, whole_g);
+        for (int k = 0; k < R; ++k)
+            if (k == e && k < rows && at[k + 1] - at[k] <= piece) e = k + 1;
+        int p = 0;
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            p = k == r ? at[k] : p;
+            cur_end = k == r ? at[k + 1] : cur_end;
+            end = k + 1 == e ? at[k + 1] : end;
         }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        if (v + r >= vocab || at[r + 1] - at[r] > kPiece) continue;
+        if (e == r) {
+            ++r;
+            continue;
+        }
         float acc[N] = {};
+        auto finish = [&]() {  // row r is whole
+            V y;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+            for (int k = 0; k < N; ++k) {
+                y[k] = (T)(acc[k] * scale);
+                acc[k] = 0.f;
+            }
+            store_vec<T>(dw + (long long)(v0 + r) * ld_dw, c, cols, whole, y);
+            ++r;
 #pragma unroll
-            for (int k = 0; k < N; ++k) acc[k] += (float)x[r][u][k];
-        add_rows<T>(acc, g, ld_g, toks, at[r] + U, at[r + 1], 1, c, cols, whole_g);
-        V y;
+            for (int k = 0; k < R; ++k) cur_end = k == r ? at[k + 1] : cur_end;
+        };
+        for (; p < end; p += U) {
+            V x[U];
 #pragma unroll
-        for (int k = 0; k < N; ++k) y[k] = (T)(acc[k] * scale);
-        store_vec<T>(dw + (long long)(v + r) * ld_dw, c, cols, whole, y);
+            for (int u = 0; u < U; ++u)
+                x[u] = load_vec<T>(g + (long long)toks[p + u < end ? p + u : end - 1] * ld_g, c, cols,
+                                   whole_g);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (p + u >= end) break;
+                while (p + u >= cur_end) finish();
+#pragma unroll
+                for (int k = 0; k < N; ++k) acc[k] += (float)x[u][k];
+            }
+        }
+        while (r < e) finish();
     }
 }
 
@@ -351,6 +376,14 @@ inline int embed_lanes(int cols, int dtype) {
 
 inline bool rows_whole(const void* p, long long ld, int dtype) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((uintptr_t)ld * dtype_size(dtype) & 15) == 0;
+}
+
+// Tokens of a piece: few, so that no group adds up many rows in a line, but at most
+// kMaxPieces pieces in all, whose partial sums an id of all tokens joins in a line.
+inline int piece_of(int n) {
+    int p = kMinPiece;
+    while ((long long)p * kMaxPieces < n) p *= 2;
+    return p;
 }
 
 struct SortPlan {
@@ -386,7 +419,8 @@ inline GradLayout grad_layout(int n, int vocab, int cols) {
     }
     l.counts = take((size_t)kSortMaxBlocks * 256 * 4);
     l.first = take(((size_t)vocab + 1) * 4);
-    l.part = take(((size_t)n + kPiece - 1) / kPiece * 2 * cols * 4);
+    const int piece = piece_of(n);
+    l.part = take(((size_t)n + piece - 1) / piece * 2 * cols * 4);
     l.bytes = at;
     return l;
 }
@@ -398,16 +432,26 @@ int embed_grad_sums(const unsigned* keys, const unsigned* toks, const int* first
     constexpr int N = Vec16<T>::N;
     const int whole_g = rows_whole(g, ld_g, dtype), whole = rows_whole(dw, ld_dw, dtype);
     const int slabs = (cols + LPR * N - 1) / (LPR * N);
-    if (n > kPiece) {
-        const int pieces = (n + kPiece - 1) / kPiece;
+    const int piece = piece_of(n);
+    if (n > piece) {
+        const int pieces = (n + piece - 1) / piece;
         k_embed_pieces<T, LPR><<<dim3(2 * pieces, slabs), kEmbedBlock, 0, s>>>(
-            keys, toks, first, n, vocab, g, ld_g, cols, whole_g, part);
+            keys, toks, first, n, vocab, piece, g, ld_g, cols, whole_g, part);
         k_embed_join<T, LPR><<<dim3(pieces, slabs), kEmbedBlock, 0, s>>>(
-            keys, first, n, vocab, cols, part, scale, dw, ld_dw, whole);
+            keys, first, n, vocab, piece, cols, part, scale, dw, ld_dw, whole);
     }
     constexpr int RPB = kEmbedBlock / LPR;
-    k_embed_rows<T, LPR><<<dim3(((vocab + 1) / 2 + RPB - 1) / RPB, slabs), kEmbedBlock, 0, s>>>(
-        toks, first, vocab, g, ld_g, whole_g, cols, scale, dw, ld_dw, whole);
+    // several table rows a group where there are enough of them for all CUs
+    auto rows = [&](auto r) {
+        constexpr int R = decltype(r)::value;
+        const int groups = (vocab + R - 1) / R;
+        k_embed_rows<T, LPR, R><<<dim3((groups + RPB - 1) / RPB, slabs), kEmbedBlock, 0, s>>>(
+            toks, first, vocab, piece, g, ld_g, whole_g, cols, scale, dw, ld_dw, whole);
+    };
+    if ((long long)vocab * slabs >= 4ll * 256 * 8 * RPB)
+        rows(std::integral_constant<int, 4>());
+    else
+        rows(std::integral_constant<int, 1>());
     return status_of(hipGetLastError());
 }
 

@@ -47,6 +47,7 @@ struct Rows {  // a [tokens, heads, dim] tensor; strides in elements
 
 struct AttnArgs {
     Rows q, k, v, g, o;  // o: the forward's output
+    void* low;           // bf16: what o's rounding left, as o lies; may be null
     Rows dq, dk, dv;
     float* lse;    // [queries, heads]
     float* delta;  // [queries, heads] sum_d g y
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
     const int lim_whole = uniform(a.causal ? limit(t.index * BM) : INT_MAX);  // keys that all rows see
     int from = 0, to = lim_block;
     if (a.splits > 1) {
-        const int per = ((nk + a.splits - 1) / a.splits + BN - 1) / BN * BN;
+        const int per = ((lim_block + a.splits - 1) / a.splits + BN - 1) / BN * BN;
         from = blockIdx.z * per;
         to = from + per < lim_block ? from + per : lim_block;
     }
@@ -529,6 +530,19 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
         l = 1.f;
     }
     store_column<T, DP>(out, acc, 1.f / l, a.dim);
+    if constexpr (sizeof(T) == 2) {
+        if (a.low != nullptr) {
+            const float f = 1.f / l;
+#pragma unroll
+            for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float y = acc[d][i] * f;
+                    acc[d][i] = y - (float)(T)y;
+                }
+            store_column<T, DP>(static_cast<T*>(a.low) + qh * a.dim, acc, 1.f, a.dim);
+        }
+    }
     if (a.lse != nullptr && half == 0)
         a.lse[qh] = lim == 0 ? -INFINITY : m * score_scale(a.scale) + logf(l);
 }
@@ -557,7 +571,11 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     const long long tok = qh / (a.kv_heads * a.group), head = qh % (a.kv_heads * a.group);
     T* out = static_cast<T*>(const_cast<void*>(a.o.p)) + tok * a.o.row + head * a.o.head + d;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = (T)(acc[e] / l);
+    for (int e = 0; e < 4; ++e) {
+        const float y = acc[e] / l;
+        out[e] = (T)y;
+        if (sizeof(T) == 2 && a.low != nullptr) static_cast<T*>(a.low)[qh * a.dim + d + e] = (T)(y - (float)(T)y);
+    }
     if (a.lse != nullptr && d == 0)
         a.lse[qh] = m == -INFINITY ? -INFINITY : m * score_scale(a.scale) + logf(l);
 }
@@ -576,14 +594,14 @@ __global__ __launch_bounds__(256) void k_attn_sum(const float* part, int splits,
 
 // ---------------------------------------------------------------------------
 // dq: columns = queries, rows = keys.  P comes back from the scores and lse; dS is
-// rounded to k's type for the product with k.  sum_d g y is formed here, in float32 from
-// the stored y, and left for the dk/dv kernel.
+// rounded to k's type for the product with k.  sum_d g y is formed here, in float32, and
+// left for the dk/dv kernel.
 // ---------------------------------------------------------------------------
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * kWave) void k_attn_dq(AttnArgs a) {
+template <typename T, int DP, int NW, int R>
+__global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnArgs a) {
     typedef Shape<T, DP> S;
     typedef typename Vec16<T>::type V;
-    constexpr int BM = 32 * NW, BN = 32, SLAB = S::slab(BN);
+    constexpr int BM = 32 * NW, BN = 32 * R, SLAB = S::slab(BN);
     __shared__ __align__(16) T lds[4 * SLAB + S::kSlack];
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
@@ -616,7 +634,7 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dq(AttnArgs a) {
     const int lim_whole = uniform(a.causal ? limit(t.index * BM) : INT_MAX);  // keys that all rows see
     int from = 0, to = lim_block;
     if (a.splits > 1) {
-        const int per = ((nk + a.splits - 1) / a.splits + BN - 1) / BN * BN;
+        const int per = ((lim_block + a.splits - 1) / a.splits + BN - 1) / BN * BN;
         from = blockIdx.z * per;
         to = from + per < lim_block ? from + per : lim_block;
     }
@@ -628,17 +646,21 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dq(AttnArgs a) {
                         a.dim, mine && a.scale != 0.f, a.scale < 0.f);
     load_columns<T, DP>(gc, static_cast<const T*>(a.g.p) + tok * a.g.row + (long long)head * a.g.head,
                         a.dim, mine, false);
+    // From y and, in bf16, what its rounding left: the rounding alone would be the larger part
+    // of dq's error where few keys are seen (measured at 64 to 1000 keys: 3.0e-3 to 2.5e-3 of
+    // dq's norm against 2.3e-3 to 2.45e-3)
     float delta = 0.f;
-    {
+    auto add_delta = [&](const T* from_row) {
         V oc[S::STEPS];
-        load_columns<T, DP>(oc, static_cast<const T*>(a.o.p) + tok * a.o.row +
-                                    (long long)head * a.o.head, a.dim, mine, false);
+        load_columns<T, DP>(oc, from_row, a.dim, mine, false);
 #pragma unroll
         for (int s = 0; s < S::STEPS; ++s)
 #pragma unroll
             for (int e = 0; e < S::N; ++e) delta = fmaf((float)gc[s][e], (float)oc[s][e], delta);
-        delta += __shfl_xor(delta, 32);
-    }
+    };
+    if (sizeof(T) == 2 && a.low != nullptr) add_delta(static_cast<const T*>(a.low) + qh * a.dim);
+    add_delta(static_cast<const T*>(a.o.p) + tok * a.o.row + (long long)head * a.o.head);
+    delta += __shfl_xor(delta, 32);
     if (mine && half == 0 && blockIdx.z == 0) a.delta[qh] = delta;
     const float lse2 = mine ? a.lse[qh] * kLog2e : 0.f;
     const T* kb = static_cast<const T*>(a.k.p) + (long long)k0 * a.k.row + (long long)kh * a.k.head;
@@ -668,29 +690,40 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dq(AttnArgs a) {
             mend = bad == n0 + 1;
         }
         if (n0 >= lim_last && !mend) continue;
-        f32x16 s = scores<T, DP>(lk, qc);
-        const f32x16 dp = scores<T, DP>(lv, gc);
+        f32x16 s[R], dp[R];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lse2));
-            s[i] = p * (dp[i] - delta);
+        for (int j = 0; j < R; ++j) {
+            s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
+            dp[j] = scores<T, DP>(lv + S::slab(32 * j), gc);
         }
-        if (n0 + BN > lim_first) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (n0 + row_of(i, half) >= lim) s[i] = 0.f;
+        for (int j = 0; j < R; ++j) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -lse2));
+                s[j][i] = p * (dp[j][i] - delta);
+            }
+            if (n0 + 32 * j + 32 > lim_first) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = 0.f;
+            }
         }
         if (mend) {
             __syncthreads();
             look_over<T, DP, NW, BN, true>(lk, nullptr, 0);
             __syncthreads();
         }
-        add_products<DP>(acc, lk, s);
-        if (mend) {
-            unsigned seen = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) seen |= (n0 + row_of(i, half) < lim ? 1u : 0u) << i;
-            add_non_finite<T, DP>(acc, s, seen, n0, nk, a.dim, k_at);
+        for (int j = 0; j < R; ++j) {
+            add_products<DP>(acc, lk + S::slab(32 * j), s[j]);
+            if (mend) {
+                unsigned seen = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
+                add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, k_at);
+            }
         }
     }
     if (!mine) return;
@@ -707,11 +740,11 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dq(AttnArgs a) {
 // ---------------------------------------------------------------------------
 // dk, dv: columns = keys, rows = (query, head of the group).
 // ---------------------------------------------------------------------------
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
+template <typename T, int DP, int NW, int R>
+__global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
     typedef Shape<T, DP> S;
     typedef typename Vec16<T>::type V;
-    constexpr int BM = 32 * NW, BN = 32, SLAB = S::slab(BN);
+    constexpr int BM = 32 * NW, BN = 32 * R, SLAB = S::slab(BN);
     __shared__ __align__(16) T lds[4 * SLAB + S::kSlack];  // q and g, two tiles of each
     __shared__ __align__(16) float sums[2][2][BN];          // lse and delta of their rows
     __shared__ int bad;
@@ -741,10 +774,9 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
     const int beg_whole = start(t.index * BM + BM - 1 < t.len ? t.index * BM + BM - 1 : t.len - 1);
     int from = start(t.index * BM) / BN * BN, to = rows;
     if (a.splits > 1) {
-        const int per = ((rows + a.splits - 1) / a.splits + BN - 1) / BN * BN;
-        const int z = blockIdx.z * per;
-        if (from < z) from = z;
-        if (to > z + per) to = z + per;
+        const int per = ((rows - from + a.splits - 1) / a.splits + BN - 1) / BN * BN;
+        from += blockIdx.z * per;
+        to = from + per < rows ? from + per : rows;
     }
 
     V kcol[S::STEPS], vcol[S::STEPS];
@@ -765,7 +797,7 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
         const int i = div_group(a, row);
         return gb + (long long)i * a.g.row + (long long)(row - i * a.group) * a.g.head;
     };
-    // lse (in log2) and delta of a row tile, by the first wave's lower half
+    // lse (in log2) and delta of a row tile, a row each of the first wave's lanes
     float rl = 0.f, rd = 0.f;
     auto load_sums = [&](int n0) {
         const int row = n0 + threadIdx.x;
@@ -813,23 +845,30 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
             mend = bad == n0 + 1;
         }
         if (n0 + BN <= beg_first && !mend) continue;
-        f32x16 p = scores<T, DP>(lq, kcol);
-        f32x16 ds = scores<T, DP>(lg, vcol);
+        f32x16 p[R], ds[R];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const f32x4 l4 = *reinterpret_cast<const f32x4*>(ll + 8 * b + 4 * half);
-            const f32x4 d4 = *reinterpret_cast<const f32x4*>(ldl + 8 * b + 4 * half);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = 4 * b + e;
-                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], c, -l4[e]));
-                ds[i] = p[i] * (ds[i] - d4[e]);
-            }
+        for (int j = 0; j < R; ++j) {
+            p[j] = scores<T, DP>(lq + S::slab(32 * j), kcol);
+            ds[j] = scores<T, DP>(lg + S::slab(32 * j), vcol);
         }
-        if (n0 < beg_last) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (n0 + row_of(i, half) < beg) p[i] = ds[i] = 0.f;
+        for (int j = 0; j < R; ++j) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(ll + 32 * j + 8 * b + 4 * half);
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(ldl + 32 * j + 8 * b + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 4 * b + e;
+                    p[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j][i], c, -l4[e]));
+                    ds[j][i] = p[j][i] * (ds[j][i] - d4[e]);
+                }
+            }
+            if (n0 + 32 * j < beg_last) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (n0 + 32 * j + row_of(i, half) < beg) p[j][i] = ds[j][i] = 0.f;
+            }
         }
         if (mend) {
             __syncthreads();
@@ -837,14 +876,18 @@ __global__ __launch_bounds__(NW * kWave) void k_attn_dkv(AttnArgs a) {
             look_over<T, DP, NW, BN, true>(lg, nullptr, 0);
             __syncthreads();
         }
-        add_products<DP>(dv, lg, p);
-        add_products<DP>(dk, lq, ds);
-        if (mend) {
-            unsigned seen = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) seen |= (n0 + row_of(i, half) >= beg ? 1u : 0u) << i;
-            add_non_finite<T, DP>(dv, p, seen, n0, rows, a.dim, g_at);
-            add_non_finite<T, DP>(dk, ds, seen, n0, rows, a.dim, q_at);
+        for (int j = 0; j < R; ++j) {
+            add_products<DP>(dv, lg + S::slab(32 * j), p[j]);
+            add_products<DP>(dk, lq + S::slab(32 * j), ds[j]);
+            if (mend) {
+                unsigned seen = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    seen |= (n0 + 32 * j + row_of(i, half) >= beg ? 1u : 0u) << i;
+                add_non_finite<T, DP>(dv, p[j], seen, n0 + 32 * j, rows, a.dim, g_at);
+                add_non_finite<T, DP>(dk, ds[j], seen, n0 + 32 * j, rows, a.dim, q_at);
+            }
         }
     }
     if (!mine) return;
@@ -874,14 +917,17 @@ struct Plan {
 // cols: rows of the axis whose tiles the grid walks; streamed: the other's.
 inline Plan plan_of(long long cols, long long streamed, int count, int kv_heads) {
     const int n = count > 0 ? count : 1;
+    auto tiles = [&](int waves) {
+        return std::max<long long>(n, (cols + 32 * waves - 1) / (32 * waves)) * kv_heads;
+    };
     Plan p;
-    p.waves = cols <= 32ll * n ? 1 : 4;
-    const long long bm = 32 * p.waves;
-    const long long tiles = std::max<long long>(n, (cols + bm - 1) / bm) * kv_heads;
-    // Below about 8 waves a CU the axis is split, into parts of at least 128 rows
-    const long long want = (256ll * 8 / p.waves + tiles - 1) / tiles;
-    const long long most = streamed / n / 128;
-    p.splits = (int)std::max<long long>(1, std::min<long long>({want, most, 128}));
+    // A workgroup shares its row tiles between its waves; short sequences fill one or two,
+    // and fewer than 4 workgroups a CU leave CUs idle behind the longest.
+    p.waves = cols <= 32ll * n ? 1 : cols <= 64ll * n || tiles(4) < 4 * 256 ? 2 : 4;
+    // Fewer waves than 3 a SIMD: the streamed axis is split, into 256 rows or more each.
+    const long long waves = tiles(p.waves) * p.waves;
+    const long long want = (3ll * 4 * 256 + waves - 1) / waves;
+    p.splits = (int)std::max<long long>(1, std::min<long long>({want, streamed / n / 256, 128}));
     return p;
 }
 
@@ -938,16 +984,20 @@ int attn_launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
     const bool keys = PASS == kDkv;
     const long long slots = slots_of(keys ? a.nk : a.nq, keys ? 1 : a.group, 32 * p.waves, a.count);
     const dim3 grid((unsigned)slots, a.kv_heads, p.splits);
-    [[maybe_unused]] constexpr int R = sizeof(T) == 2 ? 2 : 1;  // 32-row tiles a step of the forward
-    if (p.waves == 1) {
-        if constexpr (PASS == kFwd) k_attn_fwd<T, DP, 1, 1><<<grid, 64, 0, s>>>(a);
-        if constexpr (PASS == kDq) k_attn_dq<T, DP, 1><<<grid, 64, 0, s>>>(a);
-        if constexpr (PASS == kDkv) k_attn_dkv<T, DP, 1><<<grid, 64, 0, s>>>(a);
-    } else {
-        if constexpr (PASS == kFwd) k_attn_fwd<T, DP, 4, R><<<grid, 256, 0, s>>>(a);
-        if constexpr (PASS == kDq) k_attn_dq<T, DP, 4><<<grid, 256, 0, s>>>(a);
-        if constexpr (PASS == kDkv) k_attn_dkv<T, DP, 4><<<grid, 256, 0, s>>>(a);
-    }
+    // 32-row tiles a step: two where the registers allow it (their chains interleave)
+    constexpr int R = sizeof(T) == 4 ? 1 : PASS == kFwd ? 2 : DP <= 64 ? 2 : 1;
+    auto call = [&](auto waves) {
+        constexpr int NW = decltype(waves)::value;
+        if constexpr (PASS == kFwd) k_attn_fwd<T, DP, NW, NW == 4 ? R : 1><<<grid, 64 * NW, 0, s>>>(a);
+        if constexpr (PASS == kDq) k_attn_dq<T, DP, NW, R><<<grid, 64 * NW, 0, s>>>(a);
+        if constexpr (PASS == kDkv) k_attn_dkv<T, DP, NW, R><<<grid, 64 * NW, 0, s>>>(a);
+    };
+    if (p.waves == 1)
+        call(std::integral_constant<int, 1>());
+    else if (p.waves == 2)
+        call(std::integral_constant<int, 2>());
+    else
+        call(std::integral_constant<int, 4>());
     return status_of(hipGetLastError());
 }
 
@@ -995,8 +1045,8 @@ int gat_packed_attention(const void* q, long long q_row, long long q_head, const
                          long long k_row, long long k_head, const void* v, long long v_row,
                          long long v_head, const void* ptr, const void* kv_ptr, int ptr64, int count,
                          int nq, int nk, int heads, int kv_heads, int dim, float scale, int causal,
-                         void* out, float* lse, void* workspace, size_t workspace_bytes, int dtype,
-                         void* stream) {
+                         void* out, void* low, float* lse, void* workspace, size_t workspace_bytes,
+                         int dtype, void* stream) {
     const int rc = attn_check(nq, nk, count, heads, kv_heads, dim, dtype);
     if (rc != GAT_OK) return rc;
     if (nq == 0) return GAT_OK;
@@ -1013,7 +1063,8 @@ int gat_packed_attention(const void* q, long long q_row, long long q_head, const
     const AttnSizes sz = attn_sizes(nq, nk, count, heads, kv_heads, dim);
     if (sz.fwd_bytes > 0 && (workspace == nullptr || workspace_bytes < sz.fwd_bytes))
         return GAT_EWORKSPACE;
-    if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return GAT_EINVAL;
+    if (((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(low)) & 15) != 0)
+        return GAT_EINVAL;
     a.ptr = ptr;
     a.kv_ptr = kv_ptr;
     a.ptr64 = ptr64;
@@ -1026,6 +1077,7 @@ int gat_packed_attention(const void* q, long long q_row, long long q_head, const
     a.scale = scale;
     a.causal = causal;
     a.lse = lse;
+    a.low = dtype == GAT_F32 ? nullptr : low;
     a.part = static_cast<float*>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int st = attn_pass<kFwd>(a, sz.fwd, dtype, s);
@@ -1052,7 +1104,7 @@ int gat_packed_attention_backward_workspace_size(int nq, int nk, int count, int 
 int gat_packed_attention_backward(const void* g, long long g_row, long long g_head, const void* q,
                                   long long q_row, long long q_head, const void* k, long long k_row,
                                   long long k_head, const void* v, long long v_row, long long v_head,
-                                  const void* out, const float* lse, const void* ptr,
+                                  const void* out, const void* low, const float* lse, const void* ptr,
                                   const void* kv_ptr, int ptr64, int count, int nq, int nk, int heads,
                                   int kv_heads, int dim, float scale, int causal, void* dq, void* dk,
                                   void* dv, void* workspace, size_t workspace_bytes, int dtype,
@@ -1078,7 +1130,8 @@ int gat_packed_attention_backward(const void* g, long long g_row, long long g_he
     if (workspace_bytes < sz.delta_bytes + std::max(sz.dq_bytes, sz.dkv_bytes) ||
         (workspace == nullptr && workspace_bytes > 0))
         return GAT_EWORKSPACE;
-    if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return GAT_EINVAL;
+    if (((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(low)) & 15) != 0)
+        return GAT_EINVAL;
     a.ptr = ptr;
     a.kv_ptr = kv_ptr;
     a.ptr64 = ptr64;
@@ -1091,6 +1144,7 @@ int gat_packed_attention_backward(const void* g, long long g_row, long long g_he
     a.scale = scale;
     a.causal = causal;
     a.lse = const_cast<float*>(lse);
+    a.low = dtype == GAT_F32 ? nullptr : const_cast<void*>(low);
     a.delta = static_cast<float*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sz.delta_bytes);
     hipStream_t s = static_cast<hipStream_t>(stream);

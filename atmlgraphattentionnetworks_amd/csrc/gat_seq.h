@@ -36,9 +36,10 @@ __device__ __forceinline__ typename Vec16<T>::type load_vec(const T* row, int co
         v = typename Vec16<T>::type{};
         if (col0 < cols && col0 + N > 0) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
+            for (int e = 0; e < N; ++e) {  // no branch between the loads: one wait for all
                 const int c = col0 + e;
-                if (c >= 0 && c < cols) v[e] = row[c];
+                const T x = row[c < 0 ? 0 : c < cols ? c : cols - 1];
+                v[e] = c >= 0 && c < cols ? x : (T)0.f;
             }
         }
     }

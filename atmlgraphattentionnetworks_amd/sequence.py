@@ -283,13 +283,14 @@ def _vectors(t: torch.Tensor) -> torch.Tensor:
     return torch.nn.functional.pad(t, (0, -d % n))
 
 
-def _attn_forward(q, k, v, ptr, kv_ptr, causal, scale, want_lse):
+def _attn_forward(q, k, v, ptr, kv_ptr, causal, scale, want_lse, want_low=False):
     """``q``, ``k``, ``v`` as :func:`_vectors` gives them."""
     nq, h, d = q.shape
     nk, hk = k.shape[:2]
     dev, dt, count = q.device, _DTYPES[q.dtype], ptr.numel() - 1
     out = torch.empty(nq, h, d, dtype=q.dtype, device=dev)
     lse = torch.empty(nq, h, dtype=torch.float32, device=dev) if want_lse else None
+    low = torch.empty_like(out) if want_low and dt != _lib.GAT_F32 else None
     size = _lib.packed_attention_workspace_size(False, nq, nk, count, h, hk, d, dt)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     with _on(dev):
@@ -297,10 +298,10 @@ def _attn_forward(q, k, v, ptr, kv_ptr, causal, scale, want_lse):
             q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
             v.data_ptr(), v.stride(0), v.stride(1), ptr.data_ptr(), kv_ptr.data_ptr(),
             int(ptr.dtype == torch.int64), count, nq, nk, h, hk, d, scale, int(causal),
-            out.data_ptr(), _ptr(lse), _ptr(ws), size, dt, _stream(dev))
+            out.data_ptr(), _ptr(low), _ptr(lse), _ptr(ws), size, dt, _stream(dev))
     if rc:
         _lib.check(rc, "gat_packed_attention")
-    return out, lse
+    return out, lse, low
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -308,8 +309,8 @@ class _PackedAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, ptr, kv_ptr, causal, scale):
         d = q.shape[2]
         q, k, v = _vectors(q), _vectors(k), _vectors(v)
-        out, lse = _attn_forward(q, k, v, ptr, kv_ptr, causal, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, ptr, kv_ptr)
+        out, lse, low = _attn_forward(q, k, v, ptr, kv_ptr, causal, scale, True, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, ptr, kv_ptr)
         ctx.causal, ctx.scale, ctx.dim = causal, scale, d
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)  # no zeros for lse
@@ -318,7 +319,7 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
-        q, k, v, out, lse, ptr, kv_ptr = ctx.saved_tensors
+        q, k, v, out, low, lse, ptr, kv_ptr = ctx.saved_tensors
         if g is None:
             return (None,) * 7
         g = _vectors(g)
@@ -333,7 +334,7 @@ class _PackedAttention(torch.autograd.Function):
             rc = _lib.load().gat_packed_attention_backward(
                 g.data_ptr(), g.stride(0), g.stride(1), q.data_ptr(), q.stride(0), q.stride(1),
                 k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                out.data_ptr(), lse.data_ptr(), ptr.data_ptr(), kv_ptr.data_ptr(),
+                out.data_ptr(), _ptr(low), lse.data_ptr(), ptr.data_ptr(), kv_ptr.data_ptr(),
                 int(ptr.dtype == torch.int64), count, nq, nk, h, hk, d, ctx.scale,
                 int(ctx.causal), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), size,
                 dt, _stream(dev))
@@ -407,7 +408,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _PackedAttention.apply(q, k, v, ptr, kv_ptr, bool(causal), scale)
         return (out, lse) if return_lse else out
-    out, lse = _attn_forward(_vectors(q), _vectors(k), _vectors(v), ptr, kv_ptr, bool(causal),
-                             scale, return_lse)
+    out, lse, _ = _attn_forward(_vectors(q), _vectors(k), _vectors(v), ptr, kv_ptr, bool(causal),
+                                scale, return_lse)
     out = out if out.shape[2] == d else out[..., :d].contiguous()
     return (out, lse) if return_lse else out

@@ -646,13 +646,17 @@ int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void*
  *   out = softmax(scale q k^T) v over the sequence's visible keys
  * causal: key j of a sequence is visible to its query i iff j <= i + (keys - queries).
  *   q        [nq, heads, dim], k, v [nk, kv_heads, dim]: GAT_F32 or GAT_BF16, token and head
- *            strides in elements; addresses and strides multiples of 16 bytes, dim a
+ *            strides in elements; addresses and strides multiples of 16 bytes, token
+ *            strides of dim to 2^22 elements, heads / kv_heads * head stride up to 2^28, dim a
  *            multiple of 16 bytes of elements and <= GAT_PACKED_MAX_DIM (GAT_EUNSUPPORTED
  *            otherwise); heads a multiple of kv_heads
  *   ptr, kv_ptr  [count + 1] int64 if ptr64, else int32, ascending.  Boundaries outside
  *            [0, nq] / [0, nk] are held to it: nothing outside the tensors is touched.
  *   out      [nq, heads, dim] contiguous.  Queries that see no key (an empty sequence, causal
  *            queries before the first key) and rows outside all sequences: zeros
+ *   low      bfloat16: as out, the part of each result that out's rounding leaves (16-byte
+ *            aligned), from which the backward forms sum_d g out more exactly; may be NULL.
+ *            Not used in float32
  *   lse      [nq, heads] float32 log of the softmax sum (-inf where no key is seen);
  *            may be NULL
  *   workspace  16-byte aligned, gat_packed_attention_workspace_size bytes
@@ -664,12 +668,12 @@ int gat_packed_attention(const void* q, long long q_row, long long q_head, const
                          long long k_row, long long k_head, const void* v, long long v_row,
                          long long v_head, const void* ptr, const void* kv_ptr, int ptr64, int count,
                          int nq, int nk, int heads, int kv_heads, int dim, float scale, int causal,
-                         void* out, float* lse, void* workspace, size_t workspace_bytes, int dtype,
-                         void* stream);
+                         void* out, void* low, float* lse, void* workspace, size_t workspace_bytes,
+                         int dtype, void* stream);
 
 /*
  * Gradients of gat_packed_attention for the incoming gradient g [nq, heads, dim] (strides as
- * q's); out and lse as the forward stored them.  dq [nq, heads, dim], dk, dv
+ * q's); out, low (or NULL) and lse as the forward stored them.  dq [nq, heads, dim], dk, dv
  * [nk, kv_heads, dim] contiguous; dk and dv are sums over the query heads of a key head.
  * Rows outside all sequences get zeros.  Deterministic.
  */
@@ -678,7 +682,7 @@ int gat_packed_attention_backward_workspace_size(int nq, int nk, int count, int 
 int gat_packed_attention_backward(const void* g, long long g_row, long long g_head, const void* q,
                                   long long q_row, long long q_head, const void* k, long long k_row,
                                   long long k_head, const void* v, long long v_row, long long v_head,
-                                  const void* out, const float* lse, const void* ptr,
+                                  const void* out, const void* low, const float* lse, const void* ptr,
                                   const void* kv_ptr, int ptr64, int count, int nq, int nk, int heads,
                                   int kv_heads, int dim, float scale, int causal, void* dq, void* dk,
                                   void* dv, void* workspace, size_t workspace_bytes, int dtype,
