@@ -442,8 +442,6 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
     auto v_at = [&](int row) { return vb + (long long)row * a.v.row; };
     const float c = score_scale(a.scale) * kLog2e;
 
-    f32x16 acc[S::DT] = {};
-    float m = -INFINITY, l = 0.f;
     Loader<T, DP, NW, BN> kl, vl;
     kl.init(a.k.row, a.dim);
     vl.init(a.v.row, a.dim);
@@ -451,63 +449,82 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
         kl.load(kb + (long long)n0 * a.k.row, a.k.row, nk - n0, a.dim, to_lds);
         vl.load(vb + (long long)n0 * a.v.row, a.v.row, nk - n0, a.dim, to_lds + SLAB);
     };
-    if (from < to) load_tile(from, lds);
-    for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
-        T* lk = lds + 2 * SLAB * turn;
-        T* lv = lk + SLAB;
-        wait_loads();
+    f32x16 acc[S::DT];
+    float m, l;
+    // Returns false where it met a hidden infinity or NaN that only MEND knows to deal with.
+    auto pass = [&](auto mends) {
+        constexpr bool MEND = decltype(mends)::value;
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) acc[d] = f32x16{};
+        m = -INFINITY;
+        l = 0.f;
+        if (from < to) load_tile(from, lds);
+        for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
+            T* lk = lds + 2 * SLAB * turn;
+            T* lv = lk + SLAB;
+            wait_loads();
+            __syncthreads();
+            if (n0 + BN < to) load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
+            bool mend = false;
+            if (n0 + BN > lim_whole) {
+                look_over<T, DP, NW, BN, false>(lv, &bad, n0 + 1);
+                __syncthreads();
+                mend = bad == n0 + 1;
+                if (!MEND && mend) {
+                    wait_loads();
+                    return false;
+                }
+                if (MEND && mend) {
+                    look_over<T, DP, NW, BN, true>(lv, nullptr, 0);
+                    __syncthreads();
+                }
+            }
+            if (n0 >= lim_last) continue;
+            f32x16 s[R];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
+                if (n0 + 32 * j + 32 > lim_first) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[j][i]);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            if (__any((mx - m) * c > kRescale)) {  // -inf - -inf: false
+                const float to_m = fmaxf(m, mx);
+                const float f = m == -INFINITY ? 0.f : exp2f((m - to_m) * c);
+                m = to_m;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < S::DT; ++d) acc[d] *= f;
+            }
+            const float mc = m == -INFINITY ? 0.f : m * c;
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -mc));
+                    l += s[j][i];
+                }
+                add_products<DP>(acc, lv + S::slab(32 * j), s[j]);
+                if (MEND && mend) {
+                    unsigned seen = 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
+                    add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, v_at);
+                }
+            }
+        }
+        return true;
+    };
+    if (!pass(std::false_type())) {
         __syncthreads();
-        if (n0 + BN < to) load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
-        bool mend = false;
-        if (n0 + BN > lim_whole) {
-            look_over<T, DP, NW, BN, false>(lv, &bad, n0 + 1);
-            __syncthreads();
-            mend = bad == n0 + 1;
-        }
-        if (n0 >= lim_last && !mend) continue;
-        f32x16 s[R];
-        float mx = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
-            if (n0 + 32 * j + 32 > lim_first) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[j][i]);
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        if (__any((mx - m) * c > kRescale)) {  // -inf - -inf: false
-            const float to_m = fmaxf(m, mx);
-            const float f = m == -INFINITY ? 0.f : exp2f((m - to_m) * c);
-            m = to_m;
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < S::DT; ++d) acc[d] *= f;
-        }
-        const float mc = m == -INFINITY ? 0.f : m * c;
-        if (mend) {
-            look_over<T, DP, NW, BN, true>(lv, nullptr, 0);
-            __syncthreads();
-        }
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -mc));
-                l += s[j][i];
-            }
-            add_products<DP>(acc, lv + S::slab(32 * j), s[j]);
-            if (mend) {
-                unsigned seen = 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
-                add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, v_at);
-            }
-        }
+        pass(std::true_type());
     }
     l += __shfl_xor(l, 32);
     if (!mine) return;
@@ -668,7 +685,6 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
     auto k_at = [&](int row) { return kb + (long long)row * a.k.row; };
     const float c = score_scale(a.scale) * kLog2e;
 
-    f32x16 acc[S::DT] = {};
     Loader<T, DP, NW, BN> kl, vl;
     kl.init(a.k.row, a.dim);
     vl.init(a.v.row, a.dim);
@@ -676,55 +692,70 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
         kl.load(kb + (long long)n0 * a.k.row, a.k.row, nk - n0, a.dim, to_lds);
         vl.load(vb + (long long)n0 * a.v.row, a.v.row, nk - n0, a.dim, to_lds + SLAB);
     };
-    if (from < to) load_tile(from, lds);
-    for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
-        T* lk = lds + 2 * SLAB * turn;
-        T* lv = lk + SLAB;
-        wait_loads();
+    f32x16 acc[S::DT];
+    auto pass = [&](auto mends) {
+        constexpr bool MEND = decltype(mends)::value;
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) acc[d] = f32x16{};
+        if (from < to) load_tile(from, lds);
+        for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
+            T* lk = lds + 2 * SLAB * turn;
+            T* lv = lk + SLAB;
+            wait_loads();
+            __syncthreads();
+            if (n0 + BN < to) load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
+            bool mend = false;
+            if (n0 + BN > lim_whole) {
+                look_over<T, DP, NW, BN, false>(lk, &bad, n0 + 1);
+                __syncthreads();
+                mend = bad == n0 + 1;
+                if (!MEND && mend) {
+                    wait_loads();
+                    return false;
+                }
+            }
+            if (n0 >= lim_last && !(MEND && mend)) continue;
+            f32x16 s[R], dp[R];
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
+                dp[j] = scores<T, DP>(lv + S::slab(32 * j), gc);
+            }
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -lse2));
+                    s[j][i] = p * (dp[j][i] - delta);
+                }
+                if (n0 + 32 * j + 32 > lim_first) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = 0.f;
+                }
+            }
+            if (MEND && mend) {  // the scores need the keys as they are, the product needs them cleared
+                __syncthreads();
+                look_over<T, DP, NW, BN, true>(lk, nullptr, 0);
+                __syncthreads();
+            }
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                add_products<DP>(acc, lk + S::slab(32 * j), s[j]);
+                if (MEND && mend) {
+                    unsigned seen = 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
+                    add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, k_at);
+                }
+            }
+        }
+        return true;
+    };
+    if (!pass(std::false_type())) {
         __syncthreads();
-        if (n0 + BN < to) load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
-        bool mend = false;
-        if (n0 + BN > lim_whole) {
-            look_over<T, DP, NW, BN, false>(lk, &bad, n0 + 1);
-            __syncthreads();
-            mend = bad == n0 + 1;
-        }
-        if (n0 >= lim_last && !mend) continue;
-        f32x16 s[R], dp[R];
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
-            dp[j] = scores<T, DP>(lv + S::slab(32 * j), gc);
-        }
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -lse2));
-                s[j][i] = p * (dp[j][i] - delta);
-            }
-            if (n0 + 32 * j + 32 > lim_first) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = 0.f;
-            }
-        }
-        if (mend) {
-            __syncthreads();
-            look_over<T, DP, NW, BN, true>(lk, nullptr, 0);
-            __syncthreads();
-        }
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            add_products<DP>(acc, lk + S::slab(32 * j), s[j]);
-            if (mend) {
-                unsigned seen = 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
-                add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, k_at);
-            }
-        }
+        pass(std::true_type());
     }
     if (!mine) return;
     if (a.splits > 1) {
@@ -797,98 +828,117 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
         const int i = div_group(a, row);
         return gb + (long long)i * a.g.row + (long long)(row - i * a.group) * a.g.head;
     };
-    // lse (in log2) and delta of a row tile, a row each of the first wave's lanes
-    float rl = 0.f, rd = 0.f;
+    // lse (in log2) and delta of a row tile
+    constexpr int NT = NW * kWave, PER = (BN + NT - 1) / NT;
+    float rl[PER], rd[PER];
     auto load_sums = [&](int n0) {
-        const int row = n0 + threadIdx.x;
-        const bool in = threadIdx.x < BN && row < rows;
-        if (threadIdx.x < BN) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int row = n0 + j * NT + threadIdx.x;
+            const bool in = j * NT + threadIdx.x < BN && row < rows;
             const int i = in ? div_group(a, row) : 0;
-            const long long qh = ((long long)(q0 + i) * a.kv_heads + kh) * a.group + (row - i * a.group);
-            rl = in ? a.lse[qh] * kLog2e : INFINITY;  // exp(s - inf) = 0 behind the last row
-            rd = in ? a.delta[qh] : 0.f;
+            const long long qh =
+                in ? ((long long)(q0 + i) * a.kv_heads + kh) * a.group + (row - i * a.group) : 0;
+            rl[j] = in ? a.lse[qh] * kLog2e : INFINITY;  // exp(s - inf) = 0 behind the last row
+            rd[j] = in ? a.delta[qh] : 0.f;
         }
     };
     const float c = score_scale(a.scale) * kLog2e;
 
-    f32x16 dk[S::DT] = {}, dv[S::DT] = {};
     Loader<T, DP, NW, BN> ld;
     ld.init(0, a.dim);
     auto load_tile = [&](int n0, T* to_lds) {
         ld.load_packed(a, qb, a.q, n0, rows, to_lds);
         ld.load_packed(a, gb, a.g, n0, rows, to_lds + SLAB);
     };
-    if (from < to) {
-        load_sums(from);
-        load_tile(from, lds);
-    }
-    for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
-        T* lq = lds + 2 * SLAB * turn;
-        T* lg = lq + SLAB;
-        const float* ll = sums[turn][0];
-        const float* ldl = sums[turn][1];
-        if (threadIdx.x < BN) {
-            sums[turn][0][threadIdx.x] = rl;
-            sums[turn][1][threadIdx.x] = rd;
+    f32x16 dk[S::DT], dv[S::DT];
+    auto pass = [&](auto mends) {
+        constexpr bool MEND = decltype(mends)::value;
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) dk[d] = dv[d] = f32x16{};
+        if (from < to) {
+            load_sums(from);
+            load_tile(from, lds);
         }
-        wait_loads();
-        __syncthreads();
-        if (n0 + BN < to) {
-            load_sums(n0 + BN);
-            load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
-        }
-        bool mend = false;
-        if (n0 < beg_whole) {
-            look_over<T, DP, NW, BN, false>(lq, &bad, n0 + 1);
-            look_over<T, DP, NW, BN, false>(lg, &bad, n0 + 1);
+        for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
+            T* lq = lds + 2 * SLAB * turn;
+            T* lg = lq + SLAB;
+            const float* ll = sums[turn][0];
+            const float* ldl = sums[turn][1];
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (j * NT + threadIdx.x < BN) {
+                    sums[turn][0][j * NT + threadIdx.x] = rl[j];
+                    sums[turn][1][j * NT + threadIdx.x] = rd[j];
+                }
+            wait_loads();
             __syncthreads();
-            mend = bad == n0 + 1;
-        }
-        if (n0 + BN <= beg_first && !mend) continue;
-        f32x16 p[R], ds[R];
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            p[j] = scores<T, DP>(lq + S::slab(32 * j), kcol);
-            ds[j] = scores<T, DP>(lg + S::slab(32 * j), vcol);
-        }
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(ll + 32 * j + 8 * b + 4 * half);
-                const f32x4 d4 = *reinterpret_cast<const f32x4*>(ldl + 32 * j + 8 * b + 4 * half);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = 4 * b + e;
-                    p[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j][i], c, -l4[e]));
-                    ds[j][i] = p[j][i] * (ds[j][i] - d4[e]);
+            if (n0 + BN < to) {
+                load_sums(n0 + BN);
+                load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
+            }
+            bool mend = false;
+            if (n0 < beg_whole) {
+                look_over<T, DP, NW, BN, false>(lq, &bad, n0 + 1);
+                look_over<T, DP, NW, BN, false>(lg, &bad, n0 + 1);
+                __syncthreads();
+                mend = bad == n0 + 1;
+                if (!MEND && mend) {
+                    wait_loads();
+                    return false;
                 }
             }
-            if (n0 + 32 * j < beg_last) {
+            if (n0 + BN <= beg_first && !(MEND && mend)) continue;
+            f32x16 p[R], ds[R];
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (n0 + 32 * j + row_of(i, half) < beg) p[j][i] = ds[j][i] = 0.f;
+            for (int j = 0; j < R; ++j) {
+                p[j] = scores<T, DP>(lq + S::slab(32 * j), kcol);
+                ds[j] = scores<T, DP>(lg + S::slab(32 * j), vcol);
+            }
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(ll + 32 * j + 8 * b + 4 * half);
+                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(ldl + 32 * j + 8 * b + 4 * half);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = 4 * b + e;
+                        p[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j][i], c, -l4[e]));
+                        ds[j][i] = p[j][i] * (ds[j][i] - d4[e]);
+                    }
+                }
+                if (n0 + 32 * j < beg_last) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (n0 + 32 * j + row_of(i, half) < beg) p[j][i] = ds[j][i] = 0.f;
+                }
+            }
+            if (MEND && mend) {
+                __syncthreads();
+                look_over<T, DP, NW, BN, true>(lq, nullptr, 0);
+                look_over<T, DP, NW, BN, true>(lg, nullptr, 0);
+                __syncthreads();
+            }
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                add_products<DP>(dv, lg + S::slab(32 * j), p[j]);
+                add_products<DP>(dk, lq + S::slab(32 * j), ds[j]);
+                if (MEND && mend) {
+                    const int n = n0 + 32 * j;
+                    unsigned seen = 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) seen |= (n + row_of(i, half) >= beg ? 1u : 0u) << i;
+                    add_non_finite<T, DP>(dv, p[j], seen, n, rows, a.dim, g_at);
+                    add_non_finite<T, DP>(dk, ds[j], seen, n, rows, a.dim, q_at);
+                }
             }
         }
-        if (mend) {
-            __syncthreads();
-            look_over<T, DP, NW, BN, true>(lq, nullptr, 0);
-            look_over<T, DP, NW, BN, true>(lg, nullptr, 0);
-            __syncthreads();
-        }
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            add_products<DP>(dv, lg + S::slab(32 * j), p[j]);
-            add_products<DP>(dk, lq + S::slab(32 * j), ds[j]);
-            if (mend) {
-                unsigned seen = 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    seen |= (n0 + 32 * j + row_of(i, half) >= beg ? 1u : 0u) << i;
-                add_non_finite<T, DP>(dv, p[j], seen, n0 + 32 * j, rows, a.dim, g_at);
-                add_non_finite<T, DP>(dk, ds[j], seen, n0 + 32 * j, rows, a.dim, q_at);
-            }
-        }
+        return true;
+    };
+    if (!pass(std::false_type())) {
+        __syncthreads();
+        pass(std::true_type());
     }
     if (!mine) return;
     if (a.splits > 1) {
