@@ -277,6 +277,9 @@ __device__ __forceinline__ void add_non_finite(f32x16* acc, f32x16 w, unsigned s
                     const int d = 32 * t + row_of(e, half);
                     const float v = d < dim ? (float)x[d] : 0.f;
                     if (non_finite(v)) acc[t][e] += f * v;
+                    // one value at a time: all of them in flight would take the registers
+                    // that the ordinary tiles need
+                    asm volatile("" ::: "memory");
                 }
         }
     }
@@ -288,11 +291,12 @@ __device__ __forceinline__ void add_non_finite(f32x16* acc, f32x16 w, unsigned s
 // rows behind it and dimensions behind `dim` arrive as zeros.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned offset, unsigned lds) {
+__device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned offset, int scalar_offset,
+                                            unsigned lds) {
     // m0 holds the LDS address; the nops cover scalar operands that a vector instruction wrote
     asm volatile(
-        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset),
-        "s"(buffer)
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds),
+        "v"(offset), "s"(buffer), "s"(scalar_offset)
         : "memory");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -318,11 +322,15 @@ struct Loader {
     typedef Shape<T, DP> S;
     static constexpr int LOADS = (BN * S::CPR + kWave - 1) / kWave;  // of a wave each
     static constexpr int CNT = (LOADS + NW - 1) / NW;
-    unsigned offset[CNT];  // of this lane's vectors within a tile
+    // A wave's loads lie STEP rows apart; where that is a multiple of 8 they differ by a
+    // scalar only.
+    static constexpr int STEP = NW * kWave % S::CPR == 0 ? NW * kWave / S::CPR : 0;
+    static constexpr bool EVEN = CNT == 1 || (STEP > 0 && STEP % 8 == 0);
+    unsigned offset[EVEN ? 1 : CNT];  // of this lane's vectors within a tile
 
     __device__ __forceinline__ void init(long long row_elements, int dim) {
 #pragma unroll
-        for (int j = 0; j < CNT; ++j) {
+        for (int j = 0; j < (EVEN ? 1 : CNT); ++j) {
             const int at = (threadIdx.x / kWave + NW * j) * kWave + threadIdx.x % kWave;
             const int r = at / S::CPR, c = at % S::CPR ^ S::turn(r);
             offset[j] = c * S::N < dim ? (unsigned)(r * (int)row_elements + c * S::N) * (unsigned)sizeof(T)
@@ -330,17 +338,17 @@ struct Loader {
         }
     }
     // rows [0, rows) from `base` on, into `lds`
-    __device__ __forceinline__ void load(const T* base, long long row_elements, int rows, int dim,
+    __device__ __forceinline__ void load(const T* base, int row_elements, int rows, int dim,
                                          T* lds) const {
         const int n = rows < BN ? rows : BN;
-        const i32x4 b =
-            make_buffer(base, (unsigned)((n - 1) * (int)row_elements + dim) * (unsigned)sizeof(T));
+        const i32x4 b = make_buffer(base, (unsigned)((n - 1) * row_elements + dim) * (unsigned)sizeof(T));
         const unsigned to = lds_address(lds);
 #pragma unroll
         for (int j = 0; j < CNT; ++j) {
             const int k = uniform(threadIdx.x / kWave) + NW * j;
             if (LOADS % NW != 0 && k >= LOADS) break;
-            load_to_lds(b, offset[j], uniform((int)(to + k * kWave * 16)));
+            load_to_lds(b, offset[EVEN ? 0 : j], EVEN ? j * STEP * row_elements * (int)sizeof(T) : 0,
+                        uniform((int)(to + k * kWave * 16)));
         }
     }
     // The same for rows of the packed (query, head of the group) axis: rows [r0, end), row r
@@ -357,8 +365,8 @@ struct Loader {
             const int at = k * kWave + threadIdx.x % kWave;
             const int r = r0 + at / S::CPR, i = div_group(a, r);
             const unsigned o = (unsigned)((i - i0) * (int)x.row + (r - i * a.group) * (int)x.head) *
-                                   (unsigned)sizeof(T) + offset[j];
-            load_to_lds(b, r < end ? o : 0x80000000u, uniform((int)(to + k * kWave * 16)));
+                                   (unsigned)sizeof(T) + offset[EVEN ? 0 : j];
+            load_to_lds(b, r < end ? o : 0x80000000u, 0, uniform((int)(to + k * kWave * 16)));
         }
     }
 };
@@ -424,7 +432,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
     const int lim_last = uniform(r0 < rows ? limit(r0 + 31 < rows ? r0 + 31 : rows - 1) : 0);
     const int last = t.index * BM + BM - 1;
     const int lim_block = uniform(limit(last < rows ? last : rows - 1));
-    const int lim_whole = uniform(a.causal ? limit(t.index * BM) : INT_MAX);  // keys that all rows see
+    const int lim_whole = uniform(limit(t.index * BM));  // keys that all rows see
     int from = 0, to = lim_block;
     if (a.splits > 1) {
         const int per = ((lim_block + a.splits - 1) / a.splits + BN - 1) / BN * BN;
@@ -446,85 +454,81 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
     kl.init(a.k.row, a.dim);
     vl.init(a.v.row, a.dim);
     auto load_tile = [&](int n0, T* to_lds) {
-        kl.load(kb + (long long)n0 * a.k.row, a.k.row, nk - n0, a.dim, to_lds);
-        vl.load(vb + (long long)n0 * a.v.row, a.v.row, nk - n0, a.dim, to_lds + SLAB);
+        kl.load(kb + (long long)n0 * a.k.row, (int)a.k.row, nk - n0, a.dim, to_lds);
+        vl.load(vb + (long long)n0 * a.v.row, (int)a.v.row, nk - n0, a.dim, to_lds + SLAB);
     };
-    f32x16 acc[S::DT];
-    float m, l;
-    // Returns false where it met a hidden infinity or NaN that only MEND knows to deal with.
-    auto pass = [&](auto mends) {
-        constexpr bool MEND = decltype(mends)::value;
+    f32x16 acc[S::DT] = {};
+    float m = -INFINITY, l = 0.f;
+    // One tile.  MASK: some column may not see all of its rows; mend: and a hidden one may
+    // hold an infinity or NaN.
+    auto tile = [&](int n0, const T* lk, const T* lv, auto masks, bool mend) {
+        constexpr bool MASK = decltype(masks)::value;
+        f32x16 s[R];
+        float mx = -INFINITY;
 #pragma unroll
-        for (int d = 0; d < S::DT; ++d) acc[d] = f32x16{};
-        m = -INFINITY;
-        l = 0.f;
-        if (from < to) load_tile(from, lds);
-        for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
-            T* lk = lds + 2 * SLAB * turn;
-            T* lv = lk + SLAB;
-            wait_loads();
-            __syncthreads();
-            if (n0 + BN < to) load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
-            bool mend = false;
-            if (n0 + BN > lim_whole) {
-                look_over<T, DP, NW, BN, false>(lv, &bad, n0 + 1);
-                __syncthreads();
-                mend = bad == n0 + 1;
-                if (!MEND && mend) {
-                    wait_loads();
-                    return false;
-                }
-                if (MEND && mend) {
-                    look_over<T, DP, NW, BN, true>(lv, nullptr, 0);
-                    __syncthreads();
-                }
+        for (int j = 0; j < R; ++j) {
+            s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
+            if (MASK) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = -INFINITY;
             }
-            if (n0 >= lim_last) continue;
-            f32x16 s[R];
-            float mx = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-                s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
-                if (n0 + 32 * j + 32 > lim_first) {
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[j][i]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        if (__any((mx - m) * c > kRescale)) {  // -inf - -inf: false
+            const float to_m = fmaxf(m, mx);
+            const float f = m == -INFINITY ? 0.f : exp2f((m - to_m) * c);
+            m = to_m;
+            l *= f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = -INFINITY;
-                }
+            for (int d = 0; d < S::DT; ++d) acc[d] *= f;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[j][i]);
+        for (int j = 0; j < R; ++j) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -mc));
+                l += s[j][i];
             }
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            if (__any((mx - m) * c > kRescale)) {  // -inf - -inf: false
-                const float to_m = fmaxf(m, mx);
-                const float f = m == -INFINITY ? 0.f : exp2f((m - to_m) * c);
-                m = to_m;
-                l *= f;
+            add_products<DP>(acc, lv + S::slab(32 * j), s[j]);
+            if (MASK && mend) {
+                unsigned seen = 0;
 #pragma unroll
-                for (int d = 0; d < S::DT; ++d) acc[d] *= f;
-            }
-            const float mc = m == -INFINITY ? 0.f : m * c;
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -mc));
-                    l += s[j][i];
-                }
-                add_products<DP>(acc, lv + S::slab(32 * j), s[j]);
-                if (MEND && mend) {
-                    unsigned seen = 0;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
-                    add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, v_at);
-                }
+                for (int i = 0; i < 16; ++i)
+                    seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
+                add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, v_at);
             }
         }
-        return true;
     };
-    if (!pass(std::false_type())) {
+    const int whole = lim_whole < to ? lim_whole : to;  // tiles up to here need no mask
+    int n0 = from, turn = 0;
+    auto arrive = [&]() {  // tile n0 is in LDS, the next one on its way
+        wait_loads();
         __syncthreads();
-        pass(std::true_type());
+        if (n0 + BN < to) load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
+        return lds + 2 * SLAB * turn;
+    };
+    if (from < to) load_tile(from, lds);
+    for (; n0 + BN <= whole; n0 += BN, turn ^= 1) {
+        const T* at = arrive();
+        tile(n0, at, at + SLAB, std::false_type(), false);
+    }
+    for (; n0 < to; n0 += BN, turn ^= 1) {
+        T* at = arrive();
+        bool mend = false;
+        if (a.causal) {
+            look_over<T, DP, NW, BN, false>(at + SLAB, &bad, n0 + 1);
+            __syncthreads();
+            mend = bad == n0 + 1;
+        }
+        if (mend) {
+            look_over<T, DP, NW, BN, true>(at + SLAB, nullptr, 0);
+            __syncthreads();
+        }
+        if (n0 < lim_last) tile(n0, at, at + SLAB, std::true_type(), mend);
     }
     l += __shfl_xor(l, 32);
     if (!mine) return;
@@ -648,7 +652,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
     const int lim_last = uniform(r0 < rows ? limit(r0 + 31 < rows ? r0 + 31 : rows - 1) : 0);
     const int last = t.index * BM + BM - 1;
     const int lim_block = uniform(limit(last < rows ? last : rows - 1));
-    const int lim_whole = uniform(a.causal ? limit(t.index * BM) : INT_MAX);  // keys that all rows see
+    const int lim_whole = uniform(limit(t.index * BM));  // keys that all rows see
     int from = 0, to = lim_block;
     if (a.splits > 1) {
         const int per = ((lim_block + a.splits - 1) / a.splits + BN - 1) / BN * BN;
@@ -689,73 +693,66 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
     kl.init(a.k.row, a.dim);
     vl.init(a.v.row, a.dim);
     auto load_tile = [&](int n0, T* to_lds) {
-        kl.load(kb + (long long)n0 * a.k.row, a.k.row, nk - n0, a.dim, to_lds);
-        vl.load(vb + (long long)n0 * a.v.row, a.v.row, nk - n0, a.dim, to_lds + SLAB);
+        kl.load(kb + (long long)n0 * a.k.row, (int)a.k.row, nk - n0, a.dim, to_lds);
+        vl.load(vb + (long long)n0 * a.v.row, (int)a.v.row, nk - n0, a.dim, to_lds + SLAB);
     };
-    f32x16 acc[S::DT];
-    auto pass = [&](auto mends) {
-        constexpr bool MEND = decltype(mends)::value;
+    f32x16 acc[S::DT] = {};
+    auto tile = [&](int n0, T* lk, const T* lv, auto masks, bool mend) {
+        constexpr bool MASK = decltype(masks)::value;
+        f32x16 s[R], dp[R];
 #pragma unroll
-        for (int d = 0; d < S::DT; ++d) acc[d] = f32x16{};
-        if (from < to) load_tile(from, lds);
-        for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
-            T* lk = lds + 2 * SLAB * turn;
-            T* lv = lk + SLAB;
-            wait_loads();
-            __syncthreads();
-            if (n0 + BN < to) load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
-            bool mend = false;
-            if (n0 + BN > lim_whole) {
-                look_over<T, DP, NW, BN, false>(lk, &bad, n0 + 1);
-                __syncthreads();
-                mend = bad == n0 + 1;
-                if (!MEND && mend) {
-                    wait_loads();
-                    return false;
-                }
-            }
-            if (n0 >= lim_last && !(MEND && mend)) continue;
-            f32x16 s[R], dp[R];
+        for (int j = 0; j < R; ++j) {
+            s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
+            dp[j] = scores<T, DP>(lv + S::slab(32 * j), gc);
+        }
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-                s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
-                dp[j] = scores<T, DP>(lv + S::slab(32 * j), gc);
-            }
+        for (int j = 0; j < R; ++j) {
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -lse2));
-                    s[j][i] = p * (dp[j][i] - delta);
-                }
-                if (n0 + 32 * j + 32 > lim_first) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = 0.f;
-                }
-            }
-            if (MEND && mend) {  // the scores need the keys as they are, the product needs them cleared
-                __syncthreads();
-                look_over<T, DP, NW, BN, true>(lk, nullptr, 0);
-                __syncthreads();
-            }
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-                add_products<DP>(acc, lk + S::slab(32 * j), s[j]);
-                if (MEND && mend) {
-                    unsigned seen = 0;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
-                    add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, k_at);
-                }
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -lse2));
+                s[j][i] = p * (dp[j][i] - delta);
+                if (MASK && n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = 0.f;
             }
         }
-        return true;
+        if (MASK && mend) {  // the scores need the keys as they are, the product needs them cleared
+            __syncthreads();
+            look_over<T, DP, NW, BN, true>(lk, nullptr, 0);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            add_products<DP>(acc, lk + S::slab(32 * j), s[j]);
+            if (MASK && mend) {
+                unsigned seen = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
+                add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, k_at);
+            }
+        }
     };
-    if (!pass(std::false_type())) {
+    const int whole = lim_whole < to ? lim_whole : to;
+    int n0 = from, turn = 0;
+    auto arrive = [&]() {
+        wait_loads();
         __syncthreads();
-        pass(std::true_type());
+        if (n0 + BN < to) load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
+        return lds + 2 * SLAB * turn;
+    };
+    if (from < to) load_tile(from, lds);
+    for (; n0 + BN <= whole; n0 += BN, turn ^= 1) {
+        T* at = arrive();
+        tile(n0, at, at + SLAB, std::false_type(), false);
+    }
+    for (; n0 < to; n0 += BN, turn ^= 1) {
+        T* at = arrive();
+        bool mend = false;
+        if (a.causal) {
+            look_over<T, DP, NW, BN, false>(at, &bad, n0 + 1);
+            __syncthreads();
+            mend = bad == n0 + 1;
+        }
+        if (n0 < lim_last || (mend)) tile(n0, at, at + SLAB, std::true_type(), mend);
     }
     if (!mine) return;
     if (a.splits > 1) {
@@ -777,7 +774,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
     typedef typename Vec16<T>::type V;
     constexpr int BM = 32 * NW, BN = 32 * R, SLAB = S::slab(BN);
     __shared__ __align__(16) T lds[4 * SLAB + S::kSlack];  // q and g, two tiles of each
-    __shared__ __align__(16) float sums[2][2][BN];          // lse and delta of their rows
+    __shared__ __align__(16) float sums[2 * 2 * BN];               // lse and delta of their rows
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
     const Tile t = tile_of(a.kv_ptr, a.ptr64, a.count, a.nk, 1, BM, blockIdx.x);
@@ -800,7 +797,6 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
     };
     const int beg = start(kc);
     const int beg_first = uniform(c0 < t.len ? start(c0) : rows);  // the wave's smallest
-    const int beg_last = uniform(start(c0 + 31 < t.len ? c0 + 31 : t.len - 1));
     // the first row from which on all of the workgroup's keys are seen
     const int beg_whole = start(t.index * BM + BM - 1 < t.len ? t.index * BM + BM - 1 : t.len - 1);
     int from = start(t.index * BM) / BN * BN, to = rows;
@@ -851,94 +847,81 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
         ld.load_packed(a, qb, a.q, n0, rows, to_lds);
         ld.load_packed(a, gb, a.g, n0, rows, to_lds + SLAB);
     };
-    f32x16 dk[S::DT], dv[S::DT];
-    auto pass = [&](auto mends) {
-        constexpr bool MEND = decltype(mends)::value;
+    f32x16 dk[S::DT] = {}, dv[S::DT] = {};
+    auto tile = [&](int n0, T* lq, T* lg, const float* ll, auto masks, bool mend) {
+        constexpr bool MASK = decltype(masks)::value;
+        f32x16 p[R], ds[R];
 #pragma unroll
-        for (int d = 0; d < S::DT; ++d) dk[d] = dv[d] = f32x16{};
-        if (from < to) {
-            load_sums(from);
-            load_tile(from, lds);
+        for (int j = 0; j < R; ++j) {
+            p[j] = scores<T, DP>(lq + S::slab(32 * j), kcol);
+            ds[j] = scores<T, DP>(lg + S::slab(32 * j), vcol);
         }
-        for (int n0 = from, turn = 0; n0 < to; n0 += BN, turn ^= 1) {
-            T* lq = lds + 2 * SLAB * turn;
-            T* lg = lq + SLAB;
-            const float* ll = sums[turn][0];
-            const float* ldl = sums[turn][1];
 #pragma unroll
-            for (int j = 0; j < PER; ++j)
-                if (j * NT + threadIdx.x < BN) {
-                    sums[turn][0][j * NT + threadIdx.x] = rl[j];
-                    sums[turn][1][j * NT + threadIdx.x] = rd[j];
+        for (int j = 0; j < R; ++j)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(ll + 32 * j + 8 * b + 4 * half);
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(ll + BN + 32 * j + 8 * b + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 4 * b + e;
+                    p[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j][i], c, -l4[e]));
+                    ds[j][i] = p[j][i] * (ds[j][i] - d4[e]);
+                    if (MASK && n0 + 32 * j + row_of(i, half) < beg) p[j][i] = ds[j][i] = 0.f;
                 }
-            wait_loads();
+            }
+        if (MASK && mend) {
             __syncthreads();
-            if (n0 + BN < to) {
-                load_sums(n0 + BN);
-                load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
-            }
-            bool mend = false;
-            if (n0 < beg_whole) {
-                look_over<T, DP, NW, BN, false>(lq, &bad, n0 + 1);
-                look_over<T, DP, NW, BN, false>(lg, &bad, n0 + 1);
-                __syncthreads();
-                mend = bad == n0 + 1;
-                if (!MEND && mend) {
-                    wait_loads();
-                    return false;
-                }
-            }
-            if (n0 + BN <= beg_first && !(MEND && mend)) continue;
-            f32x16 p[R], ds[R];
+            look_over<T, DP, NW, BN, true>(lq, nullptr, 0);
+            look_over<T, DP, NW, BN, true>(lg, nullptr, 0);
+            __syncthreads();
+        }
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-                p[j] = scores<T, DP>(lq + S::slab(32 * j), kcol);
-                ds[j] = scores<T, DP>(lg + S::slab(32 * j), vcol);
-            }
+        for (int j = 0; j < R; ++j) {
+            add_products<DP>(dv, lg + S::slab(32 * j), p[j]);
+            add_products<DP>(dk, lq + S::slab(32 * j), ds[j]);
+            if (MASK && mend) {
+                const int n = n0 + 32 * j;
+                unsigned seen = 0;
 #pragma unroll
-            for (int j = 0; j < R; ++j) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(ll + 32 * j + 8 * b + 4 * half);
-                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(ldl + 32 * j + 8 * b + 4 * half);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int i = 4 * b + e;
-                        p[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j][i], c, -l4[e]));
-                        ds[j][i] = p[j][i] * (ds[j][i] - d4[e]);
-                    }
-                }
-                if (n0 + 32 * j < beg_last) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (n0 + 32 * j + row_of(i, half) < beg) p[j][i] = ds[j][i] = 0.f;
-                }
-            }
-            if (MEND && mend) {
-                __syncthreads();
-                look_over<T, DP, NW, BN, true>(lq, nullptr, 0);
-                look_over<T, DP, NW, BN, true>(lg, nullptr, 0);
-                __syncthreads();
-            }
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-                add_products<DP>(dv, lg + S::slab(32 * j), p[j]);
-                add_products<DP>(dk, lq + S::slab(32 * j), ds[j]);
-                if (MEND && mend) {
-                    const int n = n0 + 32 * j;
-                    unsigned seen = 0;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) seen |= (n + row_of(i, half) >= beg ? 1u : 0u) << i;
-                    add_non_finite<T, DP>(dv, p[j], seen, n, rows, a.dim, g_at);
-                    add_non_finite<T, DP>(dk, ds[j], seen, n, rows, a.dim, q_at);
-                }
+                for (int i = 0; i < 16; ++i) seen |= (n + row_of(i, half) >= beg ? 1u : 0u) << i;
+                add_non_finite<T, DP>(dv, p[j], seen, n, rows, a.dim, g_at);
+                add_non_finite<T, DP>(dk, ds[j], seen, n, rows, a.dim, q_at);
             }
         }
-        return true;
     };
-    if (!pass(std::false_type())) {
+    int n0 = from, turn = 0;
+    auto arrive = [&]() {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (j * NT + threadIdx.x < BN) {
+                sums[turn * 2 * BN + j * NT + threadIdx.x] = rl[j];
+                sums[(turn * 2 + 1) * BN + j * NT + threadIdx.x] = rd[j];
+            }
+        wait_loads();
         __syncthreads();
-        pass(std::true_type());
+        if (n0 + BN < to) {
+            load_sums(n0 + BN);
+            load_tile(n0 + BN, lds + 2 * SLAB * (turn ^ 1));
+        }
+        return lds + 2 * SLAB * turn;
+    };
+    if (from < to) {
+        load_sums(from);
+        load_tile(from, lds);
+    }
+    for (; n0 < to && n0 < beg_whole; n0 += BN, turn ^= 1) {  // causal: the first tiles
+        T* at = arrive();
+        look_over<T, DP, NW, BN, false>(at, &bad, n0 + 1);
+        look_over<T, DP, NW, BN, false>(at + SLAB, &bad, n0 + 1);
+        __syncthreads();
+        const bool mend = bad == n0 + 1;
+        if (n0 + BN > beg_first || (mend))
+            tile(n0, at, at + SLAB, sums + turn * 2 * BN, std::true_type(), mend);
+    }
+    for (; n0 < to; n0 += BN, turn ^= 1) {
+        T* at = arrive();
+        tile(n0, at, at + SLAB, sums + turn * 2 * BN, std::false_type(), false);
     }
     if (!mine) return;
     if (a.splits > 1) {
