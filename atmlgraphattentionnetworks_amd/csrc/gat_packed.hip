@@ -133,15 +133,17 @@ struct Shape {
     static constexpr int DT = (DP + 31) / 32;   // 32-wide tiles of the head dimension
     static constexpr int CPR = DP / N;          // 16-byte vectors of a row
     // A tile of `rows` in LDS, rows without gaps (as the loads to LDS write them).  Vector c
-    // of row r lies at place c ^ turn(r): reads of one vector of 8 rows, and transposing
-    // reads of 4 rows, then meet all banks.  The last tile of the head dimension may read
-    // past DP, into what follows.
+    // of row r lies at place c ^ turn(r), so that what LDS serves in one cycle, 256 bytes,
+    // meets all 64 banks: one vector of 16 rows (the scores' reads), four of 4 rows (the
+    // transposing reads).  With 8-row turns, two rows a bank: 2.6 more cycles a read.  The
+    // last tile of the head dimension may read past DP, into what follows.
     static constexpr int slab(int rows) { return rows * DP; }
     static constexpr int kSlack = 32;
     static __device__ __forceinline__ int turn(int r) {
-        if constexpr (CPR % 8 == 0) return (r & 3) << 1 | (r >> 2 & 1);
-        if constexpr (CPR % 4 == 0) return r >> 1 & 3;
-        return r >> 2 & 1;
+        if constexpr (CPR % 16 == 0) return (r & 3) << 2 | (r >> 2 & 3);
+        if constexpr (CPR % 8 == 0) return (r >> 1 & 1) << 2 | (r >> 2 & 3);
+        if constexpr (CPR % 4 == 0) return r >> 2 & 3;
+        return r >> 3 & 1;
     }
 };
 
@@ -171,9 +173,10 @@ template <int DP>
 __device__ __forceinline__ void add_products(f32x16* acc, const bf16* rows, const f32x16& w) {
     typedef Shape<bf16, DP> S;
     const int lane = threadIdx.x % kWave;
-    const int row = 4 * (lane / 32) + lane % 16 / 4;  // all rows read have row's low three bits
+    const int row = 4 * (lane / 32) + lane % 16 / 4;
     const bf16* at = rows + row * DP + lane % 2 * 4;
-    const int place = (lane % 32 / 16 * 2 + lane % 4 / 2) ^ S::turn(row);
+    const int vec = lane % 32 / 16 * 2 + lane % 4 / 2;
+    const int place_lo = vec ^ S::turn(row), place_hi = vec ^ S::turn(row + 8);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         bf16x8 b;
@@ -181,9 +184,8 @@ __device__ __forceinline__ void add_products(f32x16* acc, const bf16* rows, cons
         for (int e = 0; e < 8; ++e) b[e] = (bf16)w[8 * s + e];
 #pragma unroll
         for (int t = 0; t < S::DT; ++t) {
-            const bf16* x = at + 16 * s * DP + ((4 * t) ^ place) * 8;
-            const bf16x4 lo = read_transposed(x);
-            const bf16x4 hi = read_transposed(x + 8 * DP);
+            const bf16x4 lo = read_transposed(at + 16 * s * DP + ((4 * t) ^ place_lo) * 8);
+            const bf16x4 hi = read_transposed(at + (16 * s + 8) * DP + ((4 * t) ^ place_hi) * 8);
             acc[t] = mma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b, acc[t]);
         }
     }
@@ -195,10 +197,11 @@ __device__ __forceinline__ void add_products(f32x16* acc, const float* rows, con
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int row = 8 * (i / 4) + 4 * half + i % 4;
-        const float* x = rows + row * DP + (d / 4 ^ S::turn(row)) * 4 + d % 4;
+        const float* x = rows + row * DP + d % 4;
+        const int place = d / 4 ^ S::turn(row);
 #pragma unroll
         for (int t = 0; t < S::DT; ++t)
-            acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[32 * t], w[i], acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[((8 * t) ^ place) * 4], w[i], acc[t], 0, 0, 0);
     }
 }
 
@@ -322,10 +325,10 @@ struct Loader {
     typedef Shape<T, DP> S;
     static constexpr int LOADS = (BN * S::CPR + kWave - 1) / kWave;  // of a wave each
     static constexpr int CNT = (LOADS + NW - 1) / NW;
-    // A wave's loads lie STEP rows apart; where that is a multiple of 8 they differ by a
+    // A wave's loads lie STEP rows apart; where that is a multiple of 16 they differ by a
     // scalar only.
     static constexpr int STEP = NW * kWave % S::CPR == 0 ? NW * kWave / S::CPR : 0;
-    static constexpr bool EVEN = CNT == 1 || (STEP > 0 && STEP % 8 == 0);
+    static constexpr bool EVEN = CNT == 1 || (STEP > 0 && STEP % 16 == 0);
     unsigned offset[EVEN ? 1 : CNT];  // of this lane's vectors within a tile
 
     __device__ __forceinline__ void init(long long row_elements, int dim) {
