@@ -11,8 +11,8 @@
 // sees no key gives y = 0, lse = -inf and no gradient.
 //
 // One tile shape carries all three kernels.  A wave owns 32 COLUMNS (queries in the
-// forward and the dq kernel, keys in the dk/dv kernel), one per lane and half wave,
-// and streams ROWS of the other side through LDS, 32 at a time:
+// forward and the dq kernel, keys in the dk/dv kernel; 16 for narrow float32 heads), one per
+// lane and half wave, and streams ROWS of the other side through LDS, 32 at a time:
 //   scores[row][col]  = rows . columns        A: rows from LDS, B: columns in registers
 //   acc[d][col]      += X^T[d][row] W[row][col]     W: the scores after the softmax
 // A 32x32 matrix product leaves lane (col, half) with rows 8 i + 4 half + 0..3, and that
@@ -126,12 +126,26 @@ __device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {
     return c;
 }
 
+// W: columns of a wave.  32 with 32x32 products; 16 with 16x16 ones for narrow float32 heads,
+// where 32-wide tiles of the head dimension would be mostly empty.  The lanes that share a
+// column are its PARTS.  A step covers ROWS rows with 16 scores a lane, register i of part p
+// holding row row_of(i, p); an accumulator's register e holds dimension row_of(e, p) of its
+// tile.
 template <typename T, int DP>
 struct Shape {
     static constexpr int N = Vec16<T>::N;
-    static constexpr int STEPS = DP / (2 * N);  // products of a 32x32 score tile
-    static constexpr int DT = (DP + 31) / 32;   // 32-wide tiles of the head dimension
-    static constexpr int CPR = DP / N;          // 16-byte vectors of a row
+    static constexpr int W = sizeof(T) == 4 && DP <= 16 ? 16 : 32;
+    static constexpr int PARTS = kWave / W, ROWS = 16 * PARTS;
+    static constexpr int STEPS = W == 16 ? 1 : DP / (2 * N);  // products of a score tile
+    static constexpr int DT = W == 16 ? 1 : (DP + 31) / 32;   // tiles of the head dimension
+    static constexpr int CPR = DP / N;                        // 16-byte vectors of a row
+    static constexpr int AR = W == 16 ? 4 : 16;               // registers of an accumulator
+    static constexpr int FN = W == 16 ? DP / 4 : N;           // a lane's dimensions of a step
+    typedef float Acc __attribute__((ext_vector_type(AR)));
+    typedef T Frag __attribute__((ext_vector_type(FN)));
+    static __device__ __forceinline__ int row_of(int i, int part) {
+        return 4 * PARTS * (i / 4) + 4 * part + i % 4;
+    }
     // A tile of `rows` in LDS, rows without gaps (as the loads to LDS write them).  Vector c
     // of row r lies at place c ^ turn(r), so that what LDS serves in one cycle, 256 bytes,
     // meets all 64 banks: one vector of 16 rows (the scores' reads), four of 4 rows (the
@@ -147,17 +161,32 @@ struct Shape {
     }
 };
 
-// scores[row][col] of 32 rows in LDS against the wave's columns
+// scores[row][col] of ROWS rows in LDS against the wave's columns
 template <typename T, int DP>
-__device__ __forceinline__ f32x16 scores(const T* rows, const typename Vec16<T>::type* cols) {
+__device__ __forceinline__ f32x16 scores(const T* rows, const typename Shape<T, DP>::Frag* cols) {
     typedef Shape<T, DP> S;
-    const int lane = threadIdx.x % kWave;
-    const T* at = rows + lane % 32 * DP;
-    const int place = (lane / 32) ^ S::turn(lane % 32);
+    const int lane = threadIdx.x % kWave, row = lane % S::W, part = lane / S::W;
     f32x16 c = {};
+    if constexpr (S::W == 32) {
+        const T* at = rows + row * DP;
+        const int place = part ^ S::turn(row);
 #pragma unroll
-    for (int s = 0; s < S::STEPS; ++s)
-        c = mma(*reinterpret_cast<const typename Vec16<T>::type*>(at + ((2 * s) ^ place) * S::N), cols[s], c);
+        for (int s = 0; s < S::STEPS; ++s)
+            c = mma(*reinterpret_cast<const typename Vec16<T>::type*>(at + ((2 * s) ^ place) * S::N),
+                    cols[s], c);
+    } else {
+        const T* at = rows + row * DP + ((part * S::FN / S::N) ^ S::turn(row)) * S::N + part * S::FN % S::N;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const auto x = *reinterpret_cast<const typename S::Frag*>(at + 16 * u * DP);
+            f32x4 t = {};
+#pragma unroll
+            for (int e = 0; e < S::FN; ++e)
+                t = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], cols[0][e], t, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[4 * u + e] = t[e];
+        }
+    }
     return c;
 }
 
@@ -168,7 +197,7 @@ __device__ __forceinline__ bf16x4 read_transposed(const bf16* p) {
                                           (lds_s16x4*)(__attribute__((address_space(3))) void*)p));
 }
 
-// acc[d][col] += sum over 32 rows of X[row][d] w[row][col]
+// acc[d][col] += sum over ROWS rows of X[row][d] w[row][col]
 template <int DP>
 __device__ __forceinline__ void add_products(f32x16* acc, const bf16* rows, const f32x16& w) {
     typedef Shape<bf16, DP> S;
@@ -191,35 +220,50 @@ __device__ __forceinline__ void add_products(f32x16* acc, const bf16* rows, cons
     }
 }
 template <int DP>
-__device__ __forceinline__ void add_products(f32x16* acc, const float* rows, const f32x16& w) {
+__device__ __forceinline__ void add_products(typename Shape<float, DP>::Acc* acc, const float* rows,
+                                             const f32x16& w) {
     typedef Shape<float, DP> S;
-    const int lane = threadIdx.x % kWave, half = lane / 32, d = lane % 32;
+    const int lane = threadIdx.x % kWave, part = lane / S::W, d = lane % S::W;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const int row = 8 * (i / 4) + 4 * half + i % 4;
+        const int row = S::row_of(i, part);
         const float* x = rows + row * DP + d % 4;
         const int place = d / 4 ^ S::turn(row);
 #pragma unroll
-        for (int t = 0; t < S::DT; ++t)
-            acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[((8 * t) ^ place) * 4], w[i], acc[t], 0, 0, 0);
+        for (int t = 0; t < S::DT; ++t) {
+            const float v = x[((8 * t) ^ place) * 4];
+            if constexpr (S::W == 32)
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, w[i], acc[t], 0, 0, 0);
+            else
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, w[i], acc[t], 0, 0, 0);
+        }
     }
 }
 
-// row within the 32 of register i of a product
-__device__ __forceinline__ int row_of(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
+// over the lanes that share a column
+template <int W>
+__device__ __forceinline__ float parts_sum(float v) {
+    if (W == 16) v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+template <int W>
+__device__ __forceinline__ float parts_max(float v) {
+    if (W == 16) v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
 
-// A column's vectors out of memory: vector s of lane (col, half) holds dimensions
-// (2 s + half) N ...; zeros where `in` is false and beyond `dim`.
+// A column's dimensions out of memory: step s of lane (col, part) holds FN of them from
+// (2 s + part) FN on; zeros where `in` is false and beyond `dim`.
 template <typename T, int DP>
-__device__ __forceinline__ void load_columns(typename Vec16<T>::type* cols, const T* row, int dim,
+__device__ __forceinline__ void load_columns(typename Shape<T, DP>::Frag* cols, const T* row, int dim,
                                              bool in, bool negate) {
     typedef Shape<T, DP> S;
-    const int half = threadIdx.x % kWave / 32;
+    const int part = threadIdx.x % kWave / S::W;
 #pragma unroll
     for (int s = 0; s < S::STEPS; ++s) {
-        typename Vec16<T>::type v = {};
-        const int d = (2 * s + half) * S::N;
-        if (in && d < dim) v = *reinterpret_cast<const typename Vec16<T>::type*>(row + d);
+        typename S::Frag v = {};
+        const int d = (2 * s + part) * S::FN;
+        if (in && d < dim) v = *reinterpret_cast<const typename S::Frag*>(row + d);
         cols[s] = negate ? -v : v;
     }
 }
@@ -256,28 +300,28 @@ __device__ __forceinline__ void look_over(T* lds, int* bad, int tag) {
     if (!CLEAR && any) *bad = tag;
 }
 
-// bit i of `seen`: the column sees row r0 + row_of(i, half)
+// bit i of `seen`: the column sees row r0 + row_of(i, part)
 template <typename T, int DP, typename F>
-__device__ __forceinline__ void add_non_finite(f32x16* acc, f32x16 w, unsigned seen, int r0, int end,
-                                               int dim, F addr) {
-    const int half = threadIdx.x % kWave / 32;
-    const unsigned seen_there = __shfl_xor(seen, 32);
+__device__ __forceinline__ void add_non_finite(typename Shape<T, DP>::Acc* acc, f32x16 w, unsigned seen,
+                                               int r0, int end, int dim, F addr) {
+    typedef Shape<T, DP> S;
+    const int lane = threadIdx.x % kWave, part = lane / S::W;
 #pragma unroll 1
     for (int i = 0; i < 16; ++i) {
-        const float here = w[0], there = __shfl_xor(here, 32);
+        const float here = w[0];
         w = __builtin_shufflevector(w, w, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 0);
 #pragma unroll 1
-        for (int k = 0; k < 2; ++k) {
-            const int row = r0 + row_of(i, k);
-            const unsigned s = k == half ? seen : seen_there;
-            if (row >= end || !((s >> i) & 1)) continue;
-            const float f = k == half ? here : there;
+        for (int k = 0; k < S::PARTS; ++k) {
+            const float f = __shfl(here, lane % S::W + S::W * k);
+            const unsigned sees = __shfl(seen, lane % S::W + S::W * k);
+            const int row = r0 + S::row_of(i, k);
+            if (row >= end || !((sees >> i) & 1)) continue;
             const T* x = addr(row);
 #pragma unroll
-            for (int t = 0; t < (DP + 31) / 32; ++t)
+            for (int t = 0; t < S::DT; ++t)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int d = 32 * t + row_of(e, half);
+                for (int e = 0; e < S::AR; ++e) {
+                    const int d = 32 * t + S::row_of(e, part);
                     const float v = d < dim ? (float)x[d] : 0.f;
                     if (non_finite(v)) acc[t][e] += f * v;
                     // one value at a time: all of them in flight would take the registers
@@ -374,20 +418,22 @@ struct Loader {
     }
 };
 
-// acc[d][col] of one column as a row of T, or as float32 partial sums
-template <typename T, int DP>
-__device__ __forceinline__ void store_column(T* row, const f32x16* acc, float f, int dim) {
-    const int half = threadIdx.x % kWave / 32;
-    typedef T V4 __attribute__((ext_vector_type(4)));
+// acc[d][col] of one column as a row of U: T, or float32 for partial sums
+template <typename T, int DP, typename U>
+__device__ __forceinline__ void store_column(U* row, const typename Shape<T, DP>::Acc* acc, float f,
+                                             int dim) {
+    typedef Shape<T, DP> S;
+    const int part = threadIdx.x % kWave / S::W;
+    typedef U V4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int t = 0; t < (DP + 31) / 32; ++t)
+    for (int t = 0; t < S::DT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = 32 * t + 8 * i + 4 * half;
+        for (int i = 0; i < S::AR / 4; ++i) {
+            const int d = 32 * t + S::row_of(4 * i, part);
             if (d >= dim) continue;
             V4 y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = (T)(acc[t][4 * i + e] * f);
+            for (int e = 0; e < 4; ++e) y[e] = (U)(acc[t][4 * i + e] * f);
             *reinterpret_cast<V4*>(row + d) = y;
         }
 }
@@ -404,8 +450,9 @@ constexpr float kRescale = 8.f;  // log2 of how far p may pass 1 before the sums
 template <typename T, int DP, int NW, int R>
 __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
     typedef Shape<T, DP> S;
-    typedef typename Vec16<T>::type V;
-    constexpr int BM = 32 * NW, BN = 32 * R, SLAB = S::slab(BN);
+    typedef typename S::Frag Frag;
+    typedef typename S::Acc Acc;
+    constexpr int W = S::W, ROWS = S::ROWS, BM = W * NW, BN = ROWS * R, SLAB = S::slab(BN);
     __shared__ __align__(16) T lds[4 * SLAB + S::kSlack];  // keys and values, two tiles of each
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
@@ -417,9 +464,9 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
     const int k0 = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 1);
     int nk = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 2) - k0;
     nk = uniform(nk < 0 ? 0 : nk);
-    const int lane = threadIdx.x % kWave, half = lane / 32;
-    const int r0 = t.index * BM + threadIdx.x / kWave * 32;
-    const int r = r0 + lane % 32;
+    const int lane = threadIdx.x % kWave, part = lane / W;
+    const int r0 = t.index * BM + threadIdx.x / kWave * W;
+    const int r = r0 + lane % W;
     // the keys that a row sees: [0, limit)
     auto limit = [&](int row) {
         if (!a.causal) return nk;
@@ -432,7 +479,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
     const int head = kh * a.group + gi;
     const int lim = limit(rc);
     const int lim_first = uniform(limit(r0 < rows ? r0 : rows - 1));  // the wave's smallest
-    const int lim_last = uniform(r0 < rows ? limit(r0 + 31 < rows ? r0 + 31 : rows - 1) : 0);
+    const int lim_last = uniform(r0 < rows ? limit(r0 + W - 1 < rows ? r0 + W - 1 : rows - 1) : 0);
     const int last = t.index * BM + BM - 1;
     const int lim_block = uniform(limit(last < rows ? last : rows - 1));
     const int lim_whole = uniform(limit(t.index * BM));  // keys that all rows see
@@ -443,7 +490,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
         to = from + per < lim_block ? from + per : lim_block;
     }
 
-    V qc[S::STEPS];
+    Frag qc[S::STEPS];
     load_columns<T, DP>(qc,
                         static_cast<const T*>(a.q.p) + (long long)(t.first + qi) * a.q.row +
                             (long long)head * a.q.head,
@@ -460,7 +507,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
         kl.load(kb + (long long)n0 * a.k.row, (int)a.k.row, nk - n0, a.dim, to_lds);
         vl.load(vb + (long long)n0 * a.v.row, (int)a.v.row, nk - n0, a.dim, to_lds + SLAB);
     };
-    f32x16 acc[S::DT] = {};
+    Acc acc[S::DT] = {};
     float m = -INFINITY, l = 0.f;
     // One tile.  MASK: some column may not see all of its rows; mend: and a hidden one may
     // hold an infinity or NaN.
@@ -470,16 +517,16 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
+            s[j] = scores<T, DP>(lk + S::slab(ROWS * j), qc);
             if (MASK) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = -INFINITY;
+                    if (n0 + ROWS * j + S::row_of(i, part) >= lim) s[j][i] = -INFINITY;
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[j][i]);
         }
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        mx = parts_max<W>(mx);
         if (__any((mx - m) * c > kRescale)) {  // -inf - -inf: false
             const float to_m = fmaxf(m, mx);
             const float f = m == -INFINITY ? 0.f : exp2f((m - to_m) * c);
@@ -496,13 +543,13 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
                 s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -mc));
                 l += s[j][i];
             }
-            add_products<DP>(acc, lv + S::slab(32 * j), s[j]);
+            add_products<DP>(acc, lv + S::slab(ROWS * j), s[j]);
             if (MASK && mend) {
                 unsigned seen = 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
-                add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, v_at);
+                    seen |= (n0 + ROWS * j + S::row_of(i, part) < lim ? 1u : 0u) << i;
+                add_non_finite<T, DP>(acc, s[j], seen, n0 + ROWS * j, nk, a.dim, v_at);
             }
         }
     };
@@ -533,14 +580,14 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
         }
         if (n0 < lim_last) tile(n0, at, at + SLAB, std::true_type(), mend);
     }
-    l += __shfl_xor(l, 32);
+    l = parts_sum<W>(l);
     if (!mine) return;
     const long long qh = (long long)(t.first + qi) * a.kv_heads * a.group + head;
     if (a.splits > 1) {
         const long long at = (long long)blockIdx.z * a.nq * a.kv_heads * a.group + qh;
-        store_column<float, DP>(a.part + at * a.dim, acc, 1.f, a.dim);
+        store_column<T, DP>(a.part + at * a.dim, acc, 1.f, a.dim);
         float* ml = a.part + (long long)a.splits * a.nq * a.kv_heads * a.group * a.dim;
-        if (half == 0) {
+        if (part == 0) {
             ml[2 * at] = m;
             ml[2 * at + 1] = lim == 0 && blockIdx.z == 0 ? 1.f : l;  // no key: 0 / 1, not 0 / 0
         }
@@ -550,7 +597,7 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
              (long long)head * a.o.head;
     if (lim == 0) {  // sees no key
 #pragma unroll
-        for (int d = 0; d < S::DT; ++d) acc[d] = f32x16{};
+        for (int d = 0; d < S::DT; ++d) acc[d] = Acc{};
         l = 1.f;
     }
     store_column<T, DP>(out, acc, 1.f / l, a.dim);
@@ -560,14 +607,14 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
 #pragma unroll
             for (int d = 0; d < S::DT; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < S::AR; ++i) {
                     const float y = acc[d][i] * f;
                     acc[d][i] = y - (float)(T)y;
                 }
             store_column<T, DP>(static_cast<T*>(a.low) + qh * a.dim, acc, 1.f, a.dim);
         }
     }
-    if (a.lse != nullptr && half == 0)
+    if (a.lse != nullptr && part == 0)
         a.lse[qh] = lim == 0 ? -INFINITY : m * score_scale(a.scale) + logf(l);
 }
 
@@ -624,8 +671,9 @@ __global__ __launch_bounds__(256) void k_attn_sum(const float* part, int splits,
 template <typename T, int DP, int NW, int R>
 __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnArgs a) {
     typedef Shape<T, DP> S;
-    typedef typename Vec16<T>::type V;
-    constexpr int BM = 32 * NW, BN = 32 * R, SLAB = S::slab(BN);
+    typedef typename S::Frag Frag;
+    typedef typename S::Acc Acc;
+    constexpr int W = S::W, ROWS = S::ROWS, BM = W * NW, BN = ROWS * R, SLAB = S::slab(BN);
     __shared__ __align__(16) T lds[4 * SLAB + S::kSlack];
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
@@ -637,9 +685,9 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
     const int k0 = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 1);
     int nk = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 2) - k0;
     nk = uniform(nk < 0 ? 0 : nk);
-    const int lane = threadIdx.x % kWave, half = lane / 32;
-    const int r0 = t.index * BM + threadIdx.x / kWave * 32;
-    const int r = r0 + lane % 32;
+    const int lane = threadIdx.x % kWave, part = lane / W;
+    const int r0 = t.index * BM + threadIdx.x / kWave * W;
+    const int r = r0 + lane % W;
     // the keys that a row sees: [0, limit)
     auto limit = [&](int row) {
         if (!a.causal) return nk;
@@ -652,7 +700,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
     const int head = kh * a.group + gi;
     const int lim = limit(rc);
     const int lim_first = uniform(limit(r0 < rows ? r0 : rows - 1));  // the wave's smallest
-    const int lim_last = uniform(r0 < rows ? limit(r0 + 31 < rows ? r0 + 31 : rows - 1) : 0);
+    const int lim_last = uniform(r0 < rows ? limit(r0 + W - 1 < rows ? r0 + W - 1 : rows - 1) : 0);
     const int last = t.index * BM + BM - 1;
     const int lim_block = uniform(limit(last < rows ? last : rows - 1));
     const int lim_whole = uniform(limit(t.index * BM));  // keys that all rows see
@@ -663,7 +711,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
         to = from + per < lim_block ? from + per : lim_block;
     }
 
-    V qc[S::STEPS], gc[S::STEPS];
+    Frag qc[S::STEPS], gc[S::STEPS];
     const long long tok = t.first + qi;
     const long long qh = tok * a.kv_heads * a.group + head;
     load_columns<T, DP>(qc, static_cast<const T*>(a.q.p) + tok * a.q.row + (long long)head * a.q.head,
@@ -675,17 +723,17 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
     // dq's norm against 2.3e-3 to 2.45e-3)
     float delta = 0.f;
     auto add_delta = [&](const T* from_row) {
-        V oc[S::STEPS];
+        Frag oc[S::STEPS];
         load_columns<T, DP>(oc, from_row, a.dim, mine, false);
 #pragma unroll
         for (int s = 0; s < S::STEPS; ++s)
 #pragma unroll
-            for (int e = 0; e < S::N; ++e) delta = fmaf((float)gc[s][e], (float)oc[s][e], delta);
+            for (int e = 0; e < S::FN; ++e) delta = fmaf((float)gc[s][e], (float)oc[s][e], delta);
     };
     if (sizeof(T) == 2 && a.low != nullptr) add_delta(static_cast<const T*>(a.low) + qh * a.dim);
     add_delta(static_cast<const T*>(a.o.p) + tok * a.o.row + (long long)head * a.o.head);
-    delta += __shfl_xor(delta, 32);
-    if (mine && half == 0 && blockIdx.z == 0) a.delta[qh] = delta;
+    delta = parts_sum<W>(delta);
+    if (mine && part == 0 && blockIdx.z == 0) a.delta[qh] = delta;
     const float lse2 = mine ? a.lse[qh] * kLog2e : 0.f;
     const T* kb = static_cast<const T*>(a.k.p) + (long long)k0 * a.k.row + (long long)kh * a.k.head;
     const T* vb = static_cast<const T*>(a.v.p) + (long long)k0 * a.v.row + (long long)kh * a.v.head;
@@ -699,14 +747,14 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
         kl.load(kb + (long long)n0 * a.k.row, (int)a.k.row, nk - n0, a.dim, to_lds);
         vl.load(vb + (long long)n0 * a.v.row, (int)a.v.row, nk - n0, a.dim, to_lds + SLAB);
     };
-    f32x16 acc[S::DT] = {};
+    Acc acc[S::DT] = {};
     auto tile = [&](int n0, T* lk, const T* lv, auto masks, bool mend) {
         constexpr bool MASK = decltype(masks)::value;
         f32x16 s[R], dp[R];
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            s[j] = scores<T, DP>(lk + S::slab(32 * j), qc);
-            dp[j] = scores<T, DP>(lv + S::slab(32 * j), gc);
+            s[j] = scores<T, DP>(lk + S::slab(ROWS * j), qc);
+            dp[j] = scores<T, DP>(lv + S::slab(ROWS * j), gc);
         }
 #pragma unroll
         for (int j = 0; j < R; ++j) {
@@ -714,7 +762,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
             for (int i = 0; i < 16; ++i) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -lse2));
                 s[j][i] = p * (dp[j][i] - delta);
-                if (MASK && n0 + 32 * j + row_of(i, half) >= lim) s[j][i] = 0.f;
+                if (MASK && n0 + ROWS * j + S::row_of(i, part) >= lim) s[j][i] = 0.f;
             }
         }
         if (MASK && mend) {  // the scores need the keys as they are, the product needs them cleared
@@ -724,13 +772,13 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
         }
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            add_products<DP>(acc, lk + S::slab(32 * j), s[j]);
+            add_products<DP>(acc, lk + S::slab(ROWS * j), s[j]);
             if (MASK && mend) {
                 unsigned seen = 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    seen |= (n0 + 32 * j + row_of(i, half) < lim ? 1u : 0u) << i;
-                add_non_finite<T, DP>(acc, s[j], seen, n0 + 32 * j, nk, a.dim, k_at);
+                    seen |= (n0 + ROWS * j + S::row_of(i, part) < lim ? 1u : 0u) << i;
+                add_non_finite<T, DP>(acc, s[j], seen, n0 + ROWS * j, nk, a.dim, k_at);
             }
         }
     };
@@ -755,12 +803,12 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
             __syncthreads();
             mend = bad == n0 + 1;
         }
-        if (n0 < lim_last || (mend)) tile(n0, at, at + SLAB, std::true_type(), mend);
+        if (n0 < lim_last || mend) tile(n0, at, at + SLAB, std::true_type(), mend);
     }
     if (!mine) return;
     if (a.splits > 1) {
         const long long at = (long long)blockIdx.z * a.nq * a.kv_heads * a.group + qh;
-        store_column<float, DP>(a.part + at * a.dim, acc, 1.f, a.dim);
+        store_column<T, DP>(a.part + at * a.dim, acc, 1.f, a.dim);
         return;
     }
     store_column<T, DP>(static_cast<T*>(const_cast<void*>(a.dq.p)) + tok * a.dq.row +
@@ -774,8 +822,9 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
 template <typename T, int DP, int NW, int R>
 __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
     typedef Shape<T, DP> S;
-    typedef typename Vec16<T>::type V;
-    constexpr int BM = 32 * NW, BN = 32 * R, SLAB = S::slab(BN);
+    typedef typename S::Frag Frag;
+    typedef typename S::Acc Acc;
+    constexpr int W = S::W, ROWS = S::ROWS, BM = W * NW, BN = ROWS * R, SLAB = S::slab(BN);
     __shared__ __align__(16) T lds[4 * SLAB + S::kSlack];  // q and g, two tiles of each
     __shared__ __align__(16) float sums[2 * 2 * BN];               // lse and delta of their rows
     __shared__ int bad;
@@ -787,9 +836,9 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
     int nq = t.seq < 0 ? 0 : bound_at(a.ptr, a.ptr64, a.count, a.nq, t.seq + 2) - q0;
     if (nq < 0) nq = 0;
     const int rows = uniform(nq * a.group);
-    const int lane = threadIdx.x % kWave, half = lane / 32;
-    const int c0 = t.index * BM + threadIdx.x / kWave * 32;
-    const int key = c0 + lane % 32;
+    const int lane = threadIdx.x % kWave, part = lane / W;
+    const int c0 = t.index * BM + threadIdx.x / kWave * W;
+    const int key = c0 + lane % W;
     const bool mine = key < t.len;
     const int kc = mine ? key : t.len - 1;
     // the rows that see a key: [start, rows)
@@ -809,7 +858,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
         to = from + per < rows ? from + per : rows;
     }
 
-    V kcol[S::STEPS], vcol[S::STEPS];
+    Frag kcol[S::STEPS], vcol[S::STEPS];
     const long long tok = t.first + kc;
     load_columns<T, DP>(kcol, static_cast<const T*>(a.k.p) + tok * a.k.row + (long long)kh * a.k.head,
                         a.dim, mine && a.scale != 0.f, a.scale < 0.f);
@@ -850,27 +899,27 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
         ld.load_packed(a, qb, a.q, n0, rows, to_lds);
         ld.load_packed(a, gb, a.g, n0, rows, to_lds + SLAB);
     };
-    f32x16 dk[S::DT] = {}, dv[S::DT] = {};
+    Acc dk[S::DT] = {}, dv[S::DT] = {};
     auto tile = [&](int n0, T* lq, T* lg, const float* ll, auto masks, bool mend) {
         constexpr bool MASK = decltype(masks)::value;
         f32x16 p[R], ds[R];
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            p[j] = scores<T, DP>(lq + S::slab(32 * j), kcol);
-            ds[j] = scores<T, DP>(lg + S::slab(32 * j), vcol);
+            p[j] = scores<T, DP>(lq + S::slab(ROWS * j), kcol);
+            ds[j] = scores<T, DP>(lg + S::slab(ROWS * j), vcol);
         }
 #pragma unroll
         for (int j = 0; j < R; ++j)
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(ll + 32 * j + 8 * b + 4 * half);
-                const f32x4 d4 = *reinterpret_cast<const f32x4*>(ll + BN + 32 * j + 8 * b + 4 * half);
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(ll + ROWS * j + S::row_of(4 * b, part));
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(ll + BN + ROWS * j + S::row_of(4 * b, part));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = 4 * b + e;
                     p[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j][i], c, -l4[e]));
                     ds[j][i] = p[j][i] * (ds[j][i] - d4[e]);
-                    if (MASK && n0 + 32 * j + row_of(i, half) < beg) p[j][i] = ds[j][i] = 0.f;
+                    if (MASK && n0 + ROWS * j + S::row_of(i, part) < beg) p[j][i] = ds[j][i] = 0.f;
                 }
             }
         if (MASK && mend) {
@@ -881,13 +930,13 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
         }
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            add_products<DP>(dv, lg + S::slab(32 * j), p[j]);
-            add_products<DP>(dk, lq + S::slab(32 * j), ds[j]);
+            add_products<DP>(dv, lg + S::slab(ROWS * j), p[j]);
+            add_products<DP>(dk, lq + S::slab(ROWS * j), ds[j]);
             if (MASK && mend) {
-                const int n = n0 + 32 * j;
+                const int n = n0 + ROWS * j;
                 unsigned seen = 0;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) seen |= (n + row_of(i, half) >= beg ? 1u : 0u) << i;
+                for (int i = 0; i < 16; ++i) seen |= (n + S::row_of(i, part) >= beg ? 1u : 0u) << i;
                 add_non_finite<T, DP>(dv, p[j], seen, n, rows, a.dim, g_at);
                 add_non_finite<T, DP>(dk, ds[j], seen, n, rows, a.dim, q_at);
             }
@@ -919,7 +968,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
         look_over<T, DP, NW, BN, false>(at + SLAB, &bad, n0 + 1);
         __syncthreads();
         const bool mend = bad == n0 + 1;
-        if (n0 + BN > beg_first || (mend))
+        if (n0 + BN > beg_first || mend)
             tile(n0, at, at + SLAB, sums + turn * 2 * BN, std::true_type(), mend);
     }
     for (; n0 < to; n0 += BN, turn ^= 1) {
@@ -930,8 +979,8 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
     if (a.splits > 1) {
         const long long n = (long long)a.nk * a.kv_heads;
         const long long at = (long long)blockIdx.z * n + tok * a.kv_heads + kh;
-        store_column<float, DP>(a.part + at * a.dim, dk, 1.f, a.dim);
-        store_column<float, DP>(a.part + (a.splits * n + at) * a.dim, dv, 1.f, a.dim);
+        store_column<T, DP>(a.part + at * a.dim, dk, 1.f, a.dim);
+        store_column<T, DP>(a.part + (a.splits * n + at) * a.dim, dv, 1.f, a.dim);
         return;
     }
     store_column<T, DP>(static_cast<T*>(const_cast<void*>(a.dk.p)) + tok * a.dk.row +
@@ -950,16 +999,19 @@ struct Plan {
     int waves, splits;
 };
 
-// cols: rows of the axis whose tiles the grid walks; streamed: the other's.
-inline Plan plan_of(long long cols, long long streamed, int count, int kv_heads) {
+// The columns of a wave (Shape::W) for these heads.
+inline int wave_columns(int dim, int dtype) { return dtype == GAT_F32 && dim <= 16 ? 16 : 32; }
+
+// cols: rows of the axis whose tiles the grid walks; streamed: the other's; w: wave_columns.
+inline Plan plan_of(long long cols, long long streamed, int count, int kv_heads, int w) {
     const int n = count > 0 ? count : 1;
     auto tiles = [&](int waves) {
-        return std::max<long long>(n, (cols + 32 * waves - 1) / (32 * waves)) * kv_heads;
+        return std::max<long long>(n, (cols + w * waves - 1) / (w * waves)) * kv_heads;
     };
     Plan p;
     // A workgroup shares its row tiles between its waves; short sequences fill one or two,
     // and fewer than 4 workgroups a CU leave CUs idle behind the longest.
-    p.waves = cols <= 32ll * n ? 1 : cols <= 64ll * n || tiles(4) < 4 * 256 ? 2 : 4;
+    p.waves = cols <= (long long)w * n ? 1 : cols <= 2ll * w * n || tiles(4) < 4 * 256 ? 2 : 4;
     // Fewer waves than 3 a SIMD: the streamed axis is split, into 256 rows or more each.
     const long long waves = tiles(p.waves) * p.waves;
     const long long want = (3ll * 4 * 256 + waves - 1) / waves;
@@ -972,12 +1024,14 @@ struct AttnSizes {
     size_t fwd_bytes, delta_bytes, dq_bytes, dkv_bytes;
 };
 
-inline AttnSizes attn_sizes(long long nq, long long nk, int count, int heads, int kv_heads, int dim) {
+inline AttnSizes attn_sizes(long long nq, long long nk, int count, int heads, int kv_heads, int dim,
+                            int dtype) {
     AttnSizes s;
     const int group = heads / kv_heads;
-    s.fwd = plan_of(nq * group, nk, count, kv_heads);
+    const int w = wave_columns(dim, dtype);
+    s.fwd = plan_of(nq * group, nk, count, kv_heads, w);
     s.dq = s.fwd;
-    s.dkv = plan_of(nk, nq * group, count, kv_heads);
+    s.dkv = plan_of(nk, nq * group, count, kv_heads, w);
     const size_t q = (size_t)nq * heads, k = (size_t)nk * kv_heads;
     s.fwd_bytes = s.fwd.splits > 1 ? s.fwd.splits * q * (dim + 2) * sizeof(float) : 0;
     s.delta_bytes = align_up(q * sizeof(float));
@@ -1018,10 +1072,11 @@ enum AttnPass { kFwd, kDq, kDkv };
 template <typename T, int DP, AttnPass PASS>
 int attn_launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
     const bool keys = PASS == kDkv;
-    const long long slots = slots_of(keys ? a.nk : a.nq, keys ? 1 : a.group, 32 * p.waves, a.count);
+    const long long slots = slots_of(keys ? a.nk : a.nq, keys ? 1 : a.group, Shape<T, DP>::W * p.waves, a.count);
     const dim3 grid((unsigned)slots, a.kv_heads, p.splits);
-    // 32-row tiles a step: two where the registers allow it (their chains interleave)
-    constexpr int R = sizeof(T) == 4 ? 1 : PASS == kFwd ? 2 : DP <= 64 ? 2 : 1;
+    // row tiles a step: two where the registers allow it (their chains interleave)
+    constexpr int W = Shape<T, DP>::W;
+    constexpr int R = W == 16 ? (PASS == kDkv ? 1 : 2) : sizeof(T) == 4 ? 1 : PASS == kFwd || DP <= 64 ? 2 : 1;
     auto call = [&](auto waves) {
         constexpr int NW = decltype(waves)::value;
         if constexpr (PASS == kFwd) k_attn_fwd<T, DP, NW, NW == 4 ? R : 1><<<grid, 64 * NW, 0, s>>>(a);
@@ -1073,7 +1128,7 @@ int gat_packed_attention_workspace_size(int nq, int nk, int count, int heads, in
     const int rc = attn_check(nq, nk, count, heads, kv_heads, dim, dtype);
     if (rc != GAT_OK) return rc;
     if (bytes == nullptr) return GAT_EINVAL;
-    *bytes = attn_sizes(nq, nk, count, heads, kv_heads, dim).fwd_bytes;
+    *bytes = attn_sizes(nq, nk, count, heads, kv_heads, dim, dtype).fwd_bytes;
     return GAT_OK;
 }
 
@@ -1096,7 +1151,7 @@ int gat_packed_attention(const void* q, long long q_row, long long q_head, const
         return GAT_EINVAL;
     for (const Rows* r : {&a.q, &a.k, &a.v, &a.o})
         if (!vec_rows(*r, dim, heads / kv_heads, dtype)) return GAT_EUNSUPPORTED;
-    const AttnSizes sz = attn_sizes(nq, nk, count, heads, kv_heads, dim);
+    const AttnSizes sz = attn_sizes(nq, nk, count, heads, kv_heads, dim, dtype);
     if (sz.fwd_bytes > 0 && (workspace == nullptr || workspace_bytes < sz.fwd_bytes))
         return GAT_EWORKSPACE;
     if (((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(low)) & 15) != 0)
@@ -1132,7 +1187,7 @@ int gat_packed_attention_backward_workspace_size(int nq, int nk, int count, int 
     const int rc = attn_check(nq, nk, count, heads, kv_heads, dim, dtype);
     if (rc != GAT_OK) return rc;
     if (bytes == nullptr) return GAT_EINVAL;
-    const AttnSizes s = attn_sizes(nq, nk, count, heads, kv_heads, dim);
+    const AttnSizes s = attn_sizes(nq, nk, count, heads, kv_heads, dim, dtype);
     *bytes = s.delta_bytes + std::max(s.dq_bytes, s.dkv_bytes);  // dq is done before dk and dv begin
     return GAT_OK;
 }
@@ -1162,7 +1217,7 @@ int gat_packed_attention_backward(const void* g, long long g_row, long long g_he
         return GAT_EINVAL;
     for (const Rows* r : {&a.g, &a.q, &a.k, &a.v, &a.o, &a.dq, &a.dk, &a.dv})
         if (!vec_rows(*r, dim, heads / kv_heads, dtype)) return GAT_EUNSUPPORTED;
-    const AttnSizes sz = attn_sizes(nq, nk, count, heads, kv_heads, dim);
+    const AttnSizes sz = attn_sizes(nq, nk, count, heads, kv_heads, dim, dtype);
     if (workspace_bytes < sz.delta_bytes + std::max(sz.dq_bytes, sz.dkv_bytes) ||
         (workspace == nullptr && workspace_bytes > 0))
         return GAT_EWORKSPACE;
