@@ -79,16 +79,17 @@ __device__ __forceinline__ int bound_at(const void* ptr, int ptr64, int count, i
     return (int)(v < 0 ? 0 : v > n ? n : v);
 }
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 struct Tile {
-    int seq;    // as the caller counts, or -1 outside the sequences
-    int first;  // the sequence's first row, and its rows
-    int len;
-    int index;  // tile within the sequence
+    int first, len;              // the sequence's rows on the tile's axis
+    int other_first, other_len;  // and on the other; none outside the caller's sequences
+    int index;                   // tile within the sequence
 };
 
-// The sequence and the tile of a slot; 64 boundaries a step.
-__device__ __forceinline__ Tile tile_of(const void* ptr, int ptr64, int count, int n, int group,
-                                        int size, int slot) {
+// The sequence and the tile of a slot; 64 boundaries a step, then the four that count at once.
+__device__ __forceinline__ Tile tile_of(const void* ptr, const void* other, int ptr64, int count, int n,
+                                        int other_n, int group, int size, int slot) {
     const int lane = threadIdx.x % kWave;
     int lo = 0, hi = count + 2;
     while (hi - lo > 1) {
@@ -101,12 +102,16 @@ __device__ __forceinline__ Tile tile_of(const void* ptr, int ptr64, int count, i
         lo += (got > 0 ? got - 1 : 0) * step;
         if (lo + step < hi) hi = lo + step;
     }
+    const bool ours = lo >= 1 && lo <= count;
+    const int a = bound_at(ptr, ptr64, count, n, lo), b = bound_at(ptr, ptr64, count, n, lo + 1);
+    const int c = ours ? bound_at(other, ptr64, count, other_n, lo) : 0;
+    const int d = ours ? bound_at(other, ptr64, count, other_n, lo + 1) : 0;
     Tile t;
-    t.first = bound_at(ptr, ptr64, count, n, lo);
-    t.len = bound_at(ptr, ptr64, count, n, lo + 1) - t.first;
-    if (t.len < 0) t.len = 0;
-    t.index = slot - (int)((long long)t.first * group / size + lo);
-    t.seq = lo >= 1 && lo <= count ? lo - 1 : -1;
+    t.first = uniform(a);
+    t.len = uniform(b > a ? b - a : 0);
+    t.other_first = uniform(c);
+    t.other_len = uniform(d > c ? d - c : 0);
+    t.index = uniform(slot - (int)((long long)a * group / size + lo));
     return t;
 }
 
@@ -348,8 +353,6 @@ __device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned offset, int s
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
 __device__ __forceinline__ i32x4 make_buffer(const void* p, unsigned bytes) {
     const unsigned long long a = reinterpret_cast<unsigned long long>(p);
     i32x4 b;
@@ -457,13 +460,12 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
     // later tiles of a causal sequence take longer: they go first
-    const Tile t = tile_of(a.ptr, a.ptr64, a.count, a.nq, a.group, BM, gridDim.x - 1 - blockIdx.x);
+    const Tile t = tile_of(a.ptr, a.kv_ptr, a.ptr64, a.count, a.nq, a.nk, a.group, BM,
+                           gridDim.x - 1 - blockIdx.x);
     const int rows = t.len * a.group;
     if (t.index < 0 || (long long)t.index * BM >= rows) return;
     const int kh = blockIdx.y;
-    const int k0 = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 1);
-    int nk = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 2) - k0;
-    nk = uniform(nk < 0 ? 0 : nk);
+    const int k0 = t.other_first, nk = t.other_len;
     const int lane = threadIdx.x % kWave, part = lane / W;
     const int r0 = t.index * BM + threadIdx.x / kWave * W;
     const int r = r0 + lane % W;
@@ -518,10 +520,11 @@ __global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             s[j] = scores<T, DP>(lk + S::slab(ROWS * j), qc);
-            if (MASK) {
+            if (MASK) {  // row_of(i, part) = row_of(i, 0) + 4 part: constants on one side
+                const int left = lim - n0 - 4 * part;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (n0 + ROWS * j + S::row_of(i, part) >= lim) s[j][i] = -INFINITY;
+                    if (ROWS * j + S::row_of(i, 0) >= left) s[j][i] = -INFINITY;
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[j][i]);
@@ -678,13 +681,12 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
     // later tiles of a causal sequence take longer: they go first
-    const Tile t = tile_of(a.ptr, a.ptr64, a.count, a.nq, a.group, BM, gridDim.x - 1 - blockIdx.x);
+    const Tile t = tile_of(a.ptr, a.kv_ptr, a.ptr64, a.count, a.nq, a.nk, a.group, BM,
+                           gridDim.x - 1 - blockIdx.x);
     const int rows = t.len * a.group;
     if (t.index < 0 || (long long)t.index * BM >= rows) return;
     const int kh = blockIdx.y;
-    const int k0 = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 1);
-    int nk = t.seq < 0 ? 0 : bound_at(a.kv_ptr, a.ptr64, a.count, a.nk, t.seq + 2) - k0;
-    nk = uniform(nk < 0 ? 0 : nk);
+    const int k0 = t.other_first, nk = t.other_len;
     const int lane = threadIdx.x % kWave, part = lane / W;
     const int r0 = t.index * BM + threadIdx.x / kWave * W;
     const int r = r0 + lane % W;
@@ -751,6 +753,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
     auto tile = [&](int n0, T* lk, const T* lv, auto masks, bool mend) {
         constexpr bool MASK = decltype(masks)::value;
         f32x16 s[R], dp[R];
+        const int left = lim - n0 - 4 * part;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             s[j] = scores<T, DP>(lk + S::slab(ROWS * j), qc);
@@ -762,7 +765,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
             for (int i = 0; i < 16; ++i) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -lse2));
                 s[j][i] = p * (dp[j][i] - delta);
-                if (MASK && n0 + ROWS * j + S::row_of(i, part) >= lim) s[j][i] = 0.f;
+                if (MASK && ROWS * j + S::row_of(i, 0) >= left) s[j][i] = 0.f;
             }
         }
         if (MASK && mend) {  // the scores need the keys as they are, the product needs them cleared
@@ -829,13 +832,11 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
     __shared__ __align__(16) float sums[2 * 2 * BN];               // lse and delta of their rows
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
-    const Tile t = tile_of(a.kv_ptr, a.ptr64, a.count, a.nk, 1, BM, blockIdx.x);
+    const Tile t = tile_of(a.kv_ptr, a.ptr, a.ptr64, a.count, a.nk, a.nq, 1, BM, blockIdx.x);
     if (t.index < 0 || (long long)t.index * BM >= t.len) return;
     const int kh = blockIdx.y;
-    const int q0 = t.seq < 0 ? 0 : bound_at(a.ptr, a.ptr64, a.count, a.nq, t.seq + 1);
-    int nq = t.seq < 0 ? 0 : bound_at(a.ptr, a.ptr64, a.count, a.nq, t.seq + 2) - q0;
-    if (nq < 0) nq = 0;
-    const int rows = uniform(nq * a.group);
+    const int q0 = t.other_first, nq = t.other_len;
+    const int rows = nq * a.group;
     const int lane = threadIdx.x % kWave, part = lane / W;
     const int c0 = t.index * BM + threadIdx.x / kWave * W;
     const int key = c0 + lane % W;
@@ -903,6 +904,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
     auto tile = [&](int n0, T* lq, T* lg, const float* ll, auto masks, bool mend) {
         constexpr bool MASK = decltype(masks)::value;
         f32x16 p[R], ds[R];
+        const int hidden = beg - n0 - 4 * part;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             p[j] = scores<T, DP>(lq + S::slab(ROWS * j), kcol);
@@ -919,7 +921,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnA
                     const int i = 4 * b + e;
                     p[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j][i], c, -l4[e]));
                     ds[j][i] = p[j][i] * (ds[j][i] - d4[e]);
-                    if (MASK && n0 + ROWS * j + S::row_of(i, part) < beg) p[j][i] = ds[j][i] = 0.f;
+                    if (MASK && ROWS * j + S::row_of(i, 0) < hidden) p[j][i] = ds[j][i] = 0.f;
                 }
             }
         if (MASK && mend) {
@@ -1075,8 +1077,7 @@ int attn_launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
     const long long slots = slots_of(keys ? a.nk : a.nq, keys ? 1 : a.group, Shape<T, DP>::W * p.waves, a.count);
     const dim3 grid((unsigned)slots, a.kv_heads, p.splits);
     // row tiles a step: two where the registers allow it (their chains interleave)
-    constexpr int W = Shape<T, DP>::W;
-    constexpr int R = W == 16 ? (PASS == kDkv ? 1 : 2) : sizeof(T) == 4 ? 1 : PASS == kFwd || DP <= 64 ? 2 : 1;
+    constexpr int R = sizeof(T) == 4 ? 1 : PASS == kFwd || DP <= 64 ? 2 : 1;
     auto call = [&](auto waves) {
         constexpr int NW = decltype(waves)::value;
         if constexpr (PASS == kFwd) k_attn_fwd<T, DP, NW, NW == 4 ? R : 1><<<grid, 64 * NW, 0, s>>>(a);
