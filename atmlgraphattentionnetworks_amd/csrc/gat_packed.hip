@@ -166,6 +166,18 @@ struct Shape {
     }
 };
 
+enum AttnPass { kFwd, kDq, kDkv };
+
+// What the registers are held to: two waves a SIMD to have one's softmax under the other's
+// matrix products, as many as fit where the tiles are narrow and waiting is most of the time
+// (graphs of 85 to 150 nodes, 8 heads of 8, float32, one training step: 300 us with what the
+// compiler takes, 278 us with these); wide heads' backward needs the registers of one.
+template <typename T, int DP>
+constexpr int waves_per_simd(AttnPass pass) {
+    if (Shape<T, DP>::W == 16) return pass == kDkv ? 4 : 6;
+    return pass == kFwd || DP <= 64 ? 2 : 1;
+}
+
 // scores[row][col] of ROWS rows in LDS against the wave's columns
 template <typename T, int DP>
 __device__ __forceinline__ f32x16 scores(const T* rows, const typename Shape<T, DP>::Frag* cols) {
@@ -451,7 +463,7 @@ constexpr float kRescale = 8.f;  // log2 of how far p may pass 1 before the sums
 // product, the sum l uses the unrounded p.
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int NW, int R>
-__global__ __launch_bounds__(NW * kWave, 2) void k_attn_fwd(AttnArgs a) {
+__global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kFwd))) void k_attn_fwd(AttnArgs a) {
     typedef Shape<T, DP> S;
     typedef typename S::Frag Frag;
     typedef typename S::Acc Acc;
@@ -672,7 +684,7 @@ __global__ __launch_bounds__(256) void k_attn_sum(const float* part, int splits,
 // left for the dk/dv kernel.
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int NW, int R>
-__global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnArgs a) {
+__global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDq))) void k_attn_dq(AttnArgs a) {
     typedef Shape<T, DP> S;
     typedef typename S::Frag Frag;
     typedef typename S::Acc Acc;
@@ -823,7 +835,7 @@ __global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dq(AttnAr
 // dk, dv: columns = keys, rows = (query, head of the group).
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int NW, int R>
-__global__ __launch_bounds__(NW * kWave, DP <= 64 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
+__global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_attn_dkv(AttnArgs a) {
     typedef Shape<T, DP> S;
     typedef typename S::Frag Frag;
     typedef typename S::Acc Acc;
@@ -1068,8 +1080,6 @@ inline void set_group(AttnArgs& a, int group) {
     a.div_shift = s;
     a.div_mul = group == 1 ? 0 : (unsigned)(((1ull << (32 + s)) + group - 1) / group);
 }
-
-enum AttnPass { kFwd, kDq, kDkv };
 
 template <typename T, int DP, AttnPass PASS>
 int attn_launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
