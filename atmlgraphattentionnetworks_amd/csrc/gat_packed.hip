@@ -198,11 +198,13 @@ enum AttnPass { kFwd, kDq, kDkv };
 // What the registers are held to: two waves a SIMD to have one's softmax under the other's
 // matrix products, as many as fit where the tiles are narrow and waiting is most of the time
 // (graphs of 85 to 150 nodes, 8 heads of 8, float32, one training step: 300 us with what the
-// compiler takes, 278 us with these); wide heads' backward needs the registers of one.
+// compiler takes, 278 us with these).  bf16 heads over 64: dq too (8 sequences of 2048, 16 heads
+// of 128 over 4, causal, one training step: 1215 us with one wave, 1087 us with two); dk and
+// dv, whose two accumulators are 128 registers, spill under two (1645 us).
 template <typename T, int DP>
 constexpr int waves_per_simd(AttnPass pass) {
     if (Shape<T, DP>::W == 16) return pass == kDkv ? 4 : 6;
-    return pass == kFwd || DP <= 64 ? 2 : 1;
+    return pass == kFwd || DP <= 64 || (pass == kDq && sizeof(T) == 2) ? 2 : 1;
 }
 
 // scores[row][col] of ROWS rows in LDS against the wave's columns

@@ -15,10 +15,12 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
+from .graph import get_csr
 from .layer import GraphAttentionLayer, GraphAttentionLayerActivationTest
+from .sequence import Embedding, LayerNorm, packed_attention
 
-__all__ = ["GraphData", "GATNet", "GATModel", "GATActivationModel", "segment_mean",
-           "GATNET_CONFIGS"]
+__all__ = ["GraphData", "GATNet", "GlobalGATNet", "GATModel", "GATActivationModel",
+           "segment_mean", "GATNET_CONFIGS"]
 
 
 class GraphData:
@@ -41,6 +43,14 @@ class GraphData:
     @property
     def num_node_features(self) -> int:
         return int(self.x.size(1))
+
+    def ptr(self) -> torch.Tensor:
+        """int32 offsets ``[num_graphs + 1]`` of the graphs' nodes (``batch`` ascends, as
+        ``collate`` and PyG make it), on ``batch``'s device and without a host read."""
+        if self.batch is None or self.num_graphs is None:
+            raise ValueError("ptr() needs a batch vector and num_graphs")
+        graphs = torch.arange(self.num_graphs + 1, device=self.batch.device)
+        return torch.searchsorted(self.batch, graphs, out_int32=True)
 
     def to(self, device) -> "GraphData":
         kw = {k: (v.to(device) if isinstance(v, torch.Tensor) else v)
@@ -119,6 +129,50 @@ class GATNet(torch.nn.Module):
         x = F.dropout(x, p=0.6, training=self.training)
         x = self.conv2(x, edge_index)
         return F.log_softmax(x, dim=1)
+
+
+class GlobalGATNet(torch.nn.Module):
+    """Graph classification with attention over edges and over whole graphs: the CIFAR10
+    ``GATNet``'s two edge-attention layers (8 heads of 8), between them a residual block in
+    which every node attends to all nodes of its graph, and one query per head that reads each
+    graph's nodes in place of their mean.  Nodes also carry an embedding of their in-degree.
+
+    conv1 -> ELU (+ degree embedding) -> + attention(norm) -> + ELU(conv2(norm)) -> readout
+    -> Linear+ReLU -> Linear -> log_softmax."""
+
+    HEADS, DIM, DEGREES = 8, 8, 64
+
+    def __init__(self, num_features: int, num_classes: int = 10):
+        super().__init__()
+        h, d = self.HEADS, self.DIM
+        self.conv1 = GraphAttentionLayer(num_features, d, num_heads=h, concat=True, dropout=0.0)
+        self.degree = Embedding(self.DEGREES, h * d, scale=0.1)
+        self.norm1 = LayerNorm(h * d)
+        self.qkv = torch.nn.Linear(h * d, 3 * h * d)
+        self.proj = torch.nn.Linear(h * d, h * d)
+        self.norm2 = LayerNorm(h * d)
+        self.conv2 = GraphAttentionLayer(h * d, d, num_heads=h, concat=True, dropout=0.0)
+        self.norm3 = LayerNorm(h * d)
+        self.query = torch.nn.Parameter(torch.randn(1, h, d))
+        self.kv = torch.nn.Linear(h * d, 2 * h * d)
+        self.lin1 = torch.nn.Linear(h * d, h * d)
+        self.lin2 = torch.nn.Linear(h * d, num_classes)
+
+    def forward(self, data):
+        x, edge_index = data.x, data.edge_index
+        h, d = self.HEADS, self.DIM
+        ptr = data.ptr()
+        rowptr = get_csr(edge_index, x.size(0), x.device).rowptr
+        degree = (rowptr[1:] - rowptr[:-1] - 1).clamp(max=self.DEGREES - 1)  # without the self-loop
+        x = F.elu(self.conv1(x, edge_index)) + self.degree(degree)
+        q, k, v = self.qkv(self.norm1(x)).view(-1, 3, h, d).unbind(1)
+        x = x + self.proj(packed_attention(q, k, v, ptr).reshape(-1, h * d))
+        x = x + F.elu(self.conv2(self.norm2(x), edge_index))
+        k, v = self.kv(self.norm3(x)).view(-1, 2, h, d).unbind(1)
+        each = torch.arange(data.num_graphs + 1, dtype=torch.int32, device=x.device)
+        x = packed_attention(self.query.expand(data.num_graphs, h, d), k, v, each, ptr)
+        x = F.relu(self.lin1(x.reshape(-1, h * d)))
+        return F.log_softmax(self.lin2(x), dim=1)
 
 
 class GATModel(torch.nn.Module):

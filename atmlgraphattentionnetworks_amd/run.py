@@ -18,6 +18,7 @@ CLI::
 
     python -m atmlgraphattentionnetworks_amd.run node --dataset Cora --runs 1
     python -m atmlgraphattentionnetworks_amd.run graph --train-graphs 2048 --runs 1
+    python -m atmlgraphattentionnetworks_amd.run graph --model global --runs 1
     python -m atmlgraphattentionnetworks_amd.run heads --dataset Cora --runs 1
 """
 from __future__ import annotations
@@ -302,7 +303,7 @@ def _node_runs(make_model: Callable[[int, int], torch.nn.Module], dataset: str, 
 
 
 def main(argv=None) -> Dict:
-    from .gatnet import GATActivationModel, GATModel, GATNet
+    from .gatnet import GATActivationModel, GATModel, GATNet, GlobalGATNet
     ap = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
     ap.add_argument("task", choices=["node", "graph", "heads", "params", "act"])
     ap.add_argument("--dataset", default="Citeseer")
@@ -315,6 +316,9 @@ def main(argv=None) -> Dict:
     ap.add_argument("--train-graphs", type=int, default=2048)
     ap.add_argument("--eval-graphs", type=int, default=512)
     ap.add_argument("--batch-size", type=int, default=512)
+    ap.add_argument("--model", choices=["gat", "global"], default="gat",
+                    help="graph task: the reference's GATNet, or GlobalGATNet (attention over "
+                         "whole graphs between and after its two layers)")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--checkpoint", default=None)
     ap.add_argument("--verbose", action="store_true")
@@ -356,7 +360,8 @@ def main(argv=None) -> Dict:
         accs, details = [], []
         for r in range(a.runs):
             torch.manual_seed(a.seed + r)
-            model = GATNet("GAT", "CIFAR10", 3).to(device)
+            model = (GlobalGATNet(3) if a.model == "global" else
+                     GATNet("GAT", "CIFAR10", 3)).to(device)
             res = train_graph_classification(model, train, val, test, device, cfg)
             accs.append(res.test_acc)
             details.append({"test_acc": res.test_acc, "epochs": res.epochs,

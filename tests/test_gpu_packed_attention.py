@@ -351,3 +351,20 @@ def test_long_cache_offsets():
     # the same sums cut at other places: both sides' rounded probabilities and results
     mag = attend(q, kt, vt.abs(), torch.tensor([0, 2], device=DEV), torch.tensor([0, tail], device=DEV))
     assert bool(((got.float() - want.float()).abs() <= 2 * (2 * h + tail * U) * mag.float() * (1 + h)).all())
+
+
+def test_refusals():
+    q, k, v = tensors(8, 8, 4, 2, 16, torch.float32)
+    p = torch.tensor([0, 8], device=DEV)
+    for args, kw in (((q.half(), k.half(), v.half(), p), {}), ((q[0], k, v, p), {}),
+                     ((q, k.bfloat16(), v, p), {}), ((q, k, v[:4], p), {}),
+                     ((q[:, :3], k, v, p), {}), ((q, k[..., :8], v[..., :8], p), {}),
+                     ((q, k, v, p.float()), {}), ((q, k, v, p[None]), {}), ((q, k, v, p[:0]), {}),
+                     ((q, k, v, p), dict(kv_ptr=p[:1])),
+                     (tuple(torch.zeros(8, 1, 129, device=DEV) for _ in range(3)) + (p,), {})):
+        with pytest.raises(ValueError):
+            attend(*args, **kw)
+    with pytest.raises(RuntimeError):
+        attend(q, k, v, p.cpu())
+    with pytest.raises(TypeError):
+        attend(q, k, v, [0, 8])

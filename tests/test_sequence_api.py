@@ -68,3 +68,66 @@ def test_embedding_library_checks():
         assert grad(**bad) == _lib.GAT_EINVAL, bad
     small = _lib.embedding_grad_workspace_size(100, 50, 8)
     assert 0 < small < _lib.embedding_grad_workspace_size(100000, 50, 8)
+
+
+def test_packed_attention_library_checks():
+    from atmlgraphattentionnetworks_amd import _lib
+    lib = _lib.load()
+    EINVAL, EUNS, EWS, OK = (_lib.GAT_EINVAL, _lib.GAT_EUNSUPPORTED, _lib.GAT_EWORKSPACE, _lib.GAT_OK)
+
+    def fwd(nq=8, nk=8, count=2, h=4, hk=2, d=16, dt=0, q=64, k=64, out=64, ptr=64, row=64, head=16,
+            kv_row=32, ws=None, size=0, low=None):
+        return lib.gat_packed_attention(q, row, head, k, kv_row, head, k, kv_row, head, ptr, ptr, 0,
+                                        count, nq, nk, h, hk, d, 0.25, 1, out, low, None, ws, size, dt,
+                                        None)
+    assert fwd(nq=0) == OK
+    for bad in (dict(nq=-1), dict(nk=-1), dict(count=-1), dict(h=0), dict(hk=0), dict(h=5),
+                dict(d=0), dict(dt=2), dict(dt=3), dict(q=None), dict(k=None), dict(out=None),
+                dict(ptr=None), dict(ws=68), dict(low=68)):
+        assert fwd(**bad) == EINVAL, bad
+    # heads too wide, not whole 16-byte vectors, unaligned addresses or strides, tokens that
+    # overlap, strides out of reach, too many rows
+    for far in (dict(d=132, row=528, head=132, kv_row=264), dict(d=18), dict(d=12, dt=1), dict(q=72),
+                dict(row=66), dict(head=18), dict(row=12), dict(row=(1 << 22) + 4),
+                dict(head=1 << 28), dict(nq=1 << 30), dict(nk=1 << 30)):
+        assert fwd(**far) == EUNS, far
+    # one query over many keys is split: that takes a workspace
+    size = _lib.packed_attention_workspace_size(False, 1, 100000, 1, 4, 2, 16, 0)
+    assert size > 0
+    assert fwd(nq=1, nk=100000, count=1) == EWS
+    assert fwd(nq=1, nk=100000, count=1, ws=64, size=size - 1) == EWS
+    # short sequences are not
+    assert _lib.packed_attention_workspace_size(False, 65536, 65536, 2048, 4, 2, 16, 0) == 0
+
+    def bwd(nq=8, nk=8, g=64, out=64, lse=64, dq=64, dk=64, ws=64, size=1 << 20, d=16):
+        return lib.gat_packed_attention_backward(g, 64, 16, 64, 64, 16, 64, 32, 16, 64, 32, 16, out, None,
+                                                 lse, 64, 64, 0, 2, nq, nk, 4, 2, d, 0.25, 1, dq, dk, 64,
+                                                 ws, size, 0, None)
+    for bad in (dict(g=None), dict(out=None), dict(lse=None), dict(dq=None), dict(dk=None), dict(ws=72),
+                dict(nq=-1)):
+        assert bwd(**bad) == EINVAL, bad
+    assert bwd(size=0) == EWS and bwd(ws=None) == EWS
+    assert bwd(g=72) == EUNS and bwd(d=130) == EUNS
+    assert bwd(nq=0, nk=0) == OK
+    out = ctypes.c_size_t()
+    size_of = lib.gat_packed_attention_backward_workspace_size
+    assert size_of(8, 8, 2, 4, 2, 16, 0, None) == EINVAL
+    assert size_of(8, 8, 2, 4, 2, 200, 0, ctypes.byref(out)) == EUNS
+    assert size_of(8, 8, 2, 4, 2, 16, 0, ctypes.byref(out)) == OK and out.value >= 8 * 4 * 4
+
+
+def test_packed_attention_refuses_cpu_tensors_and_bad_batches():
+    import atmlgraphattentionnetworks_amd as gat
+    from atmlgraphattentionnetworks_amd.gatnet import GraphData
+    q = torch.randn(4, 2, 8)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        gat.packed_attention(q, q, q, torch.tensor([0, 4]))
+    with pytest.raises(ValueError, match="ptr"):
+        GraphData(torch.zeros(3, 1), torch.zeros(2, 0, dtype=torch.int64)).ptr()
+
+
+def test_graph_data_ptr_counts_nodes():
+    from atmlgraphattentionnetworks_amd.gatnet import GraphData
+    b = torch.tensor([0, 0, 0, 2, 2, 4])
+    d = GraphData(torch.zeros(6, 1), torch.zeros(2, 0, dtype=torch.int64), batch=b, num_graphs=6)
+    assert d.ptr().tolist() == [0, 3, 3, 5, 5, 6, 6] and d.ptr().dtype == torch.int32
