@@ -42,7 +42,7 @@ def _stream(device: torch.device) -> int:
 def _need_tensor(what: str, name: str, t, dtypes=_DTYPES) -> torch.Tensor:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: {name} must be a torch.Tensor, got {type(t).__name__}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{what} needs ROCm device tensors ({name} is on {t.device}); "
                            "there is no CPU path")
     if t.dtype not in dtypes:
