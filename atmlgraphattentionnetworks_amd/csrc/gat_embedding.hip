@@ -14,6 +14,9 @@
 // summed by workgroups of their own, and the partial sums are joined in order.
 // Sums are float32 and rounded once, after the scale.
 //
+// Few tokens (few_tokens): one launch instead of the sort's four and more.  A workgroup owns
+// kOwnRows table rows, picks their tokens out of all ids in order, and sums as above.
+//
 // Sort: least significant digit first, 8 bits a pass, over (id, token) pairs; an id that
 // takes no gradient (out of range, or the padding id) sorts behind the table as id
 // `vocab`.  A pass is two launches: digit counts per workgroup, then every workgroup
@@ -29,6 +32,7 @@ constexpr int kSortWaves = kSortBlock / kWave;
 constexpr int kSortMinItems = 1024;
 constexpr int kSortMaxBlocks = 256;
 constexpr int kMinPiece = 16, kMaxPieces = 4096;
+constexpr int kFewTokens = 1024, kOwnRows = 64, kOwnHot = 32;
 constexpr long long kMaxTokens = 1ll << 30;
 constexpr int kEmbedBlock = 256;
 
@@ -386,6 +390,98 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_sums(
                             blockIdx.x);
 }
 
+// Few tokens: table rows [kOwnRows * blockIdx.x, ...).  Rows with up to kOwnHot tokens are one
+// group's, walking the workgroup's list; for the others the groups share the tokens.
+template <typename T, int LPR>
+__global__ __launch_bounds__(kEmbedBlock) void k_embed_own(Ids s, int n, const T* g, long long ld_g,
+                                                           int whole_g, int cols, float scale, T* dw,
+                                                           long long ld_dw, int whole) {
+    constexpr int N = Vec16<T>::N, U = 8, G = kEmbedBlock / LPR, WAVES = kEmbedBlock / kWave;
+    typedef typename Vec16<T>::type V;
+    __shared__ unsigned list[kFewTokens];  // row << 16 | token, ascending tokens
+    __shared__ int found[kOwnRows], wave_found[WAVES];
+    __shared__ float lds[kEmbedBlock * N];
+    const int tid = threadIdx.x, lane = tid % LPR, grp = tid / LPR;
+    const int v0 = blockIdx.x * kOwnRows;
+    const int rows = s.vocab - v0 < kOwnRows ? s.vocab - v0 : kOwnRows;
+    const int c = (blockIdx.y * LPR + lane) * N;
+    if (tid < kOwnRows) found[tid] = 0;
+    int total = 0;
+    for (int t0 = 0; t0 < n; t0 += kEmbedBlock) {
+        const int t = t0 + tid;
+        const int r = t < n ? (int)key_at(s, t) - v0 : -1;
+        const bool ours = r >= 0 && r < rows;
+        const unsigned long long m = __ballot(ours);
+        if (tid % kWave == 0) wave_found[tid / kWave] = __popcll(m);
+        __syncthreads();
+        int at = total + __popcll(m & ((1ull << (tid % kWave)) - 1));
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) {
+            if (k < tid / kWave) at += wave_found[k];
+            total += wave_found[k];
+        }
+        if (ours) {
+            list[at] = (unsigned)r << 16 | (unsigned)t;
+            atomicAdd(&found[r], 1);
+        }
+        __syncthreads();
+    }
+    // acc += the rows of g whose list entries belong to row r, every `step`th from `skip` on
+    const unsigned long long mine =
+        LPR == kWave ? ~0ull : ((1ull << (LPR & 63)) - 1) << (tid % kWave / LPR * LPR);
+    auto sum = [&](float(&acc)[N], int r, int skip, int step) {
+        for (int i0 = 0; i0 < total; i0 += LPR) {
+            const unsigned entry = i0 + lane < total ? list[i0 + lane] : ~0u;
+            unsigned long long m = __ballot((int)(entry >> 16) == r) & mine;
+            while (m != 0) {
+                V x[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    for (; m != 0 && skip > 0; --skip) m &= m - 1;
+                    const int from = m != 0 ? __ffsll((long long)m) - 1 : 0;
+                    const unsigned tok = __shfl(entry, from) & 0xFFFF;
+                    x[u] = V{};
+                    if (m != 0) {
+                        x[u] = load_vec<T>(g + (long long)tok * ld_g, c, cols, whole_g);
+                        m &= m - 1;
+                        skip = step - 1;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int k = 0; k < N; ++k) acc[k] += (float)x[u][k];
+            }
+        }
+    };
+    auto store = [&](const float(&acc)[N], int r) {
+        V y;
+#pragma unroll
+        for (int k = 0; k < N; ++k) y[k] = (T)(acc[k] * scale);
+        store_vec<T>(dw + (long long)(v0 + r) * ld_dw, c, cols, whole, y);
+    };
+    for (int r = grp; r < rows; r += G) {
+        if (found[r] > kOwnHot) continue;
+        float acc[N] = {};
+        if (found[r] > 0) sum(acc, r, 0, 1);
+        store(acc, r);
+    }
+    for (int r = 0; r < rows; ++r) {
+        if (found[r] <= kOwnHot) continue;
+        float acc[N] = {};
+        sum(acc, r, grp, G);
+        join_groups<N, LPR>(acc, lds);
+        if (grp == 0) store(acc, r);
+    }
+}
+
+// One launch beats the sort where launches are the time: every workgroup looks at all ids, and
+// one that is all tokens' is summed by one workgroup, so the tokens are few; table rows are
+// limited so that the looking stays below writing the rows.
+inline bool few_tokens(long long tokens, int vocab) {
+    return tokens <= kFewTokens && vocab <= 1 << 20;
+}
+
 // lanes per row: the power of two in [8, 64] that covers it, if one does
 inline int embed_lanes(int cols, int dtype) {
     const int n = 16 / (int)dtype_size(dtype);
@@ -506,6 +602,23 @@ int embed_by_lanes(int lanes, const Ids& ids, long long tokens, const void* w, l
     return call(std::integral_constant<int, 64>());
 }
 
+template <typename T>
+int embed_own_by_lanes(int lanes, const Ids& ids, int n, const void* g, long long ld_g, int cols,
+                       float scale, void* dw, long long ld_dw, int dtype, hipStream_t s) {
+    const int whole_g = rows_whole(g, ld_g, dtype), whole = rows_whole(dw, ld_dw, dtype);
+    auto call = [&](auto l) {
+        constexpr int L = decltype(l)::value;
+        const int slabs = (cols + L * Vec16<T>::N - 1) / (L * Vec16<T>::N);
+        k_embed_own<T, L><<<dim3((ids.vocab + kOwnRows - 1) / kOwnRows, slabs), kEmbedBlock, 0, s>>>(
+            ids, n, static_cast<const T*>(g), ld_g, whole_g, cols, scale, static_cast<T*>(dw), ld_dw, whole);
+        return status_of(hipGetLastError());
+    };
+    if (lanes == 8) return call(std::integral_constant<int, 8>());
+    if (lanes == 16) return call(std::integral_constant<int, 16>());
+    if (lanes == 32) return call(std::integral_constant<int, 32>());
+    return call(std::integral_constant<int, 64>());
+}
+
 inline bool ids_fit(const void* ids, int ids64, long long tokens) {
     return tokens == 0 ||
            (ids != nullptr && (reinterpret_cast<uintptr_t>(ids) & (ids64 ? 7 : 3)) == 0);
@@ -535,9 +648,9 @@ int gat_embedding(const void* ids, int ids64, long long tokens, const void* w, l
 }
 
 int gat_embedding_grad_workspace_size(long long tokens, int vocab, int cols, size_t* bytes) {
-    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || cols <= 0 || bytes == nullptr)
+    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || vocab > kMaxTokens || cols <= 0 || bytes == nullptr)
         return GAT_EINVAL;
-    *bytes = grad_layout((int)tokens, vocab, cols).bytes;
+    *bytes = few_tokens(tokens, vocab) ? 0 : grad_layout((int)tokens, vocab, cols).bytes;
     return GAT_OK;
 }
 
@@ -545,16 +658,25 @@ int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void*
                        int vocab, int cols, float scale, long long padding, void* dw,
                        long long ld_dw, void* workspace, size_t workspace_bytes, int dtype,
                        void* stream) {
-    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || cols <= 0 || !known_dtype(dtype) ||
+    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || vocab > kMaxTokens || cols <= 0 || !known_dtype(dtype) ||
         ld_g < 0 || ld_dw < cols || dw == nullptr || !element_aligned(dw, dtype) ||
         !ids_fit(ids, ids64, tokens) ||
         (tokens > 0 && (g == nullptr || !element_aligned(g, dtype))))
         return GAT_EINVAL;
     const int n = (int)tokens;
+    const Ids s{ids, ids64, padding, vocab};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int lanes = embed_lanes(cols, dtype);
+    if (few_tokens(n, vocab)) {
+        if (dtype == GAT_F32)
+            return embed_own_by_lanes<float>(lanes, s, n, g, ld_g, cols, scale, dw, ld_dw, dtype, st);
+        if (dtype == GAT_BF16)
+            return embed_own_by_lanes<bf16>(lanes, s, n, g, ld_g, cols, scale, dw, ld_dw, dtype, st);
+        return embed_own_by_lanes<f16>(lanes, s, n, g, ld_g, cols, scale, dw, ld_dw, dtype, st);
+    }
     const GradLayout l = grad_layout(n, vocab, cols);
     if (workspace == nullptr || workspace_bytes < l.bytes) return GAT_EWORKSPACE;
     if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return GAT_EINVAL;
-    hipStream_t st = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
     unsigned* keys[2] = {reinterpret_cast<unsigned*>(ws + l.keys[0]),
                          reinterpret_cast<unsigned*>(ws + l.keys[1])};
@@ -563,7 +685,6 @@ int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void*
     unsigned* counts = reinterpret_cast<unsigned*>(ws + l.counts);
     int* first = reinterpret_cast<int*>(ws + l.first);
     float* part = reinterpret_cast<float*>(ws + l.part);
-    const Ids s{ids, ids64, padding, vocab};
     int cur = 0;
     if (n > 0) {
         const SortPlan p = sort_plan(n, vocab);
@@ -584,7 +705,6 @@ int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void*
         }
     }
     k_sort_firsts<<<n / 256 + 1, 256, 0, st>>>(keys[cur], n, vocab, first);
-    const int lanes = embed_lanes(cols, dtype);
     if (dtype == GAT_F32)
         return embed_grad_by_lanes<float>(lanes, keys[cur], toks[cur], first, n, vocab, g, ld_g, cols,
                                           scale, part, dw, ld_dw, dtype, st);

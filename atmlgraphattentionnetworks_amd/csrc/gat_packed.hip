@@ -1124,6 +1124,7 @@ int attn_launch(const AttnArgs& a, const Plan& p, hipStream_t s) {
     const bool keys = PASS == kDkv;
     const long long need = slots_of(keys ? a.nk : a.nq, keys ? 1 : a.group, Shape<T, DP>::W * p.waves, a.count);
     const long long slots = a.by_xcd ? (need + 7) / 8 * 8 : need;
+    if (slots * 64 * p.waves > 0xFFFFFFFFll) return GAT_EUNSUPPORTED;  // lanes of one launch
     const dim3 grid((unsigned)slots, a.kv_heads, p.splits);
     // row tiles a step: two where the registers allow it (their chains interleave)
     constexpr int R = sizeof(T) == 4 ? 1 : PASS == kFwd || DP <= 64 ? 2 : 1;

@@ -200,11 +200,11 @@ class _Embedding(torch.autograd.Function):
         g = _rows(g)
         dw = torch.empty(v, c, dtype=g.dtype, device=g.device)
         size = _lib.embedding_grad_workspace_size(ids.numel(), v, c)
-        ws = torch.empty(size, dtype=torch.uint8, device=g.device)
+        ws = torch.empty(size, dtype=torch.uint8, device=g.device) if size else None
         with _on(g.device):
             rc = _lib.load().gat_embedding_grad(
                 ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(), g.data_ptr(),
-                g.stride(0), v, c, ctx.scale, ctx.padding, dw.data_ptr(), c, ws.data_ptr(), size,
+                g.stride(0), v, c, ctx.scale, ctx.padding, dw.data_ptr(), c, _ptr(ws), size,
                 _DTYPES[g.dtype], _stream(g.device))
         if rc:
             _lib.check(rc, "gat_embedding_grad")
@@ -219,7 +219,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     rows are read like any other.
 
     An id outside ``[0, vocab)`` gives a row of NaN and takes no gradient: checking on the
-    host would cost a synchronisation per call.  At most 2^30 ids."""
+    host would cost a synchronisation per call.  At most 2^30 ids and 2^30 table rows."""
     _need_tensor("embedding", "weight", weight)
     _need_tensor("embedding", "ids", ids, (torch.int64, torch.int32))
     _need_like("embedding", "ids", ids, weight, dtype=False)
@@ -227,8 +227,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
         raise ValueError(f"embedding: weight must be [vocab, C] with both at least 1, "
                          f"got {tuple(weight.shape)}")
     v = weight.shape[0]
-    if v > 0x7FFFFFFE or ids.numel() > 1 << 30:
-        raise ValueError("embedding: at most 2^31 - 2 table rows and 2^30 ids")
+    if v > 1 << 30 or ids.numel() > 1 << 30:
+        raise ValueError("embedding: at most 2^30 table rows and 2^30 ids")
     pad = -1
     if padding_idx is not None:
         if not -v <= padding_idx < v:

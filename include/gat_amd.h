@@ -632,7 +632,8 @@ int gat_embedding_grad_workspace_size(long long tokens, int vocab, int cols, siz
  * [0, vocab); rows without a token are zeros.  Deterministic.
  *   padding  an id whose tokens take no gradient, or -1.  Ids outside [0, vocab) take
  *            none either.
- *   workspace  16-byte aligned
+ *   vocab    at most 2^30
+ *   workspace  16-byte aligned; none where the size is 0 (few tokens)
  */
 int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void* g, long long ld_g,
                        int vocab, int cols, float scale, long long padding, void* dw,

@@ -230,6 +230,43 @@ def test_embedding_columns(cols, t):
                torch.randn(900, cols, device=DEV).to(t), 3.3, what=f"{cols} {t}")
 
 
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("cols", [1, 3, 8, 32, 63, 64, 100, 128, 257, 512, 1000])
+def test_embedding_columns_of_many_tokens(cols, t):
+    torch.manual_seed(cols)
+    ids = torch.randint(0, 37, (3000,), device=DEV)
+    ids[:700] = 5
+    embed_case(ids, torch.randn(37, cols, device=DEV).to(t),
+               torch.randn(3000, cols, device=DEV).to(t), 3.3, what=f"{cols} {t}")
+
+
+# a row's tokens around what one group sums alone, rows around what a workgroup owns
+@pytest.mark.parametrize("count", [1, 31, 32, 33, 64, 400])
+@pytest.mark.parametrize("vocab", [1, 63, 64, 65, 1000])
+def test_embedding_few_tokens(vocab, count):
+    torch.manual_seed(vocab + count)
+    for cols, t in ((20, torch.float32), (100, torch.bfloat16), (300, torch.float16)):
+        ids = torch.randint(0, vocab, (2 * count + 7,), device=DEV)
+        ids[torch.randperm(len(ids), device=DEV)[:count]] = vocab // 2
+        ids[-3:] = vocab - 1
+        embed_case(ids, torch.randn(vocab, cols, device=DEV).to(t),
+                   torch.randn(len(ids), cols, device=DEV).to(t), -0.7,
+                   padding=vocab - 1 if vocab > 60 else None, what=f"{vocab} {count} {cols}")
+
+
+def test_embedding_few_tokens_outside_ids():
+    torch.manual_seed(5)
+    ids = torch.randint(0, 30, (200,), device=DEV)
+    ids[5], ids[6], ids[7] = -1, 30, 1 << 40
+    g = torch.randn(200, 16, device=DEV)
+    ws = torch.randn(30, 16, device=DEV).requires_grad_()
+    dw, = torch.autograd.grad(ops().embedding(ids, ws), ws, g)
+    keep = torch.ones(200, dtype=torch.bool, device=DEV)
+    keep[5:8] = False
+    only, = torch.autograd.grad(ops().embedding(ids[keep], ws), ws, g[keep])
+    assert torch.equal(dw, only)  # the same sums in the same order
+
+
 # table sizes at the digits' borders, token counts at the pieces' and the sort's
 @pytest.mark.parametrize("vocab", [1, 2, 255, 256, 257, 65535, 65536, 70001])
 @pytest.mark.parametrize("tokens", [1, 127, 128, 129, 1024, 1025, 5000])

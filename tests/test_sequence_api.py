@@ -59,14 +59,16 @@ def test_embedding_library_checks():
                 dict(ids=68), dict(ids=66, ids64=0), dict(w=66)):
         assert fwd(**bad) == _lib.GAT_EINVAL, bad
 
-    def grad(tokens=4, vocab=8, ld=8, size=1 << 24, ws=64, g=64, dw=64):
+    def grad(tokens=4000, vocab=8, ld=8, size=1 << 24, ws=64, g=64, dw=64):
         return lib.gat_embedding_grad(64, 1, tokens, g, ld, vocab, 8, 1.0, -1, dw, ld, ws, size, 0,
                                       None)
     assert grad(size=16) == _lib.GAT_EWORKSPACE
     assert grad(ws=None) == _lib.GAT_EWORKSPACE
-    for bad in (dict(ws=68), dict(g=None), dict(dw=None), dict(ld=7), dict(tokens=-1)):
+    for bad in (dict(ws=68), dict(g=None), dict(dw=None), dict(ld=7), dict(tokens=-1),
+                dict(vocab=(1 << 30) + 1)):
         assert grad(**bad) == _lib.GAT_EINVAL, bad
-    small = _lib.embedding_grad_workspace_size(100, 50, 8)
+    assert _lib.embedding_grad_workspace_size(100, 50, 8) == 0
+    small = _lib.embedding_grad_workspace_size(2000, 50, 8)
     assert 0 < small < _lib.embedding_grad_workspace_size(100000, 50, 8)
 
 
