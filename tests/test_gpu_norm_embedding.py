@@ -178,6 +178,33 @@ def test_norm_non_finite_rows_stay_apart():
     assert bool(got[[7, 21]].isnan().all())
 
 
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("cols", [1, 7, 9, 31, 100, 515, 1433])
+@pytest.mark.parametrize("rows", [1, 2, 3, 40])
+def test_norm_between_non_finite_neighbours(rows, cols, t):
+    """What lies around a row's ends, in other rows or in the columns left out of a view,
+    has no part in it."""
+    torch.manual_seed(rows + cols)
+    gat = ops()
+    w, b = torch.randn(cols, device=DEV).to(t), torch.randn(cols, device=DEV).to(t)
+    for gap, first in ((0, 0), (3, 1), (16, 8)):
+        x, g = (torch.full((rows, first + cols + gap), float("nan"), device=DEV, dtype=t)
+                for _ in range(2))
+        xv, gv = x[:, first:first + cols], g[:, first:first + cols]
+        xv.copy_(torch.randn(rows, cols, device=DEV))
+        gv.copy_(torch.randn(rows, cols, device=DEV))
+        if rows > 3 and gap == 0:
+            xv[5::7] = float("inf")
+        keep = torch.isfinite(xv).all(1)
+        leaf = xv.detach().requires_grad_()
+        y = gat.layer_norm(leaf, w, b)
+        dx, = torch.autograd.grad(y, leaf, gv)
+        want = norm_reference(xv[keep].cpu(), w.cpu(), b.cpu(), 1e-5, gv[keep].cpu())
+        for name, got, (v, e) in zip(("y", "dx"), (y, dx), want):
+            close(got[keep], v, e + half_step(t) * (v.abs() + e) + torch.finfo(t).tiny,
+                  f"{rows} {cols} {t} {gap} {name}")
+
+
 def test_norm_gradient_against_differences():
     torch.manual_seed(5)
     x, g = torch.randn(2, 6, 20, device=DEV)
