@@ -1,12 +1,15 @@
 #pragma once
 // MI355X (gfx950) GAT attention layer: HIP kernels + C-ABI — shared helpers.
 //
-// The library is five translation units that include this header:
+// The library is eight translation units that include this header:
 //   gat_abi.hip       ABI version, table layout, the knob snapshot
 //   gat_project.hip   projection + score epilogue (gat_project*)
 //   gat_edge.hip      fused edge kernel, hub merge, gat_layer_forward
 //   gat_csr.hip       CSR / CSC builds (gat_csr_build, gat_csc_build)
 //   gat_backward.hip  recompute backward, weight and input gradients
+//   gat_norm.hip      layer norm, forward and backward      (these three share
+//   gat_embedding.hip embedding and its sorted gradient      gat_seq.h: element
+//   gat_packed.hip    attention over packed sequences        types, row vectors)
 //
 // Replaces the hot path of danieldritter/ATMLGraphAttentionNetworks
 // GraphAttentionLayer.forward (GAT.py:37-67) and the PyG pieces it calls:
