@@ -390,13 +390,11 @@ __device__ __forceinline__ void add_non_finite(typename Shape<T, DP>::Acc* acc, 
 // rows behind it and dimensions behind `dim` arrive as zeros.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned offset, int scalar_offset,
-                                            unsigned lds) {
+__device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned offset, unsigned lds) {
     // m0 holds the LDS address; the nops cover scalar operands that a vector instruction wrote
-    asm volatile(
-        "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds),
-        "v"(offset), "s"(buffer), "s"(scalar_offset)
-        : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds),
+                 "v"(offset), "s"(buffer)
+                 : "memory");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -419,8 +417,8 @@ struct Loader {
     typedef Shape<T, DP> S;
     static constexpr int LOADS = (BN * S::CPR + kWave - 1) / kWave;  // of a wave each
     static constexpr int CNT = (LOADS + NW - 1) / NW;
-    // A wave's loads lie STEP rows apart; where that is a multiple of 16 they differ by a
-    // scalar only.
+    // A wave's loads lie STEP rows apart; where that is a multiple of 16 they differ by one
+    // value for all lanes.
     static constexpr int STEP = NW * kWave % S::CPR == 0 ? NW * kWave / S::CPR : 0;
     static constexpr bool EVEN = CNT == 1 || (STEP > 0 && STEP % 16 == 0);
     unsigned offset[EVEN ? 1 : CNT];  // of this lane's vectors within a tile
@@ -444,8 +442,10 @@ struct Loader {
         for (int j = 0; j < CNT; ++j) {
             const int k = uniform(threadIdx.x / kWave) + NW * j;
             if (LOADS % NW != 0 && k >= LOADS) break;
-            load_to_lds(b, offset[EVEN ? 0 : j], EVEN ? j * STEP * row_elements * (int)sizeof(T) : 0,
-                        uniform((int)(to + k * kWave * 16)));
+            // added to the lane's offset, not as the scalar one: that is no part of what the
+            // buffer's size is compared with
+            const unsigned more = EVEN ? (unsigned)(j * STEP * row_elements) * (unsigned)sizeof(T) : 0u;
+            load_to_lds(b, offset[EVEN ? 0 : j] + more, uniform((int)(to + k * kWave * 16)));
         }
     }
     // The same for rows of the packed (query, head of the group) axis: rows [r0, end), row r
@@ -463,7 +463,7 @@ struct Loader {
             const int r = r0 + at / S::CPR, i = div_group(a, r);
             const unsigned o = (unsigned)((i - i0) * (int)x.row + (r - i * a.group) * (int)x.head) *
                                    (unsigned)sizeof(T) + offset[EVEN ? 0 : j];
-            load_to_lds(b, r < end ? o : 0x80000000u, 0, uniform((int)(to + k * kWave * 16)));
+            load_to_lds(b, r < end ? o : 0x80000000u, uniform((int)(to + k * kWave * 16)));
         }
     }
 };

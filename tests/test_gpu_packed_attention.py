@@ -187,6 +187,29 @@ def test_rows_outside_the_sequences(t):
     assert bool((lse[:11] == -math.inf).all()) and bool((lse[81:] == -math.inf).all())
 
 
+@pytest.mark.parametrize("t", BOTH, ids=str)
+@pytest.mark.parametrize("d", [8, 16, 32, 40, 64, 80, 96, 128])
+def test_rows_behind_a_tile_of_every_length(d, t):
+    """What lies behind a sequence's last row, to the end of the last tile, has no part."""
+    for n in (1, 2, 15, 16, 17, 31, 33, 48, 63, 65, 100):
+        for h, hk in ((2, 2), (4, 1)):
+            clean = (*tensors(n, n, h, hk, d, t, seed=n), torch.randn(n, h, d, device=DEV).to(t))
+            leaves = []
+            for x in clean:  # the same rows at the start of a tensor of NaN
+                behind = torch.full((n + 130, *x.shape[1:]), math.nan, device=DEV, dtype=t)
+                behind[:n] = x
+                leaves.append(behind[:n])
+            ptr = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+            for causal in (False, True):
+                got = []
+                for q, k, v, g in (clean, leaves):
+                    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+                    y = attend(q, k, v, ptr, causal=causal)
+                    got.append([y, *torch.autograd.grad(y, (q, k, v), g)])
+                for a, b in zip(*got):
+                    assert bool(a.isfinite().all()) and torch.equal(a, b), (n, h, hk, causal)
+
+
 def test_no_sequences_and_no_rows():
     for t in BOTH:
         q, k, v = tensors(5, 6, 2, 1, 16, t)
