@@ -174,10 +174,14 @@ class LayerNorm(torch.nn.Module):
 # Embedding
 # ---------------------------------------------------------------------------
 def _embed_forward(ids, w, scale):
+    w = _rows(w)
+    ld = w.stride(0) if w.shape[0] > 1 else w.shape[1]  # one row: its stride says nothing
+    if ld < w.shape[1]:  # a row repeated by expand()
+        w, ld = w.contiguous(), w.shape[1]
     out = torch.empty(ids.numel(), w.shape[1], dtype=w.dtype, device=w.device)
     with _on(w.device):
         rc = _lib.load().gat_embedding(ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(),
-                                       w.data_ptr(), w.stride(0), w.shape[0], w.shape[1], scale,
+                                       w.data_ptr(), ld, w.shape[0], w.shape[1], scale,
                                        out.data_ptr(), out.stride(0), _DTYPES[w.dtype],
                                        _stream(w.device))
     if rc:
@@ -190,7 +194,7 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, ids, w, scale, padding):
         ctx.save_for_backward(ids)
         ctx.table, ctx.scale, ctx.padding = tuple(w.shape), scale, padding
-        return _embed_forward(ids, _rows(w), scale)
+        return _embed_forward(ids, w, scale)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -237,7 +241,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     ids = ids.contiguous()
     if torch.is_grad_enabled() and weight.requires_grad:
         return _Embedding.apply(ids, weight, float(scale), pad)
-    return _embed_forward(ids, _rows(weight), float(scale))
+    return _embed_forward(ids, weight, float(scale))
 
 
 class Embedding(torch.nn.Module):
@@ -267,16 +271,17 @@ class Embedding(torch.nn.Module):
 # ---------------------------------------------------------------------------
 # Attention over packed sequences
 # ---------------------------------------------------------------------------
-def _vectors(t: torch.Tensor) -> torch.Tensor:
+def _vectors(t: torch.Tensor, query: bool = False) -> torch.Tensor:
     """[tokens, heads, dim] as the kernels read it: adjacent dimensions, rows of whole
-    16-byte vectors on 16-byte boundaries, no two tokens in one place and strides that 31-bit offsets
-    reach.  ``t`` itself where it is that already (a view of a fused projection's output,
-    say), else a copy padded with zeros."""
+    16-byte vectors on 16-byte boundaries, no two tokens in one place and strides that 31-bit
+    offsets reach (of the heads for queries only: a key head's rows have a base of their own).
+    ``t`` itself where it is that already (a view of a fused projection's output, say), else
+    a copy padded with zeros."""
     n = 16 // t.element_size()
     d = t.shape[2]
     row, head, one = t.stride()
     if d % n == 0 and one == 1 and row % n == 0 and head % n == 0 and t.data_ptr() % 16 == 0 \
-            and d <= row <= 1 << 22 and head * t.shape[1] <= 1 << 28:
+            and d <= row <= 1 << 22 and (not query or head * t.shape[1] <= 1 << 28):
         return t
     if d % n == 0:
         return t.clone(memory_format=torch.contiguous_format)
@@ -308,7 +313,7 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, ptr, kv_ptr, causal, scale):
         d = q.shape[2]
-        q, k, v = _vectors(q), _vectors(k), _vectors(v)
+        q, k, v = _vectors(q, True), _vectors(k), _vectors(v)
         out, lse, low = _attn_forward(q, k, v, ptr, kv_ptr, causal, scale, True, True)
         ctx.save_for_backward(q, k, v, out, low, lse, ptr, kv_ptr)
         ctx.causal, ctx.scale, ctx.dim = causal, scale, d
@@ -322,7 +327,7 @@ class _PackedAttention(torch.autograd.Function):
         q, k, v, out, low, lse, ptr, kv_ptr = ctx.saved_tensors
         if g is None:
             return (None,) * 7
-        g = _vectors(g)
+        g = _vectors(g, True)
         nq, h, d = q.shape
         nk, hk = k.shape[:2]
         dev, dt, count = q.device, _DTYPES[q.dtype], ptr.numel() - 1
@@ -409,7 +414,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _PackedAttention.apply(q, k, v, ptr, kv_ptr, bool(causal), scale)
         return (out, lse) if return_lse else out
-    out, lse, _ = _attn_forward(_vectors(q), _vectors(k), _vectors(v), ptr, kv_ptr, bool(causal),
+    out, lse, _ = _attn_forward(_vectors(q, True), _vectors(k), _vectors(v), ptr, kv_ptr, bool(causal),
                                 scale, return_lse)
     out = out if out.shape[2] == d else out[..., :d].contiguous()
     return (out, lse) if return_lse else out

@@ -648,7 +648,7 @@ int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void*
  * causal: key j of a sequence is visible to its query i iff j <= i + (keys - queries).
  *   q        [nq, heads, dim], k, v [nk, kv_heads, dim]: GAT_F32 or GAT_BF16, token and head
  *            strides in elements; addresses and strides multiples of 16 bytes, token
- *            strides of dim to 2^22 elements, heads / kv_heads * head stride up to 2^28, dim a
+ *            strides of dim to 2^22 elements, heads / kv_heads * q's head stride up to 2^28, dim a
  *            multiple of 16 bytes of elements and <= GAT_PACKED_MAX_DIM (GAT_EUNSUPPORTED
  *            otherwise); heads a multiple of kv_heads
  *   ptr, kv_ptr  [count + 1] int64 if ptr64, else int32, ascending.  Boundaries outside

@@ -333,6 +333,20 @@ def test_embedding_shapes_strides_and_int32():
                what="expanded gradient")
 
 
+def test_embedding_of_broadcast_and_single_rows():
+    gat = ops()
+    torch.manual_seed(6)
+    row = torch.randn(12, device=DEV, requires_grad=True)
+    ids = torch.randint(0, 9, (70,), device=DEV)
+    g = torch.randn(70, 12, device=DEV)
+    y = gat.embedding(ids, row.expand(9, 12), 2.0)
+    drow, = torch.autograd.grad(y, row, g)
+    assert torch.equal(y, (row * 2.0).expand(70, 12))
+    close(drow, 2 * g.cpu().double().sum(0), 90 * U * 2 * g.cpu().double().abs().sum(0), "broadcast row")
+    one = torch.randn(12, 1, device=DEV).t()  # [1, 12], stride 1
+    embed_case(torch.zeros(70, dtype=torch.int64, device=DEV), one, g, what="one row")
+
+
 def test_embedding_padding_and_outside_ids():
     gat = ops()
     torch.manual_seed(4)

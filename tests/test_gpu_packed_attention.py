@@ -376,6 +376,25 @@ def test_long_cache_offsets():
     assert bool(((got.float() - want.float()).abs() <= 2 * (2 * h + tail * U) * mag.float() * (1 + h)).all())
 
 
+def test_caches_with_distant_heads():
+    """A head-major cache: each key head's rows far from the next one's, read in place."""
+    gap = (1 << 28) + 8
+    room = torch.empty(gap + 64 * 16, device=DEV, dtype=torch.bfloat16)
+    far = room.as_strided((50, 2, 16), (16, gap, 1))
+    k = torch.randn(50, 2, 16, device=DEV).bfloat16()
+    far.copy_(k)
+    q = torch.randn(50, 4, 16, device=DEV).bfloat16()
+    ptr = torch.tensor([0, 20, 50], dtype=torch.int32, device=DEV)
+    got = []
+    for kv in (k, far):
+        leaves = [x.detach().requires_grad_() for x in (q, kv)]
+        before = torch.cuda.memory_allocated()
+        y = attend(leaves[0], leaves[1], leaves[1], ptr, causal=True)
+        got.append([y, *torch.autograd.grad(y, leaves, q)])
+        assert torch.cuda.memory_allocated() - before < 1 << 24
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_refusals():
     q, k, v = tensors(8, 8, 4, 2, 16, torch.float32)
     p = torch.tensor([0, 8], device=DEV)
