@@ -409,6 +409,7 @@ __global__ __launch_bounds__(kEmbedBlock) void k_embed_own(Ids s, int n, const T
     const int rows = s.vocab - v0 < kOwnRows ? s.vocab - v0 : kOwnRows;
     const int c = (blockIdx.y * LPR + lane) * N;
     if (tid < kOwnRows) found[tid] = 0;
+    __syncthreads();  // no tokens: nothing below waits before found is read
     int total = 0;
     for (int t0 = 0; t0 < n; t0 += kEmbedBlock) {
         const int t = t0 + tid;

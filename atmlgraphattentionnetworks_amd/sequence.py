@@ -8,7 +8,7 @@ is no CPU path), float32, bfloat16 or float16 where an operator does not say oth
 float32 sums and statistics, one rounding at the end.  Work is enqueued on torch's
 current stream of the tensors' device, nothing synchronises the host, and every
 workspace comes from torch's allocator within the call, so calls can be captured in HIP
-graphs.  Results do not depend on timing: no kernel adds with atomics.
+graphs.  Results do not depend on timing: no kernel adds floats with atomics.
 
 When a step is captured in a graph, keep no autograd graph of an eager step on the same
 leaves alive (detach what is kept of the warm-up steps): its gradient accumulators

@@ -440,3 +440,17 @@ def test_modules_match_torch_state():
     a = gat.Embedding(11, 40, padding_idx=2)
     torch.manual_seed(8)
     assert torch.equal(a.weight, torch.nn.Embedding(11, 40, padding_idx=2).weight)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("cols", [3, 40, 600])
+def test_embedding_no_tokens_many_rows(cols, t):
+    """Between calls that leave other contents in a workgroup's shared memory."""
+    gat = ops()
+    w = torch.randn(5000, cols, device=DEV).to(t).requires_grad_()
+    ids = torch.zeros(1000, dtype=torch.int64, device=DEV)
+    for _ in range(20):
+        torch.autograd.grad(gat.embedding(ids, w), w, torch.ones(1000, cols, device=DEV, dtype=t))
+        y = gat.embedding(ids[:0], w)
+        dw, = torch.autograd.grad(y, w, torch.empty(0, cols, device=DEV, dtype=t))
+        assert not dw.any()
