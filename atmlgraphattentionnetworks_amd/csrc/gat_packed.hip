@@ -33,7 +33,7 @@
 // are few, softmax arithmetic and latency where heads are narrow and sequences short.
 // Measured: prompts of 300 to 6,000 tokens, 16 heads of 128 over 4, bf16, causal: 544 us (970
 // TFLOP/s); 8 sequences of 2,048 with the backward: 1,070 us; one query for each of 48
-// sequences of up to 8,192, 32 heads of 128 over 8: 162 us (4.5 TB/s); 512 graphs of 85 to 150
+// sequences of up to 8,192, 32 heads of 128 over 8: 164 us (4.4 TB/s); 512 graphs of 85 to 150
 // nodes, 8 heads of 8, float32, with the backward: 276 us.
 
 #include <climits>
@@ -502,7 +502,7 @@ constexpr float kRescale = 8.f;  // log2 of how far p may pass 1 before the sums
 // exp(s - m), sums of p and p v; m follows the maximum only when that has grown by over
 // 2^8, so most tiles skip the rescaling of the accumulators (p stays far inside float32
 // and keeps its relative precision in bf16).  p is rounded to v's type for the second
-// product, the sum l uses the unrounded p.
+// product (single waves: in two halves), the sum l uses the unrounded p.
 // ---------------------------------------------------------------------------
 template <typename T, int DP, int NW, int R>
 __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kFwd))) void k_attn_fwd(AttnArgs a) {
@@ -602,7 +602,11 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kFwd))) void k_a
                 s[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], c, -mc));
                 l += s[j][i];
             }
-            add_products<DP>(acc, lv + S::slab(ROWS * j), s[j]);
+            // Single waves wait for memory, not for products: what rounding p leaves goes in too
+            // (one query each of 48 sequences: y off by 1.66e-3 of its norm, its own rounding,
+            // for 2.2e-3; 164 us for 162).  Graphs of 85 to 150 nodes, 8 heads of 32: 73 us for
+            // 66, so not there.
+            add_products<DP, NW == 1>(acc, lv + S::slab(ROWS * j), s[j]);
             if (MASK && mend) {
                 unsigned seen = 0;
 #pragma unroll
