@@ -374,10 +374,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     ``[queries, heads]`` logarithm of each softmax sum (-inf where no key is seen; not
     differentiable).  Differentiable in ``q``, ``k`` and ``v``.  Scores, softmax sums and
     accumulators are float32; in bfloat16 the probabilities and the scores' gradients are
-    rounded to bfloat16 for the second matrix product (not where sequences have, on
-    average, 32 queries or fewer times the heads of a key head, and not for ``q``'s gradient
-    with ``dim`` up to 32).  Inputs may be strided views
-    (16-byte aligned rows are read in place, others are copied)."""
+    rounded to bfloat16 for the second matrix product (not where a sequence's queries
+    times the query heads of a key head are 32 or fewer on average, and not for ``q``'s
+    gradient with ``dim`` up to 32).  Inputs may be strided views (16-byte aligned rows are
+    read in place, others are copied)."""
     kinds = (torch.float32, torch.bfloat16)
     for name, t in (("q", q), ("k", k), ("v", v)):
         _need_tensor("packed_attention", name, t, kinds)
