@@ -26,6 +26,7 @@ import weakref
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, tuning
 from .graph import CSRGraph, get_csr, rotated_col, sched_csr
@@ -33,6 +34,14 @@ from .graph import CSRGraph, get_csr, rotated_col, sched_csr
 __all__ = ["GraphAttentionLayer", "GraphAttentionLayerActivationTest", "score_activation_code",
            "PackedParams", "pack_params", "gat_forward", "ForwardPlan", "wh_slices", "NodeTable",
            "alloc_table", "project", "edge_aggregate"]
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
+    """The kernels have a backward and no forward-mode derivative.  They read a dual
+    tensor's values only, so its tangent would be lost without a word."""
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
+           for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 class PackedParams:
@@ -683,6 +692,8 @@ class GraphAttentionLayer(torch.nn.Module):
         return pp
 
     def forward(self, x, edge_index):
+        if forward_ad._current_level >= 0:  # inside a dual_level(): elsewhere there are none
+            refuse_tangents("GraphAttentionLayer", x, *self.parameters())
         x = _check_x(x, self.input_channels)
         csr = get_csr(edge_index, x.size(0), x.device)
         p = float(self.dropout_val) if self.training else 0.0

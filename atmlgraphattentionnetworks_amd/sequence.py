@@ -5,10 +5,11 @@ backward, next to :class:`GraphAttentionLayer`.
 
 Common to all: tensors on one ROCm device (a CPU tensor raises ``RuntimeError``; there
 is no CPU path), float32, bfloat16 or float16 where an operator does not say otherwise,
-float32 sums and statistics, one rounding at the end.  Work is enqueued on torch's
-current stream of the tensors' device, nothing synchronises the host, and every
-workspace comes from torch's allocator within the call, so calls can be captured in HIP
-graphs.  Results do not depend on timing: no kernel adds floats with atomics.
+float32 sums and statistics, one rounding at the end.  Gradients are reverse mode only: a
+tensor that carries a forward-mode tangent raises ``NotImplementedError``.  Work is
+enqueued on torch's current stream of the tensors' device, nothing synchronises the host,
+and every workspace comes from torch's allocator within the call, so calls can be captured
+in HIP graphs.  Results do not depend on timing: no kernel adds floats with atomics.
 
 When a step is captured in a graph, keep no autograd graph of an eager step on the same
 leaves alive (detach what is kept of the warm-up steps): its gradient accumulators
@@ -20,8 +21,10 @@ import contextlib
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
+from .layer import refuse_tangents
 
 __all__ = ["layer_norm", "embedding", "packed_attention", "LayerNorm", "Embedding"]
 
@@ -42,6 +45,8 @@ def _stream(device: torch.device) -> int:
 def _need_tensor(what: str, name: str, t, dtypes=_DTYPES) -> torch.Tensor:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: {name} must be a torch.Tensor, got {type(t).__name__}")
+    if forward_ad._current_level >= 0:  # inside a dual_level(): elsewhere there are none
+        refuse_tangents(what, t)
     if not t.is_cuda:
         raise RuntimeError(f"{what} needs ROCm device tensors ({name} is on {t.device}); "
                            "there is no CPU path")
