@@ -44,6 +44,15 @@ def refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
         raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
+def refuse_recording(what: str, jit: bool = False) -> None:
+    """What records torch's operations does not see the library write into its outputs: a
+    recorded call would give whatever the memory held.  ``jit``: the caller has no form that
+    ``torch.jit.trace`` can keep either (an autograd function is kept as a whole)."""
+    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None or \
+            (jit and torch._C._is_tracing()):
+        raise RuntimeError(f"{what} cannot be recorded: its kernels are outside torch's operators")
+
+
 class PackedParams:
     """Device buffers derived from the per-head ``Linear`` parameters (never
     stored in the state_dict; rebuilt when any parameter's version moves)."""
@@ -694,6 +703,7 @@ class GraphAttentionLayer(torch.nn.Module):
     def forward(self, x, edge_index):
         if forward_ad._current_level >= 0:  # inside a dual_level(): elsewhere there are none
             refuse_tangents("GraphAttentionLayer", x, *self.parameters())
+        refuse_recording("GraphAttentionLayer")
         x = _check_x(x, self.input_channels)
         csr = get_csr(edge_index, x.size(0), x.device)
         p = float(self.dropout_val) if self.training else 0.0
@@ -706,6 +716,7 @@ class GraphAttentionLayer(torch.nn.Module):
             from .training import gat_train_forward, next_seed_slot
             slot = next_seed_slot(self, x.device) if p > 0.0 else None
             return gat_train_forward(self, x, csr, p, 0, act, act_param, seed_slot=slot)
+        refuse_recording("GraphAttentionLayer without gradients", jit=True)
         return self._eval_forward(x, csr, act_param)
 
     def _eval_forward(self, x: torch.Tensor, csr: CSRGraph, slope: float) -> torch.Tensor:

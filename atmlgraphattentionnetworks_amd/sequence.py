@@ -6,10 +6,11 @@ backward, next to :class:`GraphAttentionLayer`.
 Common to all: tensors on one ROCm device (a CPU tensor raises ``RuntimeError``; there
 is no CPU path), float32, bfloat16 or float16 where an operator does not say otherwise,
 float32 sums and statistics, one rounding at the end.  Gradients are reverse mode only: a
-tensor that carries a forward-mode tangent raises ``NotImplementedError``.  Work is
-enqueued on torch's current stream of the tensors' device, nothing synchronises the host,
-and every workspace comes from torch's allocator within the call, so calls can be captured
-in HIP graphs.  Results do not depend on timing: no kernel adds floats with atomics.
+tensor that carries a forward-mode tangent raises ``NotImplementedError``.
+``torch.jit.trace`` keeps a call as one opaque function; ``make_fx`` could not, and is
+refused (``RuntimeError``).  Work is enqueued on torch's current stream of the tensors'
+device, nothing synchronises the host, and every workspace comes from torch's allocator
+within the call, so calls can be captured in HIP graphs.  Results do not depend on timing: no kernel adds floats with atomics.
 
 When a step is captured in a graph, keep no autograd graph of an eager step on the same
 leaves alive (detach what is kept of the warm-up steps): its gradient accumulators
@@ -24,7 +25,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
-from .layer import refuse_tangents
+from .layer import refuse_recording, refuse_tangents
 
 __all__ = ["layer_norm", "embedding", "packed_attention", "LayerNorm", "Embedding"]
 
@@ -69,6 +70,17 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
         return t
     t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _as_function(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call goes through its autograd function: where a gradient may be asked for,
+    and under ``torch.jit.trace``, which keeps a function as one call (of a library call it
+    would keep the empty output)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return torch._C._is_tracing()
 
 
 def _ptr(t: Optional[torch.Tensor]) -> int:
@@ -133,6 +145,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     Differentiable in all three; the gradients of ``weight`` and ``bias`` are summed
     over the rows in float32 in a fixed order.  Up to 16,384 columns (16,377 where the
     rows do not all start on 16-byte boundaries; float32: 16,381)."""
+    refuse_recording("layer_norm")
     _need_tensor("layer_norm", "x", x)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"layer_norm: x needs a last dimension of at least 1, got {tuple(x.shape)}")
@@ -147,8 +160,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     if x.numel() // x.shape[-1] > 0x7FFFFFFF:
         raise ValueError("layer_norm: at most 2^31 - 1 rows")
     w, b = (None if p is None else p.contiguous() for p in (weight, bias))
-    if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)
-                                    or (b is not None and b.requires_grad)):
+    if _as_function(x, w, b):
         return _LayerNorm.apply(x, w, b, float(eps))
     return _norm_forward(_rows(x), w, b, float(eps), None).view(x.shape)
 
@@ -229,6 +241,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
 
     An id outside ``[0, vocab)`` gives a row of NaN and takes no gradient: checking on the
     host would cost a synchronisation per call.  At most 2^30 ids and 2^30 table rows."""
+    refuse_recording("embedding")
     _need_tensor("embedding", "weight", weight)
     _need_tensor("embedding", "ids", ids, (torch.int64, torch.int32))
     _need_like("embedding", "ids", ids, weight, dtype=False)
@@ -244,7 +257,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
             raise ValueError(f"embedding: padding_idx {padding_idx} is outside a table of {v}")
         pad = int(padding_idx) % v
     ids = ids.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if _as_function(weight):
         return _Embedding.apply(ids, weight, float(scale), pad)
     return _embed_forward(ids, weight, float(scale))
 
@@ -383,6 +396,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     times the query heads of a key head are 32 or fewer on average, and not for ``q``'s
     gradient with ``dim`` up to 32).  Inputs may be strided views (16-byte aligned rows are
     read in place, others are copied)."""
+    refuse_recording("packed_attention")
     kinds = (torch.float32, torch.bfloat16)
     for name, t in (("q", q), ("k", k), ("v", v)):
         _need_tensor("packed_attention", name, t, kinds)
@@ -417,7 +431,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
         ptr, kv_ptr = ptr.long(), kv_ptr.long()
     ptr, kv_ptr = ptr.contiguous(), kv_ptr.contiguous()
     scale = float(d) ** -0.5 if scale is None else float(scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _as_function(q, k, v):
         out, lse = _PackedAttention.apply(q, k, v, ptr, kv_ptr, bool(causal), scale)
         return (out, lse) if return_lse else out
     out, lse, _ = _attn_forward(_vectors(q, True), _vectors(k), _vectors(v), ptr, kv_ptr, bool(causal),

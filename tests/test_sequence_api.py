@@ -155,3 +155,45 @@ def test_forward_mode_tangents_are_refused():
                     call(dual)
             with pytest.raises(Exception, match="no CPU path|ROCm"):  # without one: as ever
                 call(at)
+
+
+def test_recording_by_make_fx_is_refused():
+    """It sees torch's operators only: the recorded call would be an empty tensor."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    import atmlgraphattentionnetworks_amd as gat
+    x, q = torch.randn(4, 8), torch.randn(4, 2, 8)
+    ids, ptr = torch.zeros(3, dtype=torch.int64), torch.tensor([0, 4])
+    layer, edges = gat.GraphAttentionLayer(8, 4), torch.zeros(2, 0, dtype=torch.int64)
+    for call, at in ((lambda t: gat.layer_norm(t), x), (lambda t: gat.embedding(ids, t), x),
+                     (lambda t: gat.packed_attention(t, q, q, ptr), q), (lambda t: layer(t, edges), x)):
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            make_fx(call)(at)
+
+
+def test_tracing_keeps_the_calls_as_functions(monkeypatch):
+    """torch.jit.trace without gradients: the function is kept, not the output that the
+    library fills behind its back.  (Here with the library's part replaced.)"""
+    import atmlgraphattentionnetworks_amd as gat
+    from atmlgraphattentionnetworks_amd import sequence
+    monkeypatch.setattr(sequence, "_need_tensor", lambda what, name, t, dtypes=None: t)
+
+    def fill(to, value):  # as the library does: by address
+        ctypes.memmove(to.data_ptr(), value.contiguous().data_ptr(), to.numel() * to.element_size())
+        return to
+    monkeypatch.setattr(sequence, "_norm_forward",
+                        lambda x, w, b, eps, stats: fill(torch.empty(x.shape), x * 2))
+    monkeypatch.setattr(sequence, "_embed_forward",
+                        lambda ids, w, scale: fill(torch.empty(*ids.shape, w.shape[1]), w[ids] * scale))
+    monkeypatch.setattr(sequence, "_attn_forward",
+                        lambda q, k, v, *a, **kw: (fill(torch.empty(q.shape), q + k), torch.zeros(4, 2), None))
+    ids, ptr = torch.tensor([1, 0, 3]), torch.tensor([0, 4])
+    x, q, k = torch.randn(4, 8), torch.randn(4, 2, 8), torch.randn(4, 2, 8)
+    with torch.no_grad():
+        for call, at in ((lambda t: gat.layer_norm(t), x), (lambda t: gat.embedding(ids, t, 3.0), x),
+                         (lambda t: gat.packed_attention(t, k, k, ptr), q)):
+            traced = torch.jit.trace(call, (at,), check_trace=False)
+            for other in (at, at + 1, torch.randn_like(at)):
+                want, filler = call(other), [torch.full((64,), 7.0) for _ in range(64)]
+                del filler
+                assert torch.equal(traced(other), want)
