@@ -935,6 +935,14 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_a
                         a.dim, mine && a.scale != 0.f, a.scale < 0.f);
     load_columns<T, DP>(vcol, static_cast<const T*>(a.v.p) + tok * a.v.row + (long long)kh * a.v.head,
                         a.dim, mine, false);
+    // Rows behind the last arrive as zeros and have p = exp(0 - inf) = 0, but zero times a key's
+    // infinity is NaN: the last tile of a wave with such a key is masked.
+    float zero = 0.f;
+#pragma unroll
+    for (int i = 0; i < S::STEPS; ++i)
+#pragma unroll
+        for (int e = 0; e < S::FN; ++e) zero = fmaf((float)kcol[i][e], 0.f, fmaf((float)vcol[i][e], 0.f, zero));
+    const bool odd = __any(zero != 0.f);
     const T* qb = static_cast<const T*>(a.q.p) + (long long)q0 * a.q.row +
                   (long long)kh * a.group * a.q.head;
     const T* gb = static_cast<const T*>(a.g.p) + (long long)q0 * a.g.row +
@@ -975,7 +983,7 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_a
         constexpr bool MASK = decltype(masks)::value;
         schedule<T, MASK>();
         f32x16 p[R], ds[R];
-        const int hidden = beg - n0 - 4 * part;
+        const int hidden = beg - n0 - 4 * part, behind = rows - n0 - 4 * part;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             p[j] = scores<T, DP>(lq + S::slab(ROWS * j), kcol);
@@ -992,7 +1000,8 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_a
                     const int i = 4 * b + e;
                     p[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j][i], c, -l4[e]));
                     ds[j][i] = p[j][i] * (ds[j][i] - d4[e]);
-                    if (MASK && ROWS * j + S::row_of(i, 0) < hidden) p[j][i] = ds[j][i] = 0.f;
+                    const int r = ROWS * j + S::row_of(i, 0);
+                    if (MASK && (r < hidden || r >= behind)) p[j][i] = ds[j][i] = 0.f;
                 }
             }
         if (MASK && mend) {
@@ -1044,9 +1053,14 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_a
         if (n0 + BN > beg_first || mend)
             tile(n0, at, at + SLAB, sums + turn * 2 * BN, std::true_type(), mend);
     }
-    for (; n0 < to; n0 += BN, turn ^= 1) {
+    const int whole = odd ? to - BN + 1 : to;
+    for (; n0 < whole; n0 += BN, turn ^= 1) {
         T* at = arrive();
         tile(n0, at, at + SLAB, sums + turn * 2 * BN, std::false_type(), false);
+    }
+    if (n0 < to) {
+        T* at = arrive();
+        tile(n0, at, at + SLAB, sums + turn * 2 * BN, std::true_type(), false);
     }
     if (!mine) return;
     if (a.splits > 1) {
