@@ -1,0 +1,50 @@
+"""layer_norm and embedding where a group of lanes walks several rows; the float64 definitions
+and tolerances are those of test_gpu_norm_embedding."""
+import pytest
+import torch
+
+from test_gpu_norm_embedding import DEV, TYPES, embed_case, norm_case
+
+pytestmark = pytest.mark.gpu
+
+
+# a launch has at most 256 x (resident workgroups a CU) workgroups of 256 / lanes rows each,
+# the backward at most 1024 workgroups: more rows than that for every number of lanes
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("rows,cols", [(140000, 31), (90000, 63), (70003, 120), (40001, 300), (20011, 515),
+                                       (9001, 1433), (8200, 2049), (4700, 4099), (2500, 8191)])
+def test_norm_groups_of_several_rows(rows, cols, t):
+    torch.manual_seed(cols)
+    x = (torch.randn(rows, cols, device=DEV) * 1.5 + 0.3).to(t)
+    w, b = ((torch.randn(cols, device=DEV) * 0.2 + k).to(t) for k in (1.0, 0.0))
+    norm_case(x, w, b, torch.randn(rows, cols, device=DEV).to(t), what=f"{rows} {cols} {t}")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("rows,cols", [(90000, 61), (9100, 1029)])
+def test_norm_several_rows_of_a_view(rows, cols, t):
+    torch.manual_seed(rows)
+    big = torch.randn(rows, cols + 10, device=DEV).to(t)
+    w, b = torch.rand(2, cols, device=DEV).to(t)
+    g = torch.randn(rows, cols + 3, device=DEV).to(t)[:, 3:]
+    norm_case(big[:, 5:5 + cols], w, b, g, what=f"{rows} {cols} {t}")
+
+
+# tables with enough rows that a group takes four of them, for each number of lanes, with
+# some ids over and most under a piece
+@pytest.mark.parametrize("vocab,cols,t", [(300000, 20, torch.float32), (150001, 60, torch.float32),
+                                          (70001, 128, torch.float32), (40000, 250, torch.float32),
+                                          (20000, 600, torch.float32), (270000, 64, torch.bfloat16),
+                                          (140000, 100, torch.float16), (66000, 256, torch.bfloat16),
+                                          (33001, 512, torch.bfloat16), (17001, 1000, torch.float16)],
+                         ids=str)
+def test_embedding_gradient_of_large_tables(vocab, cols, t):
+    torch.manual_seed(vocab)
+    tokens = 20000
+    ids = torch.randint(0, vocab, (tokens,), device=DEV)
+    ids[:3000] = vocab // 3
+    ids[3000:3040] = vocab - 1
+    ids[3040:6000] = torch.randint(vocab // 2, vocab // 2 + 300, (2960,), device=DEV)
+    ids = ids[torch.randperm(tokens, device=DEV)]
+    embed_case(ids, torch.randn(vocab, cols, device=DEV).to(t), torch.randn(tokens, cols, device=DEV).to(t),
+               1.7, padding=5, what=f"{vocab} {cols} {t}")
