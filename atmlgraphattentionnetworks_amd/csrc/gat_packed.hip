@@ -397,12 +397,17 @@ __device__ __forceinline__ void add_non_finite(typename Shape<T, DP>::Acc* acc, 
 // rows behind it and dimensions behind `dim` arrive as zeros.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+// (m0 is on the clobber list so that no value of the compiler's own stays in it across the
+// statement; the compiler warns that it would not save m0, which nothing here asks of it)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned offset, unsigned lds) {
     // m0 holds the LDS address; the nops cover scalar operands that a vector instruction wrote
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds),
                  "v"(offset), "s"(buffer)
-                 : "memory");
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 __device__ __forceinline__ i32x4 make_buffer(const void* p, unsigned bytes) {

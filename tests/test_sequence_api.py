@@ -197,3 +197,19 @@ def test_tracing_keeps_the_calls_as_functions(monkeypatch):
                 want, filler = call(other), [torch.full((64,), 7.0) for _ in range(64)]
                 del filler
                 assert torch.equal(traced(other), want)
+
+
+def test_inline_assembly_names_the_m0_it_writes():
+    """Else the compiler may keep a value of its own in m0 across the statement."""
+    import glob
+    import os
+    import re
+
+    import atmlgraphattentionnetworks_amd as gat
+    found = 0
+    for path in glob.glob(os.path.join(os.path.dirname(gat.__file__), "csrc", "*")):
+        for statement in re.findall(r"\basm\b.*?\);", open(path).read(), re.S):
+            if re.search(r"s_\w+ m0", statement):
+                found += 1
+                assert re.search(r':[^:]*"m0"[^:]*\)', statement), (path, statement)
+    assert found > 0
