@@ -161,7 +161,10 @@ __global__ __launch_bounds__(kNormBlock, (NV == 1 ? 6 : 1)) void k_norm_fwd(Norm
         }
         if (AHEAD && row + groups < p.rows) load_row(next, row + groups);
         row_sum2<LPR>(s, unused, red[turn]);
-        const float mean = s * inv;
+        // Divided, not times 1 / cols: the product's rounding, which the compiler may also leave
+        // out of v - mean, would give rows of one value deviations from their mean, which
+        // 1 / sqrt(eps) enlarges (3 columns of 1000: z = 9e-3 for 0).
+        const float mean = s / (float)p.cols;
         float q = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)

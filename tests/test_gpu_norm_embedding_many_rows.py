@@ -1,9 +1,9 @@
-"""layer_norm and embedding where a group of lanes walks several rows; the float64 definitions
-and tolerances are those of test_gpu_norm_embedding."""
+"""layer_norm and embedding where a group of lanes walks several rows, and layer_norm of
+constant rows; the float64 definitions and tolerances are those of test_gpu_norm_embedding."""
 import pytest
 import torch
 
-from test_gpu_norm_embedding import DEV, TYPES, embed_case, norm_case
+from test_gpu_norm_embedding import DEV, TYPES, U, close, embed_case, half_step, norm_case, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -28,6 +28,25 @@ def test_norm_several_rows_of_a_view(rows, cols, t):
     w, b = torch.rand(2, cols, device=DEV).to(t)
     g = torch.randn(rows, cols + 3, device=DEV).to(t)[:, 3:]
     norm_case(big[:, 5:5 + cols], w, b, g, what=f"{rows} {cols} {t}")
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_norm_of_constant_rows_is_the_bias(t):
+    """The mean of equal values whose sum float32 holds is that value, so nothing is left for
+    1 / sqrt(eps) to enlarge."""
+    gat = ops()
+    for cols in list(range(1, 140)) + [255, 257, 511, 1000, 1433, 2049, 5001]:
+        x = torch.tensor([[2.5], [1000.0], [-768.0], [0.0]], device=DEV).expand(4, cols).to(t)
+        w, b = torch.rand(2, cols, device=DEV).to(t)
+        leaf = x.detach().requires_grad_()
+        y = gat.layer_norm(leaf, w, b)
+        assert torch.equal(y, b.expand(4, cols)), cols
+        g = torch.randn(4, cols, device=DEV).to(t)
+        dx, = torch.autograd.grad(y, leaf, g)
+        h = (g.double() * w.double()).cpu()
+        r = (1.0 / torch.tensor(1e-5, dtype=torch.float32).double() ** 0.5)
+        want = r * (h - h.mean(1, keepdim=True))
+        e = r * ((cols + 16) * U * h.abs().mean(1, keepdim=True) + 8 * U * h.abs()) + 8 * U * want.abs()
+        close(dx, want, e + half_step(t) * (want.abs() + e) + torch.finfo(t).tiny, f"{cols} dx")
 
 
 # tables with enough rows that a group takes four of them, for each number of lanes, with
