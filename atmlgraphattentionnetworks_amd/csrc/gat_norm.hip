@@ -238,17 +238,18 @@ __global__ __launch_bounds__(kNormBlock) void k_norm_bwd(NormArgs p) {
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                // outside the row g and w are 0, so nothing is added there
-                const float z = ((float)v[i][e] - m) * rs;
+                // outside the row g and w are 0, so nothing is added there; d is finite where z
+                // of a large mean is not, whose product with 0 would reach the whole row
+                const float d = (float)v[i][e] - m;
                 const float h = (float)g[i][e] * (float)w[i][e];
                 sh += h;
-                shz += h * z;
-                dw[i][e] += (float)g[i][e] * z;
+                shz += h * d;
+                dw[i][e] += (float)g[i][e] * (d * rs);
                 db[i][e] += (float)g[i][e];
             }
         row_sum2<LPR>(sh, shz, red[turn]);
         sh *= inv;
-        shz *= inv;
+        shz *= rs * inv;
         if (p.out != nullptr) {
             T* dr = static_cast<T*>(p.out) + row * p.ld_out;
 #pragma unroll
@@ -506,8 +507,8 @@ int gat_layer_norm_backward(const void* g, long long ld_g, const void* x, long l
         a.rows = rows;
         a.cols = cols;
         a.inner_x = inner_rows(rows, ld_x, 1, dtype);
-    a.whole_g = lies_as(x, ld_x, g, ld_g, dtype);
-    a.inner_g = inner_rows(rows, ld_g, a.whole_g, dtype);
+        a.whole_g = lies_as(x, ld_x, g, ld_g, dtype);
+        a.inner_g = inner_rows(rows, ld_g, a.whole_g, dtype);
         a.whole_out = dx != nullptr && lies_as(x, ld_x, dx, ld_dx, dtype);
         const hipError_t e = norm_by_type<true>(sh, a, dtype, &parts, s);
         if (e != hipSuccess) return status_of(e);

@@ -3,7 +3,8 @@ constant rows; the float64 definitions and tolerances are those of test_gpu_norm
 import pytest
 import torch
 
-from test_gpu_norm_embedding import DEV, TYPES, U, close, embed_case, half_step, norm_case, ops
+from test_gpu_norm_embedding import (DEV, TYPES, U, close, embed_case, half_step, norm_case,
+                                     norm_reference, ops)
 
 pytestmark = pytest.mark.gpu
 
@@ -47,6 +48,40 @@ def test_norm_of_constant_rows_is_the_bias(t):
         want = r * (h - h.mean(1, keepdim=True))
         e = r * ((cols + 16) * U * h.abs().mean(1, keepdim=True) + 8 * U * h.abs()) + 8 * U * want.abs()
         close(dx, want, e + half_step(t) * (want.abs() + e) + torch.finfo(t).tiny, f"{cols} dx")
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("cols", [7, 20, 64, 100, 300, 1030])
+def test_norm_rows_of_huge_constants(cols, t):
+    """Lanes outside a row have no part in it, whatever its mean: values whose product with
+    1 / sqrt(eps) passes float32's range."""
+    gat = ops()
+    c = 2.0 ** 117  # cols times this is finite and their mean exact: deviations of 0
+    x = torch.full((5, cols), c, device=DEV, dtype=t)
+    x[1], x[3] = -c, torch.randn(cols, device=DEV).to(t)
+    w, b = torch.rand(2, cols, device=DEV).to(t)
+    g = torch.randn(5, cols, device=DEV).to(t)
+    eps = 1e-12
+    leaves = [p.detach().requires_grad_() for p in (x, w, b)]
+    y = gat.layer_norm(*leaves, eps)
+    got = [y, *torch.autograd.grad(y, leaves, g)]
+    want = norm_reference(x.cpu(), w.cpu(), b.cpu(), eps, g.cpu())
+    # of a constant row z = 0 exactly: dx = r (h - mean(h)), y = b
+    h = (g.double() * w.double()).cpu()
+    r = 1.0 / (torch.tensor(eps, dtype=torch.float32).double() ** 0.5)
+    for i in (0, 1, 2, 4):
+        assert torch.equal(y[i], leaves[2].detach())
+        dx = r * (h[i] - h[i].mean())
+        bound = r * ((cols + 16) * U * h[i].abs().mean() + 8 * U * h[i].abs()) + 8 * U * dx.abs()
+        close(got[1][i], dx, bound + half_step(t) * (dx.abs() + bound), f"{cols} dx {i}")
+    v, e = (p[3] for p in want[1])
+    close(got[1][3], v, e + half_step(t) * (v.abs() + e), "dx of the ordinary row")
+    db = g.double().sum(0).cpu()
+    close(got[3], db, 45 * U * g.double().abs().sum(0).cpu() + half_step(t) * db.abs() * (1 + 45 * U), "db")
+    x3, w1, b0 = x[3:4].cpu(), torch.ones(cols).to(t), torch.zeros(cols).to(t)
+    (z, ez), _, _, _ = norm_reference(x3, w1, b0, eps, g[3:4].cpu())
+    dw, e = (g[3].cpu().double() * z[0]), g[3].cpu().double().abs() * (ez[0] + 45 * U * z[0].abs())
+    close(got[2], dw, e + half_step(t) * (dw.abs() + e), "dw: the ordinary row's share alone")
 
 
 # tables with enough rows that a group takes four of them, for each number of lanes, with
