@@ -493,6 +493,12 @@ inline int embed_lanes(int cols, int dtype) {
     return vecs <= 8 ? 8 : vecs <= 16 ? 16 : vecs <= 32 ? 32 : 64;
 }
 
+// A launch has at most 65535 slabs of 64 vectors for a row; columns beyond them would also
+// wrap the lookup's int steps.
+inline bool cols_fit(int cols, int dtype) {
+    return cols > 0 && cols <= 65535 * kWave * (16 / (int)dtype_size(dtype));
+}
+
 inline bool rows_whole(const void* p, long long ld, int dtype) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((uintptr_t)ld * dtype_size(dtype) & 15) == 0;
 }
@@ -637,7 +643,7 @@ extern "C" {
 int gat_embedding(const void* ids, int ids64, long long tokens, const void* w, long long ld_w,
                   int vocab, int cols, float scale, void* out, long long ld_out, int dtype,
                   void* stream) {
-    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || cols <= 0 || !known_dtype(dtype) ||
+    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || !known_dtype(dtype) || !cols_fit(cols, dtype) ||
         ld_w < cols || ld_out < cols || !ids_fit(ids, ids64, tokens))
         return GAT_EINVAL;
     if (tokens == 0) return GAT_OK;
@@ -664,8 +670,8 @@ int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void*
                        int vocab, int cols, float scale, long long padding, void* dw,
                        long long ld_dw, void* workspace, size_t workspace_bytes, int dtype,
                        void* stream) {
-    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || vocab > kMaxTokens || cols <= 0 || !known_dtype(dtype) ||
-        ld_g < 0 || ld_dw < cols || dw == nullptr || !element_aligned(dw, dtype) ||
+    if (tokens < 0 || tokens > kMaxTokens || vocab <= 0 || vocab > kMaxTokens || !known_dtype(dtype) ||
+        !cols_fit(cols, dtype) || ld_g < 0 || ld_dw < cols || dw == nullptr || !element_aligned(dw, dtype) ||
         !ids_fit(ids, ids64, tokens) ||
         (tokens > 0 && (g == nullptr || !element_aligned(g, dtype))))
         return GAT_EINVAL;

@@ -90,6 +90,11 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 # ---------------------------------------------------------------------------
 # Layer norm
 # ---------------------------------------------------------------------------
+def _too_wide(cols: int) -> ValueError:
+    return ValueError(f"layer_norm: {cols} columns are more than a row may have (16384, or 16377 "
+                      "/ float32 16381 where rows are not 16-byte aligned)")
+
+
 def _norm_forward(x2, w, b, eps, stats):
     lib = _lib.load()
     y = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device)
@@ -98,8 +103,7 @@ def _norm_forward(x2, w, b, eps, stats):
                                 _ptr(b), eps, y.data_ptr(), y.stride(0), _ptr(stats),
                                 _DTYPES[x2.dtype], _stream(x2.device))
     if rc == _lib.GAT_EUNSUPPORTED:
-        raise ValueError(f"layer_norm: {x2.shape[1]} columns are more than a row may have "
-                         "(16384, or 16377 / float32 16381 where rows are not 16-byte aligned)")
+        raise _too_wide(x2.shape[1])
     if rc:
         _lib.check(rc, "gat_layer_norm")
     return y
@@ -149,6 +153,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     _need_tensor("layer_norm", "x", x)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"layer_norm: x needs a last dimension of at least 1, got {tuple(x.shape)}")
+    if x.shape[-1] > 16384:
+        raise _too_wide(x.shape[-1])
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None:
             _need_like("layer_norm", name, _need_tensor("layer_norm", name, p), x)
@@ -240,7 +246,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     rows are read like any other.
 
     An id outside ``[0, vocab)`` gives a row of NaN and takes no gradient: checking on the
-    host would cost a synchronisation per call.  At most 2^30 ids and 2^30 table rows."""
+    host would cost a synchronisation per call.  At most 2^30 ids, 2^30 table rows and
+    65,535 x 64 16-byte vectors a row (16.8 million float32 columns)."""
     refuse_recording("embedding")
     _need_tensor("embedding", "weight", weight)
     _need_tensor("embedding", "ids", ids, (torch.int64, torch.int32))
@@ -251,6 +258,9 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     v = weight.shape[0]
     if v > 1 << 30 or ids.numel() > 1 << 30:
         raise ValueError("embedding: at most 2^30 table rows and 2^30 ids")
+    most = 65535 * 64 * (16 // weight.element_size())
+    if weight.shape[1] > most:
+        raise ValueError(f"embedding: {weight.shape[1]} columns are more than a row may have ({most})")
     pad = -1
     if padding_idx is not None:
         if not -v <= padding_idx < v:
@@ -306,6 +316,14 @@ def _vectors(t: torch.Tensor, query: bool = False) -> torch.Tensor:
     return torch.nn.functional.pad(t, (0, -d % n))
 
 
+def _attn_check(rc: int, count: int) -> None:
+    if rc == _lib.GAT_EUNSUPPORTED:  # what the entry does not refuse itself
+        raise ValueError(f"packed_attention: {count} sequences are more than one launch holds "
+                         "(2^32 lanes: 64 to 256 for each sequence and 32 rows)")
+    if rc:
+        _lib.check(rc, "gat_packed_attention")
+
+
 def _attn_forward(q, k, v, ptr, kv_ptr, causal, scale, want_lse, want_low=False):
     """``q``, ``k``, ``v`` as :func:`_vectors` gives them."""
     nq, h, d = q.shape
@@ -322,8 +340,7 @@ def _attn_forward(q, k, v, ptr, kv_ptr, causal, scale, want_lse, want_low=False)
             v.data_ptr(), v.stride(0), v.stride(1), ptr.data_ptr(), kv_ptr.data_ptr(),
             int(ptr.dtype == torch.int64), count, nq, nk, h, hk, d, scale, int(causal),
             out.data_ptr(), _ptr(low), _ptr(lse), _ptr(ws), size, dt, _stream(dev))
-    if rc:
-        _lib.check(rc, "gat_packed_attention")
+    _attn_check(rc, count)
     return out, lse, low
 
 
@@ -361,8 +378,7 @@ class _PackedAttention(torch.autograd.Function):
                 int(ptr.dtype == torch.int64), count, nq, nk, h, hk, d, ctx.scale,
                 int(ctx.causal), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), size,
                 dt, _stream(dev))
-        if rc:
-            _lib.check(rc, "gat_packed_attention_backward")
+        _attn_check(rc, count)
         if ctx.dim != d:
             dq, dk, dv = (t[..., :ctx.dim] for t in (dq, dk, dv))
         return dq, dk, dv, None, None, None, None
@@ -375,7 +391,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
 
     ``q`` is ``[queries, heads, dim]``, ``k`` and ``v`` ``[keys, kv_heads, dim]`` (float32 or
     bfloat16; ``heads`` a multiple of ``kv_heads``, query head ``h`` reads key head
-    ``h // (heads // kv_heads)``; ``dim`` up to 128).  Sequence ``b`` has the queries
+    ``h // (heads // kv_heads)``; ``dim`` up to 128, ``heads * dim`` up to 2^22).  Sequence ``b`` has the queries
     ``ptr[b]:ptr[b + 1]`` and the keys ``kv_ptr[b]:kv_ptr[b + 1]``; ``ptr`` is an ascending
     int32 or int64 device tensor of ``count + 1`` offsets (a batch of graphs:
     ``GraphData.ptr()``), ``kv_ptr`` defaults to it.  One query per sequence (a readout
@@ -424,6 +440,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     if not 1 <= d <= 128 or hk > 65535:
         raise ValueError(f"packed_attention: dim must be 1 to 128 and kv_heads at most 65535, "
                          f"got {d} and {hk}")
+    n = 16 // q.element_size()
+    if h * (-(-d // n) * n) > 1 << 22:
+        raise ValueError(f"packed_attention: heads * dim must be at most 2^22 (dim in whole 16-byte "
+                         f"vectors), got {h} * {d}")
     if max(nq * (h // hk), nk) >= 1 << 30:
         raise ValueError("packed_attention: queries * heads / kv_heads and keys must be "
                          "below 2^30")

@@ -619,6 +619,7 @@ int gat_layer_norm_backward(const void* g, long long ld_g, const void* x, long l
  *   ids    int64 if ids64, else int32.  A row whose id is outside [0, vocab) is filled
  *          with NaN: nothing outside the table is read, and the error shows.
  *   w      [vocab, cols], row stride ld_w >= cols;  out [tokens, cols]
+ *   cols   at most 65535 * 256 in float32, 65535 * 512 in the 2-byte types (GAT_EINVAL)
  */
 int gat_embedding(const void* ids, int ids64, long long tokens, const void* w, long long ld_w,
                   int vocab, int cols, float scale, void* out, long long ld_out, int dtype,
@@ -632,7 +633,7 @@ int gat_embedding_grad_workspace_size(long long tokens, int vocab, int cols, siz
  * [0, vocab); rows without a token are zeros.  Deterministic.
  *   padding  an id whose tokens take no gradient, or -1.  Ids outside [0, vocab) take
  *            none either.
- *   vocab    at most 2^30
+ *   vocab    at most 2^30; cols as for gat_embedding
  *   workspace  16-byte aligned; none where the size is 0 (few tokens)
  */
 int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void* g, long long ld_g,
@@ -650,7 +651,7 @@ int gat_embedding_grad(const void* ids, int ids64, long long tokens, const void*
  *            strides in elements; addresses and strides multiples of 16 bytes, token
  *            strides of dim to 2^22 elements, heads / kv_heads * q's head stride up to 2^28, dim a
  *            multiple of 16 bytes of elements and <= GAT_PACKED_MAX_DIM (GAT_EUNSUPPORTED
- *            otherwise); heads a multiple of kv_heads
+ *            otherwise); heads a multiple of kv_heads, heads * dim up to 2^22
  *   ptr, kv_ptr  [count + 1] int64 if ptr64, else int32, ascending.  Boundaries outside
  *            [0, nq] / [0, nk] are held to it: nothing outside the tensors is touched.
  *   out      [nq, heads, dim] contiguous.  Queries that see no key (an empty sequence, causal

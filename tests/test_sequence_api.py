@@ -213,3 +213,41 @@ def test_inline_assembly_names_the_m0_it_writes():
                 found += 1
                 assert re.search(r':[^:]*"m0"[^:]*\)', statement), (path, statement)
     assert found > 0
+
+
+def test_sizes_beyond_the_kernels_are_refused(monkeypatch):
+    """Sizes that the library's int arguments would wrap around, and those that its launches
+    cannot hold, are a ValueError that names the limit.  (Tensors of no memory.)"""
+    import atmlgraphattentionnetworks_amd as gat
+    from atmlgraphattentionnetworks_amd import _lib, sequence
+    monkeypatch.setattr(sequence, "_need_tensor", lambda what, name, t, dtypes=None: t)
+    monkeypatch.setattr(sequence, "_stream", lambda device: 0)
+
+    def broad(*shape, dtype=torch.float16):
+        return torch.zeros(1, dtype=dtype).expand(*shape)
+    ids, ptr = torch.zeros(1, dtype=torch.int64), torch.tensor([0, 1])
+    for cols in (16385, (1 << 31) + 8, (1 << 32) + 8):
+        with pytest.raises(ValueError, match="columns"):
+            gat.layer_norm(broad(1, cols))
+    for cols, dtype in ((65535 * 512 + 1, torch.float16), (65535 * 256 + 1, torch.float32),
+                        ((1 << 31) + 8, torch.float16), ((1 << 32) + 8, torch.bfloat16)):
+        with pytest.raises(ValueError, match="columns"):
+            gat.embedding(ids, broad(2, cols, dtype=dtype))
+    for h, hk, d in ((32769, 1, 128), (40000, 40000, 128), (1 << 22, 1, 7)):
+        q, k = (broad(1, n, d, dtype=torch.bfloat16) for n in (h, hk))
+        with pytest.raises(ValueError, match="heads"):
+            gat.packed_attention(q, k, k, ptr)
+    # the library's own answers
+    lib = _lib.load()
+    for dt, n in ((_lib.GAT_F32, 256), (_lib.GAT_BF16, 512)):
+        for cols, want in ((65535 * n + 1, _lib.GAT_EINVAL), ((1 << 31) - 1, _lib.GAT_EINVAL),
+                           (65535 * n, _lib.GAT_OK)):
+            assert lib.gat_embedding(64, 1, 0, 64, cols, 4, cols, 1.0, 64, cols, dt, None) == want
+            if want:
+                assert lib.gat_embedding_grad(64, 1, 1, 64, cols, 4, cols, 1.0, -1, 64, cols, 64, 1 << 40,
+                                              dt, None) == want
+    many = 80_000_000  # sequences: more lanes than one launch has
+    assert lib.gat_packed_attention(64, 64, 16, 64, 32, 16, 64, 32, 16, 64, 64, 0, many, 8, 8, 4, 2, 16, 0.25, 1,
+                                    64, None, None, None, 0, 0, None) == _lib.GAT_EUNSUPPORTED
+    with pytest.raises(ValueError, match="80000000 sequences"):
+        sequence._attn_check(_lib.GAT_EUNSUPPORTED, many)
