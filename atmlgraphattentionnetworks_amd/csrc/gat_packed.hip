@@ -500,6 +500,18 @@ __device__ __forceinline__ void store_column(U* row, const typename Shape<T, DP>
         }
 }
 
+// Scores whose reference m is further than this from 0 (in log2) are subtracted before they
+// are scaled: the difference of near floats is exact, while m c is rounded, by 2^-14 here and
+// by more than exp2 holds beyond 2^31 (prompts 543 -> 546 us, single tokens 165 -> 166.5 us).
+constexpr float kFar = 1024.f;
+// The backward has the float32 lse alone, whose rounding is a factor of P: 2^(2^-13) for an lse
+// of 1024.  Where it could be 2^(1/2), the gradients are NaN, not numbers without a digit.
+constexpr float kFarthest = 4194304.f;
+__device__ __forceinline__ float lse_in_log2(float lse) {
+    const float l = lse * kLog2e;
+    return fabsf(l) > kFarthest && fabsf(l) < INFINITY ? NAN : l;
+}
+
 constexpr float kRescale = 8.f;  // log2 of how far p may pass 1 before the sums are rescaled
 
 // ---------------------------------------------------------------------------
@@ -599,7 +611,13 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kFwd))) void k_a
 #pragma unroll
             for (int d = 0; d < S::DT; ++d) acc[d] *= f;
         }
-        const float mc = m == -INFINITY ? 0.f : m * c;
+        float mc = m == -INFINITY ? 0.f : m * c;
+        if (__any(fabsf(mc) > kFar && m < INFINITY)) {
+            const float ref = m == -INFINITY ? 0.f : m;
+            mc = 0.f;
+#pragma unroll
+            for (int j = 0; j < R; ++j) s[j] -= ref;
+        }
 #pragma unroll
         for (int j = 0; j < R; ++j) {
 #pragma unroll
@@ -805,7 +823,7 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDq))) void k_at
     add_delta(static_cast<const T*>(a.o.p) + tok * a.o.row + (long long)head * a.o.head);
     delta = parts_sum<W>(delta);
     if (mine && part == 0 && blockIdx.z == 0) a.delta[qh] = delta;
-    const float lse2 = mine ? a.lse[qh] * kLog2e : 0.f;
+    const float lse2 = mine ? lse_in_log2(a.lse[qh]) : 0.f;
     const T* kb = static_cast<const T*>(a.k.p) + (long long)k0 * a.k.row + (long long)kh * a.k.head;
     const T* vb = static_cast<const T*>(a.v.p) + (long long)k0 * a.v.row + (long long)kh * a.v.head;
     auto k_at = [&](int row) { return kb + (long long)row * a.k.row; };
@@ -971,7 +989,7 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_a
             const int i = in ? div_group(a, row) : 0;
             const long long qh =
                 in ? ((long long)(q0 + i) * a.kv_heads + kh) * a.group + (row - i * a.group) : 0;
-            rl[j] = in ? a.lse[qh] * kLog2e : INFINITY;  // exp(s - inf) = 0 behind the last row
+            rl[j] = in ? lse_in_log2(a.lse[qh]) : INFINITY;  // exp(s - inf) = 0 behind the last row
             rd[j] = in ? a.delta[qh] : 0.f;
         }
     };

@@ -410,7 +410,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     accumulators are float32; in bfloat16 the probabilities and the scores' gradients are
     rounded to bfloat16 for the second matrix product (not where a sequence's queries
     times the query heads of a key head are 32 or fewer on average, and not for ``q``'s
-    gradient with ``dim`` up to 32).  Inputs may be strided views (16-byte aligned rows are
+    gradient with ``dim`` up to 32).  The backward forms the probabilities again from the
+    float32 ``lse``, whose rounding is a relative error of about ``|lse| * 2^-23``; rows
+    where that leaves no digit (``|lse|`` over 2.9 million) make their gradients NaN.  Inputs may be strided views (16-byte aligned rows are
     read in place, others are copied)."""
     refuse_recording("packed_attention")
     kinds = (torch.float32, torch.bfloat16)

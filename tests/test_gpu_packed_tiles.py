@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_packed_attention import BOTH, attend, close, definition, offsets, tensors
+from test_gpu_packed_attention import BOTH, U, attend, close, definition, offsets, tensors
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda")
@@ -195,3 +195,78 @@ def test_four_waves_with_infinities_that_the_mask_hides(t):
     rest = [i for i in range(n) if i not in set(first)]
     for j in (0, 1, 2, 3):
         assert torch.equal(got[j][rest], want[j][rest]), j
+
+
+FAR = [(torch.float32, 8, 2, 2), (torch.float32, 16, 3, 1), (torch.float32, 32, 2, 1), (torch.float32, 128, 2, 2),
+       (torch.bfloat16, 16, 2, 2), (torch.bfloat16, 64, 6, 2), (torch.bfloat16, 128, 2, 1)]
+
+
+def far_inputs(nq, nk, h, hk, d, t, root):
+    """Scores of `root`^2 + 0 .. 5, which float32 holds exactly, and the inputs of the same
+    softmax without the offset."""
+    q, k, v = tensors(nq, nk, h, hk, d, t)
+    q.zero_()
+    q[..., 1] = 1
+    k[..., 1] = torch.randint(0, 6, k.shape[:2], device=DEV).to(t)
+    k[..., 0] = 0
+    qf, kf = q.clone(), k.clone()
+    qf[..., 0], kf[..., 0] = abs(root), root
+    return q, k, v, qf, kf
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("t,d,h,hk", FAR, ids=str)
+@pytest.mark.parametrize("lens,kl", [([200, 1, 33, 0, 64], None), ([1300], None), ([1, 1, 2], [3000, 70, 900])],
+                         ids=str)
+def test_scores_far_from_zero(lens, kl, t, d, h, hk, causal):
+    """The softmax goes by differences of scores: a common offset of up to 2^22 does not change
+    the output.  The gradients go by the float32 lse: with the error of its rounding up to
+    where that leaves nothing, and NaN from there on."""
+    kl = lens if kl is None else kl
+    nq, nk = sum(lens), sum(kl)
+    ptr, kv = (torch.tensor(offsets(x), dtype=torch.int32, device=DEV) for x in (lens, kl))
+    g = torch.randn(nq, h, d, device=DEV).to(t)
+    for root in (64.0, 1024.0, -1024.0, 2048.0):
+        q, k, v, qf, kf = far_inputs(nq, nk, h, hk, d, t, root)
+        (wy, ey), (wl, el), _, _, _ = definition(q, k, v, g, offsets(lens), offsets(kl), causal, 1.0)
+        leaves = [x.requires_grad_() for x in (qf, kf, v)]
+        y, lse = attend(*leaves, ptr, kv, causal=causal, scale=1.0, return_lse=True)
+        off = root * abs(root)
+        close(y, wy, ey, t, (root, "y"))
+        close(lse, wl + off, el + 4 * U * abs(off), torch.float32, (root, "lse"))
+        grads = torch.autograd.grad(y, leaves, g)
+        if abs(off) <= 4096:  # the offset is part of the bounds: 4 U |lse|
+            want = definition(qf, kf, v, g, offsets(lens), offsets(kl), causal, 1.0)[2:]
+            for name, a, (b, e) in zip(("dq", "dk", "dv"), grads, want):
+                close(a, b, e, t, (root, name))
+        if off > 1 << 21:
+            seen = (lse > -math.inf).cpu()
+            assert bool(grads[0].cpu()[seen].isnan().all())
+
+
+@pytest.mark.parametrize("t,d,h,hk", FAR, ids=str)
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 31, 2.0 ** 58])
+def test_scores_of_any_size(size, t, d, h, hk):
+    """Scores up to float32's range, each key's far above the one before: all of a query's
+    weight is on its last key, exactly; and equal scores, however large, share it."""
+    n = 150
+    q, k, v = tensors(n, n, h, hk, d, t)
+    g = torch.randn(n, h, d, device=DEV).to(t)
+    ptr = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    q.zero_()
+    q[..., 0] = size
+    for sign in (1.0, -1.0):
+        k[..., 0] = sign * size * (torch.arange(n, device=DEV)[:, None] + 1)
+        y = attend(q, k, v, ptr, causal=True)
+        each = v if sign > 0 else v[:1].expand(n, hk, d)
+        assert torch.equal(y, each.repeat_interleave(h // hk, 1))
+    k[..., 0] = torch.where(torch.arange(n, device=DEV)[:, None] % 2 == 0, size, -size)
+    y = attend(q, k, v, ptr)
+    even = v[::2].double().mean(0).cpu()
+    hp = 0.0 if t == torch.float32 else torch.finfo(t).eps / 2
+    e = (4 * n * U + 2 * hp) * v[::2].double().abs().mean(0).cpu()
+    even, e = (x.repeat_interleave(h // hk, 0).expand(n, h, d) for x in (even, e))
+    close(y, even, e, t, (size, "mean"))
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    for x in torch.autograd.grad(attend(*leaves, ptr), leaves, g):  # beyond the lse's digits
+        assert bool(x.isnan().all())
