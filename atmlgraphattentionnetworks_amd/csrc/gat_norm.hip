@@ -27,7 +27,9 @@
 //
 // Measured: 32,768 x 2,048 bf16 forward 46.5 us (5.8 TB/s), a training step 140 us (537 MB,
 // 3.8 TB/s); 400,000 x 64 bf16 forward 17.8 us (5.8 TB/s); 10,007 x 1,433 fp16 forward 21 us
-// (2.7 TB/s: one workgroup a row, a row's two exchanges are not covered).
+// (2.7 TB/s: one workgroup a row, a row's two exchanges are not covered).  Above 8,192 columns
+// the backward's 8 or 16 vectors a lane do not fit its registers (600 to 700 bytes of scratch a
+// lane): 4,096 x 16,384 bf16, a training step, 340 us (537 MB, 1.6 TB/s).
 
 #include "gat_seq.h"
 

@@ -31,12 +31,11 @@
 //
 // Bound: matrix products where sequences are long, the keys' and values' bytes where queries
 // are few, softmax arithmetic and latency where heads are narrow and sequences short.
-// Measured: prompts of 300 to 6,000 tokens, 16 heads of 128 over 4, bf16, causal: 544 us (970
-// TFLOP/s); 8 sequences of 2,048 with the backward: 1,070 us; one query for each of 48
-// sequences of up to 8,192, 32 heads of 128 over 8: 164 us (4.4 TB/s); 512 graphs of 85 to 150
-// nodes, 8 heads of 8, float32, with the backward: 276 us.
-
-#include <climits>
+// Measured, by box: prompts of 300 to 6,000 tokens, 16 heads of 128 over 4, bf16, causal:
+// 546-557 us (970-950 TFLOP/s; the softmax arithmetic of its 10^9 scores takes as long as the
+// products); 8 sequences of 2,048 with the backward: 1,085 us; one query for each of 48 sequences
+// of up to 8,192, 32 heads of 128 over 8: 166 us (4.3 TB/s); 512 graphs of 85 to 150 nodes, 8
+// heads of 8, float32, with the backward: 279 us.
 
 #include "gat_seq.h"
 
@@ -127,8 +126,10 @@ __device__ __forceinline__ Tile tile_of(const void* ptr, const void* other, int 
 // evenly among the XCDs, an XCD gets workgroups of one head (or of heads of its own), so that
 // the rows they stream are read into one L2 or few, not into all (causal prompts of 300 to
 // 6000 tokens, 4 key heads of 128: 602 us plainly, 571 us so; a packed training batch, heads
-// of 64: 305 us and 268 us).  Single waves stream rows that no other workgroup reads: 164.3 us
-// plainly, 165.6 us so, for one query each of 48 sequences.
+// of 64: 305 us and 268 us).  Narrow heads, whose rows are a part of a line: 8 heads of 8 over 512
+// graphs, training, 281 us plainly and 279 us so in float32, 224 us either way in bf16; 8 heads
+// of 32 in bf16 lose, 290 us plainly and 297 us so.  Single waves stream rows that no other
+// workgroup reads: 164.3 us plainly, 165.6 us so, for one query each of 48 sequences.
 struct Place {
     int slot, kh;
 };
@@ -207,7 +208,12 @@ enum AttnPass { kFwd, kDq, kDkv };
 // (graphs of 85 to 150 nodes, 8 heads of 8, float32, one training step: 300 us with what the
 // compiler takes, 278 us with these).  bf16 heads over 64: dq too (8 sequences of 2048, 16 heads
 // of 128 over 4, causal, one training step: 1215 us with one wave, 1087 us with two); dk and
-// dv, whose two accumulators are 128 registers, spill under two (1645 us).
+// dv, whose two accumulators are 128 registers there, spill under two (1645 us).  Heads of 64
+// spill 116-132 bytes a lane in dk and dv under two, heads of 128 28 (bf16) and 80 (float32) in
+// the forward.
+// Single-wave workgroups have row tiles of their own in LDS: those of narrow float32 heads are
+// resident three or four times a SIMD, not six, and float32 heads over 32 once; the compiler
+// says so of each.
 template <typename T, int DP>
 constexpr int waves_per_simd(AttnPass pass) {
     if (Shape<T, DP>::W == 16) return pass == kDkv ? 4 : 6;
@@ -552,7 +558,6 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kFwd))) void k_a
     const int qi = div_group(a, rc), gi = rc - qi * a.group;
     const int head = kh * a.group + gi;
     const int lim = limit(rc);
-    const int lim_first = uniform(limit(r0 < rows ? r0 : rows - 1));  // the wave's smallest
     const int lim_last = uniform(r0 < rows ? limit(r0 + W - 1 < rows ? r0 + W - 1 : rows - 1) : 0);
     const int last = t.index * BM + BM - 1;
     const int lim_block = uniform(limit(last < rows ? last : rows - 1));
@@ -626,9 +631,11 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kFwd))) void k_a
                 l += s[j][i];
             }
             // Single waves wait for memory, not for products: what rounding p leaves goes in too
-            // (one query each of 48 sequences: y off by 1.66e-3 of its norm, its own rounding,
-            // for 2.2e-3; 164 us for 162).  Graphs of 85 to 150 nodes, 8 heads of 32: 73 us for
-            // 66, so not there.
+            // (one query each of 48 sequences: y off by 1.64e-3 of its norm, its own rounding,
+            // for 2.2e-3; 164 us for 162).  Elsewhere p is rounded once, which leaves y off by
+            // 2.1e-3, because the second product would cost more than its rounding is worth:
+            // prompts 735 us for 544, 12 sequences with heads of 64, training, 260 us for 246,
+            // graphs with 8 heads of 32 73 us for 66 (forward), with 8 heads of 8 228 us for 220.
             add_products<DP, NW == 1>(acc, lv + S::slab(ROWS * j), s[j]);
             if (MASK && mend) {
                 unsigned seen = 0;
@@ -788,7 +795,6 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDq))) void k_at
     const int qi = div_group(a, rc), gi = rc - qi * a.group;
     const int head = kh * a.group + gi;
     const int lim = limit(rc);
-    const int lim_first = uniform(limit(r0 < rows ? r0 : rows - 1));  // the wave's smallest
     const int lim_last = uniform(r0 < rows ? limit(r0 + W - 1 < rows ? r0 + W - 1 : rows - 1) : 0);
     const int last = t.index * BM + BM - 1;
     const int lim_block = uniform(limit(last < rows ? last : rows - 1));
@@ -866,7 +872,8 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDq))) void k_at
             // Narrow heads are bound by latency, not by products: what rounding dS leaves goes
             // in too (512 graphs of 85 to 150 nodes, 8 heads of 8, training: dq off by 1.8e-3
             // of its norm, of which 1.7e-3 its own rounding, for 2.6e-3; 220 us for 215).
-            // Wider ones round it once (12 sequences, heads of 64: 255 us, 268 us so; 2.4e-3).
+            // Wider ones round it once, dq off by 2.4e-3 (1.7e-3 with both halves; 12 sequences,
+            // heads of 64: 259 us for 246, heads of 128: 1126 us for 1074).
             add_products<DP, DP <= 32>(acc, lk + S::slab(ROWS * j), s[j]);
             if (MASK && mend) {
                 unsigned seen = 0;
@@ -1035,6 +1042,11 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_a
         }
 #pragma unroll
         for (int j = 0; j < R; ++j) {
+            // P and dS are rounded to g's and q's type here: dk off by 2.4e-3 of its norm and dv by
+            // 2.3e-3, their own rounding 1.7e-3 of it.  Both halves would leave just that, for
+            // 283 us instead of 246 (12 sequences, heads of 64, training), 1156 instead of 1074
+            // (heads of 128) and 237 instead of 220 (graphs, 8 heads of 8): two more products
+            // a tile, not one as in dq.
             add_products<DP>(dv, lg + S::slab(ROWS * j), p[j]);
             add_products<DP>(dk, lq + S::slab(ROWS * j), ds[j]);
             if (MASK && mend) {
@@ -1104,7 +1116,9 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_a
 // ---------------------------------------------------------------------------
 
 // A launch's waves per workgroup and its splits of the streamed axis, from the average
-// lengths (the lengths themselves are on the device).
+// lengths (the lengths themselves are on the device).  One sequence far longer than the rest of a
+// large batch is therefore streamed by as few waves as the others: of a thousand single queries,
+// 999 over ten keys and one over 100,000, the long one is one wave's.
 struct Plan {
     int waves, splits;
 };

@@ -242,7 +242,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
               padding_idx: Optional[int] = None) -> torch.Tensor:
     """``scale * weight[ids]``: ``ids`` int32 or int64 of any shape, ``weight``
     ``[vocab, C]``.  Differentiable in ``weight`` (a dense gradient, float32 sums over
-    each id's tokens in their order); tokens with ``padding_idx`` take no gradient, their
+    each id's tokens in a fixed order); tokens with ``padding_idx`` take no gradient, their
     rows are read like any other.
 
     An id outside ``[0, vocab)`` gives a row of NaN and takes no gradient: checking on the
@@ -396,7 +396,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     int32 or int64 device tensor of ``count + 1`` offsets (a batch of graphs:
     ``GraphData.ptr()``), ``kv_ptr`` defaults to it.  One query per sequence (a readout
     over a graph's nodes, the next token of a text) is the same call with
-    ``ptr = arange(count + 1)``; a few queries over many keys are split over the keys.
+    ``ptr = arange(count + 1)``; a few queries over many keys are split over the keys, by the
+    average lengths (one sequence far longer than all others of a large batch is not).
 
     ``causal``: the last query sees all keys of its sequence, each earlier one a key less
     (key ``j`` is visible to query ``i`` iff ``j <= i + keys - queries``).  ``scale``
@@ -407,10 +408,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     Returns the output ``[queries, heads, dim]``, with ``return_lse`` also the float32
     ``[queries, heads]`` logarithm of each softmax sum (-inf where no key is seen; not
     differentiable).  Differentiable in ``q``, ``k`` and ``v``.  Scores, softmax sums and
-    accumulators are float32; in bfloat16 the probabilities and the scores' gradients are
-    rounded to bfloat16 for the second matrix product (not where a sequence's queries
-    times the query heads of a key head are 32 or fewer on average, and not for ``q``'s
-    gradient with ``dim`` up to 32).  The backward forms the probabilities again from the
+    accumulators are float32.  In bfloat16 a matrix product's second operand is rounded to
+    bfloat16: the probabilities in the forward (not where a sequence's queries times the
+    query heads of a key head are 32 or fewer on average), probabilities and scores'
+    gradients in the backward (not for ``q``'s gradient with ``dim`` up to 32); a call that
+    records gradients keeps a second tensor of the output's size beside it.
+    The backward forms the probabilities again from the
     float32 ``lse``, whose rounding is a relative error of about ``|lse| * 2^-23``; rows
     where that leaves no digit (``|lse|`` over 2.9 million) make their gradients NaN.  Inputs may be strided views (16-byte aligned rows are
     read in place, others are copied)."""
