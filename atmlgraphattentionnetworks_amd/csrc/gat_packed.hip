@@ -32,10 +32,10 @@
 // Bound: matrix products where sequences are long, the keys' and values' bytes where queries
 // are few, softmax arithmetic and latency where heads are narrow and sequences short.
 // Measured, by box: prompts of 300 to 6,000 tokens, 16 heads of 128 over 4, bf16, causal:
-// 546-557 us (970-950 TFLOP/s; the softmax arithmetic of its 10^9 scores takes as long as the
-// products); 8 sequences of 2,048 with the backward: 1,085 us; one query for each of 48 sequences
-// of up to 8,192, 32 heads of 128 over 8: 166 us (4.3 TB/s); 512 graphs of 85 to 150 nodes, 8
-// heads of 8, float32, with the backward: 279 us.
+// 546-584 us (967-905 TFLOP/s; the softmax arithmetic of its 10^9 scores takes as long as the
+// products); 8 sequences of 2,048 with the backward: 1,081-1,106 us; one query for each of 48
+// sequences of up to 8,192, 32 heads of 128 over 8: 165 us (4.6 TB/s); 512 graphs of 85 to 150
+// nodes, 8 heads of 8, float32, with the backward: 279 us.
 
 #include "gat_seq.h"
 
@@ -180,9 +180,11 @@ struct Shape {
     }
     // A tile of `rows` in LDS, rows without gaps (as the loads to LDS write them).  Vector c
     // of row r lies at place c ^ turn(r), so that what LDS serves in one cycle, 256 bytes,
-    // meets all 64 banks: one vector of 16 rows (the scores' reads), four of 4 rows (the
-    // transposing reads).  With 8-row turns, two rows a bank: 2.6 more cycles a read.  The
-    // last tile of the head dimension may read past DP, into what follows.
+    // meets all 64 banks: one vector of 16 rows (the scores' reads), four of 4 rows (bf16's
+    // transposing reads; counted in bf16: no conflict.  float32 reads X one element a lane:
+    // heads of 8 conflict in 42 to 48% of the LDS cycles).  With 8-row turns, two rows a bank:
+    // 2.6 more cycles a read.  The last tile of the head dimension may read past DP, into what
+    // follows.
     static constexpr int slab(int rows) { return rows * DP; }
     static constexpr int kSlack = 32;
     static __device__ __forceinline__ int turn(int r) {

@@ -10,7 +10,8 @@ tensor that carries a forward-mode tangent raises ``NotImplementedError``.
 ``torch.jit.trace`` keeps a call as one opaque function; ``make_fx`` could not, and is
 refused (``RuntimeError``).  Work is enqueued on torch's current stream of the tensors'
 device, nothing synchronises the host, and every workspace comes from torch's allocator
-within the call, so calls can be captured in HIP graphs.  Results do not depend on timing: no kernel adds floats with atomics.
+within the call, so calls can be captured in HIP graphs.  Results do not depend on timing:
+no kernel adds floats with atomics.
 
 When a step is captured in a graph, keep no autograd graph of an eager step on the same
 leaves alive (detach what is kept of the warm-up steps): its gradient accumulators
@@ -412,11 +413,11 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     bfloat16: the probabilities in the forward (not where a sequence's queries times the
     query heads of a key head are 32 or fewer on average), probabilities and scores'
     gradients in the backward (not for ``q``'s gradient with ``dim`` up to 32); a call that
-    records gradients keeps a second tensor of the output's size beside it.
-    The backward forms the probabilities again from the
-    float32 ``lse``, whose rounding is a relative error of about ``|lse| * 2^-23``; rows
-    where that leaves no digit (``|lse|`` over 2.9 million) make their gradients NaN.  Inputs may be strided views (16-byte aligned rows are
-    read in place, others are copied)."""
+    records gradients keeps a second tensor of the output's size beside it.  The backward
+    forms the probabilities again from the float32 ``lse``, whose rounding is a relative
+    error of about ``|lse| * 2^-23``; rows where that leaves no digit (``|lse|`` over 2.9
+    million) make their gradients NaN.  Inputs may be strided views (16-byte aligned rows
+    are read in place, others are copied)."""
     refuse_recording("packed_attention")
     kinds = (torch.float32, torch.bfloat16)
     for name, t in (("q", q), ("k", k), ("v", v)):
