@@ -513,11 +513,11 @@ __device__ __forceinline__ void store_column(U* row, const typename Shape<T, DP>
 // by more than exp2 holds beyond 2^31 (prompts 543 -> 546 us, single tokens 165 -> 166.5 us).
 constexpr float kFar = 1024.f;
 // The backward has the float32 lse alone, whose rounding is a factor of P: 2^(2^-13) for an lse
-// of 1024.  Where it could be 2^(1/2), the gradients are NaN, not numbers without a digit.
+// of 1024.  Where it could be 2^(1/2), a row without a gradient is left out (P = 0) and any
+// other makes its gradients NaN, not numbers without a digit.
 constexpr float kFarthest = 4194304.f;
-__device__ __forceinline__ float lse_in_log2(float lse) {
-    const float l = lse * kLog2e;
-    return fabsf(l) > kFarthest && fabsf(l) < INFINITY ? NAN : l;
+__device__ __forceinline__ bool beyond_lse(float lse2) {
+    return fabsf(lse2) > kFarthest && fabsf(lse2) < INFINITY;
 }
 
 constexpr float kRescale = 8.f;  // log2 of how far p may pass 1 before the sums are rescaled
@@ -830,8 +830,17 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDq))) void k_at
     if (sizeof(T) == 2 && a.low != nullptr) add_delta(static_cast<const T*>(a.low) + qh * a.dim);
     add_delta(static_cast<const T*>(a.o.p) + tok * a.o.row + (long long)head * a.o.head);
     delta = parts_sum<W>(delta);
+    float lse2 = mine ? a.lse[qh] * kLog2e : 0.f, some = 0.f;
+#pragma unroll
+    for (int s = 0; s < S::STEPS; ++s)
+#pragma unroll
+        for (int e = 0; e < S::FN; ++e) some = fmaxf(some, fabsf((float)gc[s][e]));
+    some = parts_max<W>(some);
+    if (beyond_lse(lse2)) {
+        lse2 = INFINITY;
+        if (some > 0.f) delta = NAN;
+    }
     if (mine && part == 0 && blockIdx.z == 0) a.delta[qh] = delta;
-    const float lse2 = mine ? lse_in_log2(a.lse[qh]) : 0.f;
     const T* kb = static_cast<const T*>(a.k.p) + (long long)k0 * a.k.row + (long long)kh * a.k.head;
     const T* vb = static_cast<const T*>(a.v.p) + (long long)k0 * a.v.row + (long long)kh * a.v.head;
     auto k_at = [&](int row) { return kb + (long long)row * a.k.row; };
@@ -987,7 +996,7 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_a
         const int i = div_group(a, row);
         return gb + (long long)i * a.g.row + (long long)(row - i * a.group) * a.g.head;
     };
-    // lse (in log2) and delta of a row tile
+    // lse and delta of a row tile
     constexpr int NT = NW * kWave, PER = (BN + NT - 1) / NT;
     float rl[PER], rd[PER];
     auto load_sums = [&](int n0) {
@@ -998,7 +1007,7 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_a
             const int i = in ? div_group(a, row) : 0;
             const long long qh =
                 in ? ((long long)(q0 + i) * a.kv_heads + kh) * a.group + (row - i * a.group) : 0;
-            rl[j] = in ? lse_in_log2(a.lse[qh]) : INFINITY;  // exp(s - inf) = 0 behind the last row
+            rl[j] = in ? a.lse[qh] : INFINITY;  // exp(s - inf) = 0 behind the last row
             rd[j] = in ? a.delta[qh] : 0.f;
         }
     };
@@ -1066,7 +1075,9 @@ __global__ __launch_bounds__(NW * kWave, (waves_per_simd<T, DP>(kDkv))) void k_a
 #pragma unroll
         for (int j = 0; j < PER; ++j)
             if (j * NT + threadIdx.x < BN) {
-                sums[turn * 2 * BN + j * NT + threadIdx.x] = rl[j];
+                const float l = rl[j] * kLog2e;
+                sums[turn * 2 * BN + j * NT + threadIdx.x] =
+                    beyond_lse(l) ? rd[j] == 0.f ? INFINITY : NAN : l;
                 sums[(turn * 2 + 1) * BN + j * NT + threadIdx.x] = rd[j];
             }
         wait_loads();

@@ -416,8 +416,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     records gradients keeps a second tensor of the output's size beside it.  The backward
     forms the probabilities again from the float32 ``lse``, whose rounding is a relative
     error of about ``|lse| * 2^-23``; rows where that leaves no digit (``|lse|`` over 2.9
-    million) make their gradients NaN.  Inputs may be strided views (16-byte aligned rows
-    are read in place, others are copied)."""
+    million) make their gradients NaN, unless the output's gradient is 0 there.  Inputs may
+    be strided views (16-byte aligned rows are read in place, others are copied)."""
     refuse_recording("packed_attention")
     kinds = (torch.float32, torch.bfloat16)
     for name, t in (("q", q), ("k", k), ("v", v)):

@@ -678,7 +678,8 @@ int gat_packed_attention(const void* q, long long q_row, long long q_head, const
  * q's); out, low (or NULL) and lse as the forward stored them.  dq [nq, heads, dim], dk, dv
  * [nk, kv_heads, dim] contiguous; dk and dv are sums over the query heads of a key head.
  * Rows outside all sequences get zeros.  Deterministic.  The probabilities are formed from lse:
- * rows with |lse| over 2^22 / log2(e), where its rounding leaves them no digit, give NaN.
+ * rows with |lse| over 2^22 / log2(e), where its rounding leaves them no digit, give NaN, or
+ * nothing where g is 0.
  */
 int gat_packed_attention_backward_workspace_size(int nq, int nk, int count, int heads, int kv_heads,
                                                  int dim, int dtype, size_t* bytes);

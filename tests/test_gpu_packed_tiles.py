@@ -270,3 +270,36 @@ def test_scores_of_any_size(size, t, d, h, hk):
     leaves = [x.detach().requires_grad_() for x in (q, k, v)]
     for x in torch.autograd.grad(attend(*leaves, ptr), leaves, g):  # beyond the lse's digits
         assert bool(x.isnan().all())
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("t,d,h,hk", FAR, ids=str)
+@pytest.mark.parametrize("size", [1e7, 1e9, 1e30])
+def test_far_rows_without_a_gradient(size, t, d, h, hk, causal):
+    """Queries all of whose scores are far below 0, as a padded row's are whose keys were put
+    out of reach, and whose output nothing uses: no gradient comes from them, as from any row
+    with g = 0, and those of the other rows are what they are."""
+    lens = [150, 33, 70]
+    n = sum(lens)
+    q, k, v = tensors(n, n, h, hk, d, t)
+    g = torch.randn(n, h, d, device=DEV).to(t)
+    k[..., 0] = 1
+    q[..., 0] = 0
+    far = [3, 17, 40, 41, 42, 149, 150, 199, n - 1]
+    q[far] = 0
+    q[far, :, 0] = -size
+    g[far] = 0
+    ptr = torch.tensor(offsets(lens), dtype=torch.int32, device=DEV)
+    want = definition(q, k, v, g, offsets(lens), offsets(lens), causal, d ** -0.5)[2:]
+    _, *got = run(q, k, v, g, ptr, causal=causal)
+    for name, a, (b, e) in zip(("dq", "dk", "dv"), got, want):
+        close(a, b, e, t, (size, name))
+    assert not got[0][far].any()
+    if size * d ** -0.5 * math.log2(math.e) < 1 << 22:
+        return
+    g[far[0], 0, d - 1] = 1  # one that is used: NaN, in its own sequence
+    _, *got = run(q, k, v, g, ptr, causal=causal)
+    assert bool(got[0][far[0], 0].isnan().all()) and bool(got[1][0, 0].isnan().all())
+    assert bool(got[2][0, 0].isnan().all())
+    for a, (b, e) in zip(got, want):
+        close(a[150:], b[150:], e[150:], t, (size, "other sequences"))
