@@ -33,9 +33,9 @@
 // are few, softmax arithmetic and latency where heads are narrow and sequences short.
 // Measured, by box: prompts of 300 to 6,000 tokens, 16 heads of 128 over 4, bf16, causal:
 // 546-584 us (967-905 TFLOP/s; the softmax arithmetic of its 10^9 scores takes as long as the
-// products); 8 sequences of 2,048 with the backward: 1,081-1,106 us; one query for each of 48
+// products); 8 sequences of 2,048 with the backward: 1,047-1,084 us; one query for each of 48
 // sequences of up to 8,192, 32 heads of 128 over 8: 165 us (4.6 TB/s); 512 graphs of 85 to 150
-// nodes, 8 heads of 8, float32, with the backward: 279 us.
+// nodes, 8 heads of 8, float32, with the backward: 277 us.
 
 #include "gat_seq.h"
 
