@@ -96,12 +96,14 @@ def _too_wide(cols: int) -> ValueError:
                       "/ float32 16381 where rows are not 16-byte aligned)")
 
 
-def _norm_forward(x2, w, b, eps, stats):
+def _norm_forward(x2, w, b, eps, stats, shape):
+    """``shape``: x's own.  The output has it from the start: a view made within an autograd
+    function could not be changed in place."""
     lib = _lib.load()
-    y = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device)
+    y = torch.empty(shape, dtype=x2.dtype, device=x2.device)
     with _on(x2.device):
         rc = lib.gat_layer_norm(x2.data_ptr(), x2.stride(0), x2.shape[0], x2.shape[1], _ptr(w),
-                                _ptr(b), eps, y.data_ptr(), y.stride(0), _ptr(stats),
+                                _ptr(b), eps, y.data_ptr(), x2.shape[1], _ptr(stats),
                                 _DTYPES[x2.dtype], _stream(x2.device))
     if rc == _lib.GAT_EUNSUPPORTED:
         raise _too_wide(x2.shape[1])
@@ -115,9 +117,9 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, w, b, eps):
         x2 = _rows(x)
         stats = torch.empty(x2.shape[0], 2, dtype=torch.float32, device=x.device)
-        y = _norm_forward(x2, w, b, eps, stats)
+        y = _norm_forward(x2, w, b, eps, stats, x.shape)
         ctx.save_for_backward(x2, w, stats)
-        return y if x.dim() == 2 else y.view(x.shape)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -169,7 +171,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     w, b = (None if p is None else p.contiguous() for p in (weight, bias))
     if _as_function(x, w, b):
         return _LayerNorm.apply(x, w, b, float(eps))
-    return _norm_forward(_rows(x), w, b, float(eps), None).view(x.shape)
+    return _norm_forward(_rows(x), w, b, float(eps), None, x.shape)
 
 
 class LayerNorm(torch.nn.Module):
@@ -202,15 +204,15 @@ def _embed_forward(ids, w, scale):
     ld = w.stride(0) if w.shape[0] > 1 else w.shape[1]  # one row: its stride says nothing
     if ld < w.shape[1]:  # a row repeated by expand()
         w, ld = w.contiguous(), w.shape[1]
-    out = torch.empty(ids.numel(), w.shape[1], dtype=w.dtype, device=w.device)
+    out = torch.empty(*ids.shape, w.shape[1], dtype=w.dtype, device=w.device)
     with _on(w.device):
         rc = _lib.load().gat_embedding(ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(),
                                        w.data_ptr(), ld, w.shape[0], w.shape[1], scale,
-                                       out.data_ptr(), out.stride(0), _DTYPES[w.dtype],
+                                       out.data_ptr(), w.shape[1], _DTYPES[w.dtype],
                                        _stream(w.device))
     if rc:
         _lib.check(rc, "gat_embedding")
-    return out.view(*ids.shape, w.shape[1])
+    return out
 
 
 class _Embedding(torch.autograd.Function):

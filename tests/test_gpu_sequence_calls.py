@@ -106,3 +106,27 @@ def test_layer_norm_in_place(cols, t):
                                           torch.cuda.current_stream().cuda_stream), "gat_layer_norm")
     torch.cuda.synchronize()
     assert torch.equal(x, want)
+
+
+def test_outputs_can_be_changed_in_place():
+    """As torch's own operators allow it: the output is no view, and not kept for the backward."""
+    import atmlgraphattentionnetworks_amd as gat
+    torch.manual_seed(2)
+    w = torch.rand(24, device=DEV)
+    table = torch.randn(30, 24, device=DEV, requires_grad=True)
+    for shape in ((24,), (5, 24), (2, 5, 24), (2, 3, 5, 24)):
+        x, g = torch.randn(*shape, device=DEV, requires_grad=True), torch.randn(*shape, device=DEV)
+        y = gat.layer_norm(x, w)
+        z = gat.layer_norm(x, w)
+        z += 1.0
+        z.mul_(2.0)
+        assert torch.equal(z, (y + 1.0) * 2.0), shape
+        a, b = torch.autograd.grad(z, x, g)[0], torch.autograd.grad(y, x, g * 2.0)[0]
+        assert torch.equal(a, b), shape
+        ids = torch.randint(0, 30, shape[:-1], device=DEV)
+        y, z = gat.embedding(ids, table), gat.embedding(ids, table)
+        z += 1.0
+        z.mul_(2.0)
+        assert torch.equal(z, (y + 1.0) * 2.0), shape
+        a, b = torch.autograd.grad(z, table, g)[0], torch.autograd.grad(y, table, g * 2.0)[0]
+        assert torch.equal(a, b), shape

@@ -182,7 +182,7 @@ def test_tracing_keeps_the_calls_as_functions(monkeypatch):
         ctypes.memmove(to.data_ptr(), value.contiguous().data_ptr(), to.numel() * to.element_size())
         return to
     monkeypatch.setattr(sequence, "_norm_forward",
-                        lambda x, w, b, eps, stats: fill(torch.empty(x.shape), x * 2))
+                        lambda x, w, b, eps, stats, shape: fill(torch.empty(shape), x * 2))
     monkeypatch.setattr(sequence, "_embed_forward",
                         lambda ids, w, scale: fill(torch.empty(*ids.shape, w.shape[1]), w[ids] * scale))
     monkeypatch.setattr(sequence, "_attn_forward",
