@@ -414,8 +414,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: tor
     accumulators are float32.  In bfloat16 a matrix product's second operand is rounded to
     bfloat16: the probabilities in the forward (not where a sequence's queries times the
     query heads of a key head are 32 or fewer on average), probabilities and scores'
-    gradients in the backward (not for ``q``'s gradient with ``dim`` up to 32); a call that
-    records gradients keeps a second tensor of the output's size beside it.  The backward
+    gradients in the backward (not for ``q``'s gradient with ``dim`` up to 32).  A call that
+    records gradients keeps its output (which is therefore not to be changed in place) and,
+    in bfloat16, a second tensor of the output's size.  The backward
     forms the probabilities again from the float32 ``lse``, whose rounding is a relative
     error of about ``|lse| * 2^-23``; rows where that leaves no digit (``|lse|`` over 2.9
     million) make their gradients NaN, unless the output's gradient is 0 there.  Inputs may
